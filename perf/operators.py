@@ -20,29 +20,29 @@ UNIT = float(2 ** 30)  # fixed-point unit of a token's weight
 def listed():
     return [
         # acting: one environment's observation through the gated block of a 512-wide trunk
-        dict(name="gated fwd, one row", op="gated", backward=False, rows=1, features=512, hidden=2048, dtype="bf16", act="silu"),
+        dict(name="gated fwd one row", op="gated", backward=False, rows=1, features=512, hidden=2048, dtype="bf16", act="silu"),
         # acting: a few dozen environments, a wider trunk; the weights are most of what is read
-        dict(name="gated fwd, 48 rows", op="gated", backward=False, rows=48, features=2048, hidden=8192, dtype="fp16", act="gelu"),
+        dict(name="gated fwd 48 rows", op="gated", backward=False, rows=48, features=2048, hidden=8192, dtype="fp16", act="gelu"),
         # a ragged minibatch of odd sizes (rows padded to 16 bytes, as operand planes are)
-        dict(name="gated fwd, ragged", op="gated", backward=False, rows=1777, features=523, hidden=1365, dtype="fp16", act="silu"),
+        dict(name="gated fwd ragged", op="gated", backward=False, rows=1777, features=523, hidden=1365, dtype="fp16", act="silu"),
         # the widest trunk of the repository (1024, times 4) over the rows of its largest batch (32768, both halves)
-        dict(name="gated fwd, 65536 rows", op="gated", backward=False, rows=65536, features=1024, hidden=4096, dtype="bf16", act="silu"),
+        dict(name="gated fwd 65536 rows", op="gated", backward=False, rows=65536, features=1024, hidden=4096, dtype="bf16", act="silu"),
         # training at the default batch (4096 transitions, both halves; 512-wide trunk, times 4)
-        dict(name="gated bwd, 8192 rows", op="gated", backward=True, rows=8192, features=512, hidden=2048, dtype="fp16", act="silu"),
+        dict(name="gated bwd 8192 rows", op="gated", backward=True, rows=8192, features=512, hidden=2048, dtype="fp16", act="silu"),
         # training at the widest trunk and half of the largest batch's rows
-        dict(name="gated bwd, 32768 rows", op="gated", backward=True, rows=32768, features=1024, hidden=4096, dtype="bf16", act="gelu"),
+        dict(name="gated bwd 32768 rows", op="gated", backward=True, rows=32768, features=1024, hidden=4096, dtype="bf16", act="gelu"),
         # a small head (the critic's 101 atoms) distilled from its teacher's eight best, fp32 as heads write it
-        dict(name="distill, 512 x 101", op="distill", rows=512, vocab=101, top=8, dtype="fp32", grad="fp32", temperature=1.0, masked=False),
+        dict(name="distill 512 x 101", op="distill", rows=512, vocab=101, top=8, dtype="fp32", grad="fp32", temperature=1.0, masked=False),
         # a generic 32k vocabulary, fp32 logits, fp16 gradient for the next product, invalid tokens masked by -inf
-        dict(name="distill, 2048 x 32768", op="distill", rows=2048, vocab=32768, top=64, dtype="fp32", grad="fp16", temperature=2.0, masked=True),
+        dict(name="distill 2048 x 32768", op="distill", rows=2048, vocab=32768, top=64, dtype="fp32", grad="fp16", temperature=2.0, masked=True),
         # a large vocabulary of odd size: rows start at any element
-        dict(name="distill, 2047 x 128257", op="distill", rows=2047, vocab=128257, top=128, dtype="bf16", grad="bf16", temperature=1.0, masked=False),
+        dict(name="distill 2047 x 128257", op="distill", rows=2047, vocab=128257, top=128, dtype="bf16", grad="bf16", temperature=1.0, masked=False),
         # acting: 4096 environments, 256 action bins, nucleus only
-        dict(name="sample, 4096 x 256", op="sample", rows=4096, vocab=256, dtype="fp32", temperature=1.0, top_k=0, top_p=0.95, min_p=0.0, masked=True),
+        dict(name="sample 4096 x 256", op="sample", rows=4096, vocab=256, dtype="fp32", temperature=1.0, top_k=0, top_p=0.95, min_p=0.0, masked=True),
         # one request, large vocabulary: latency
-        dict(name="sample, 1 x 128257", op="sample", rows=1, vocab=128257, dtype="fp32", temperature=0.8, top_k=50, top_p=0.95, min_p=0.0, masked=False),
+        dict(name="sample 1 x 128257", op="sample", rows=1, vocab=128257, dtype="fp32", temperature=0.8, top_k=50, top_p=0.95, min_p=0.0, masked=False),
         # a full batch of requests with every filter on
-        dict(name="sample, 256 x 131072", op="sample", rows=256, vocab=131072, dtype="bf16", temperature=0.9, top_k=2000, top_p=0.9, min_p=0.001, masked=False),
+        dict(name="sample 256 x 131072", op="sample", rows=256, vocab=131072, dtype="bf16", temperature=0.9, top_k=2000, top_p=0.9, min_p=0.001, masked=False),
     ]
 
 
