@@ -852,6 +852,71 @@ int rl2_peer_reduce(const rl2_peer_reduce_args* args, const rl2_syncbn_exchange*
 long long rl2_peer_mean_flag_bytes(int world);
 int rl2_peer_mean(long long count, const rl2_syncbn_exchange* ex, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * gated feed-forward block (no counterpart in the reference, whose residual blocks are
+ * src/robolearn/flashsac/layers.py:189-240): h = act(x Wg^T) * (x Wu^T) in one kernel,
+ * and its backward pass. x [rows][features], Wg and Wu [hidden][features], h
+ * [rows][hidden], all of one 16-bit type with fp32 accumulation and one rounding of each
+ * output. Rows contiguous; bases 16-byte aligned and row strides (in elements) multiples
+ * of 16 bytes, as operand planes are; any extents.
+ *
+ * A plan is for up to `rows` rows and belongs to the device that was current at its
+ * creation. dtype 0 = fp16, 1 = bf16; activation 0 = SiLU, 1 = GELU (the error-function
+ * form), 2 = ReLU.
+ *
+ * Backward, from x, the weights and grad_out (nothing kept from the forward: g and u are
+ * computed again): grad_x = dg Wg + du Wu, grad_gate = dg^T x, grad_up = du^T x with
+ * dg = grad_out u act'(g), du = grad_out act(g), rounded to the operand type once.
+ * grad_x may be null, and grad_gate with grad_up; gradients are assigned, not added.
+ * grad_weight_fp32: the weight gradients are fp32 (row strides in floats, multiples of
+ * 4). workspace: rl2_gated_workspace_bytes(plan) bytes, 256-byte aligned, free to use
+ * again after the call's work. rows = 0 is allowed (zero weight gradients).
+ * ------------------------------------------------------------------------- */
+typedef struct rl2_gated_desc {
+    int rows, features, hidden;
+    int dtype, activation;
+} rl2_gated_desc;
+
+typedef struct rl2_gated_forward_args {
+    int rows;
+    const void* x;
+    long long ldx;
+    const void* gate_weight;
+    long long ld_gate;
+    const void* up_weight;
+    long long ld_up;
+    void* out;
+    long long ld_out;
+    int* health;
+} rl2_gated_forward_args;
+
+typedef struct rl2_gated_backward_args {
+    int rows;
+    const void* x;
+    long long ldx;
+    const void* gate_weight;
+    long long ld_gate;
+    const void* up_weight;
+    long long ld_up;
+    const void* grad_out;
+    long long ld_grad_out;
+    void* grad_x;
+    long long ld_grad_x;
+    void* grad_gate;
+    long long ld_grad_gate;
+    void* grad_up;
+    long long ld_grad_up;
+    int grad_weight_fp32;
+    void* workspace;
+    int* health;
+} rl2_gated_backward_args;
+
+void* rl2_gated_create(const rl2_gated_desc* desc);
+int rl2_gated_destroy(void* plan);
+long long rl2_gated_workspace_bytes(void* plan);
+int rl2_gated_forward(void* plan, const rl2_gated_forward_args* args, void* stream);
+int rl2_gated_backward(void* plan, const rl2_gated_backward_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -396,3 +396,38 @@ SIGNATURES.update({
     "rl2_peer_mean": ([LL, ctypes.POINTER(SyncBNExchange), P], I),
     "rl2_peer_mean_flag_bytes": ([I], LL),
 })
+
+
+class GatedDesc(ctypes.Structure):
+    """``rl2_gated_desc`` (include/rl2.h)."""
+
+    _fields_ = [("rows", I), ("features", I), ("hidden", I), ("dtype", I), ("activation", I)]
+
+
+class GatedForwardArgs(ctypes.Structure):
+    """``rl2_gated_forward_args`` (include/rl2.h)."""
+
+    _fields_ = [
+        ("rows", I), ("x", P), ("ldx", LL), ("gate_weight", P), ("ld_gate", LL), ("up_weight", P), ("ld_up", LL),
+        ("out", P), ("ld_out", LL), ("health", P),
+    ]
+
+
+class GatedBackwardArgs(ctypes.Structure):
+    """``rl2_gated_backward_args`` (include/rl2.h)."""
+
+    _fields_ = [
+        ("rows", I), ("x", P), ("ldx", LL), ("gate_weight", P), ("ld_gate", LL), ("up_weight", P), ("ld_up", LL),
+        ("grad_out", P), ("ld_grad_out", LL), ("grad_x", P), ("ld_grad_x", LL), ("grad_gate", P),
+        ("ld_grad_gate", LL), ("grad_up", P), ("ld_grad_up", LL), ("grad_weight_fp32", I), ("workspace", P),
+        ("health", P),
+    ]
+
+
+SIGNATURES.update({
+    "rl2_gated_create": ([ctypes.POINTER(GatedDesc)], P),
+    "rl2_gated_destroy": ([P], I),
+    "rl2_gated_workspace_bytes": ([P], LL),
+    "rl2_gated_forward": ([P, ctypes.POINTER(GatedForwardArgs), P], I),
+    "rl2_gated_backward": ([P, ctypes.POINTER(GatedBackwardArgs), P], I),
+})

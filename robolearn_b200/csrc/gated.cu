@@ -1,0 +1,912 @@
+// Gated feed-forward block on tcgen05: h = act(x Wg^T) * (x Wu^T), and its backward pass.
+//
+//   forward     g = x Wg^T, u = x Wu^T, h = act(g) * u                      [M][F]
+//   backward    dg = dh * u * act'(g), du = dh * act(g)                     [M][F] each
+//               dx = dg Wg + du Wu                                          [M][K]
+//               dWg = dg^T x, dWu = du^T x                                  [F][K]
+//
+// x [M][K], Wg and Wu [F][K] (the layout of a linear layer's weight), fp16 or bf16 operands,
+// fp32 accumulation. g and u are never stored: the forward's epilogue consumes them from
+// TMEM, and the backward computes them again (2 of its 6 products; storing them in fp32 would
+// write and read 16 bytes per element of [M][F], which costs more than the two products up to
+// K = 1024 or so, and storing them rounded would add their rounding to every gradient). dg and
+// du are rounded once to the operand type: they are the operands of the last two products.
+//
+// One kernel, four modes. All run 256 x (2 BNC) tiles on CTA pairs (tcgen05 cta_group::2, M =
+// 256): each CTA stages its 128 rows of A and BNC rows of B per 64-deep k-block.
+//   kForward, kGate   the pair's B rows are BNC rows of Wg (even CTA) and the same BNC rows of
+//                     Wu (odd CTA), so one MMA makes both projections of BNC hidden units and
+//                     a TMEM lane holds g in columns [0, BNC) and u in [BNC, 2 BNC). kGate also
+//                     brings the tile's dh by TMA and stores dg and du.
+//   kInput            contraction over the 2F concatenated hidden units: A = [dg | du]
+//                     (K-major), B = [Wg ; Wu] read N-contiguous, no transposed copies.
+//   kWeight           contraction over the M rows: A = dg or du read M-contiguous, B = x read
+//                     N-contiguous; split over rows when the tiles do not fill the GPU.
+// Warp roles as in the dense products: TMA producer, MMA issuer, eight epilogue warps on a
+// double-buffered accumulator. Outputs leave through shared-memory boxes and TMA stores, which
+// clip at the output's extents. Every wait is bounded by wall-clock time.
+
+#include "common.cuh"
+#include "../../include/rl2.h"
+
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <cstring>
+#include <new>
+
+namespace rl2 {
+namespace gated {
+
+constexpr int kBM = 128;  // rows of A per CTA (256 per pair)
+constexpr int kBK = 64;   // 128 bytes of 16-bit operands
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kBoxBytes = 4096;  // 32 rows x 128 bytes
+constexpr int kMaxSmem = 232448;
+constexpr int kMaxStages = 8;
+
+enum Mode { kForward = 0, kGate = 1, kInput = 2, kWeight = 3 };
+enum Act { kSilu = 0, kGelu = 1, kRelu = 2 };
+
+struct Params {
+    int kblocks;        // k-blocks of the whole contraction
+    int kb_segment;     // kInput: k-blocks of one half (F / 64, rounded up)
+    int splits, kb_per_split;
+    int bnc;            // B rows staged per CTA
+    int tile_cols;      // output columns per tile: bnc (kForward, kGate) or 2 bnc
+    int tiles_n, tiles_m, tiles_z, tiles_total;
+    int stages;
+    int box_cols;       // columns per store box
+    int out_rows, out_cols;
+    int store_cols;     // columns that the store engine writes; the rest of a row (less than 16 bytes) by plain stores
+    void* out[2];       // kForward, kInput: out[0]; kWeight: by gate / up
+    long long ld_out[2];
+    int* health;
+};
+
+struct Maps {
+    CUtensorMap a, b0, b1, d0, d1, in;
+};
+
+// ---- small device helpers ---------------------------------------------------
+
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
+           (static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32) | (static_cast<uint64_t>(1) << 46) |
+           (static_cast<uint64_t>(2) << 61);  // descriptor version, 128-byte swizzle
+}
+
+// mbarrier wait bounded to 4 s; gives up early once another role raised the CTA's abort word
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, int* health, volatile int* abort_flag) {
+    if (ptx::mbar_try_wait(bar, phase)) return true;
+    uint64_t start, now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+    for (uint32_t i = 1;; ++i) {
+        if (ptx::mbar_try_wait(bar, phase)) return true;
+        if ((i & 1023u) == 0) {
+            if (abort_flag && *abort_flag) return false;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (now - start > 4000000000ull) {
+                if (health) atomicOr(health, kHealthTimeout);
+                if (abort_flag) *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if (BF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if (BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// act(g) and act'(g). The exponential and the division are the fast fp32 forms (a few units in
+// the last place of fp32): the result is rounded to 16 bits, 2^13 to 2^16 times coarser.
+template <int ACT>
+__device__ __forceinline__ float act_value(float g) {
+    if (ACT == kSilu) return __fdividef(g, 1.0f + __expf(-g));
+    if (ACT == kGelu) return 0.5f * g * (1.0f + erff(g * 0.70710678f));
+    return g > 0.0f ? g : (g == g ? 0.0f : g);
+}
+
+template <int ACT>
+__device__ __forceinline__ void act_both(float g, float& value, float& slope) {
+    if (ACT == kSilu) {
+        const float s = __fdividef(1.0f, 1.0f + __expf(-g));
+        value = g * s;
+        slope = s * (1.0f + g * (1.0f - s));
+    } else if (ACT == kGelu) {
+        const float cdf = 0.5f * (1.0f + erff(g * 0.70710678f));
+        value = g * cdf;
+        slope = cdf + g * 0.39894228f * __expf(-0.5f * g * g);
+    } else {
+        value = g > 0.0f ? g : (g == g ? 0.0f : g);
+        slope = g > 0.0f ? 1.0f : 0.0f;
+    }
+}
+
+struct Tile {
+    int n, m, z, split, kb0, kb1;
+};
+
+__device__ __forceinline__ Tile decode(const Params& p, int t) {
+    Tile w;
+    w.n = t % p.tiles_n;
+    t /= p.tiles_n;
+    w.m = t % p.tiles_m;
+    t /= p.tiles_m;
+    w.z = t % p.tiles_z;
+    w.split = t / p.tiles_z;
+    w.kb0 = w.split * p.kb_per_split;
+    w.kb1 = min(p.kblocks, w.kb0 + p.kb_per_split);
+    return w;
+}
+
+// ---- roles --------------------------------------------------------------------
+
+template <int MODE>
+__device__ __forceinline__ void produce(const Maps& maps, const Params& p, uint8_t* smem, uint32_t stage_bytes,
+                                        uint64_t* full, uint64_t* empty, volatile int* abort_flag) {
+    const int rank = static_cast<int>(blockIdx.x & 1u);
+    ptx::prefetch_tensormap(&maps.a);
+    ptx::prefetch_tensormap(&maps.b0);
+    int s = 0;
+    uint32_t phase = 0;
+    long long issued = 0;
+    bool ok = true;
+    for (int t = blockIdx.x >> 1; t < p.tiles_total && ok; t += gridDim.x >> 1) {
+        const Tile w = decode(p, t);
+        const int row0 = w.m * 2 * kBM + rank * kBM;
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+            if (!wait_bar(&empty[s], phase ^ 1, p.health, abort_flag)) {
+                ok = false;
+                break;
+            }
+            if (rank == 0) ptx::mbar_arrive_expect_tx(&full[s], 2 * stage_bytes);
+            ++issued;
+            const uint32_t bar = ptx::cluster_addr(&full[s], 0);
+            uint8_t* sa = smem + s * stage_bytes;
+            uint8_t* sb = sa + kBM * 128;
+            if (MODE == kForward || MODE == kGate) {
+                ptx::tma_load_3d_pair(sa, &maps.a, bar, kb * kBK, row0, 0);
+                ptx::tma_load_3d_pair(sb, rank == 0 ? &maps.b0 : &maps.b1, bar, kb * kBK, w.n * p.bnc, 0);
+            } else if (MODE == kInput) {
+                const int seg = kb >= p.kb_segment ? 1 : 0;
+                const int f0 = (kb - seg * p.kb_segment) * kBK;
+                const int n0 = w.n * p.tile_cols + rank * p.bnc;
+                ptx::tma_load_3d_pair(sa, &maps.a, bar, f0, row0, seg);
+                for (int c = 0; c < p.bnc / 64; ++c)
+                    ptx::tma_load_3d_pair(sb + c * (kBK * 128), seg ? &maps.b1 : &maps.b0, bar, n0 + c * 64, f0, 0);
+            } else {
+                const int n0 = w.n * p.tile_cols + rank * p.bnc;
+                for (int c = 0; c < kBM / 64; ++c)
+                    ptx::tma_load_3d_pair(sa + c * (kBK * 128), &maps.a, bar, row0 + c * 64, kb * kBK, w.z);
+                for (int c = 0; c < p.bnc / 64; ++c)
+                    ptx::tma_load_3d_pair(sb + c * (kBK * 128), &maps.b0, bar, n0 + c * 64, kb * kBK, 0);
+            }
+            if (++s == p.stages) {
+                s = 0;
+                phase ^= 1;
+            }
+        }
+    }
+    // Every armed stage has landed before the pair may exit, also after an abort (the even
+    // CTA's barriers count both CTAs' loads; the odd CTA leaves after the even one).
+    if (rank != 0) return;
+    for (int st = 0; st < p.stages; ++st) {
+        const long long armed = issued > st ? (issued - 1 - st) / p.stages + 1 : 0;
+        if (armed > 0) wait_bar(&full[st], static_cast<uint32_t>((armed - 1) & 1), p.health, nullptr);
+    }
+}
+
+// One thread of the even CTA issues every MMA of the pair.
+template <int MODE, bool BF16>
+__device__ __forceinline__ void issue(const Params& p, uint8_t* smem, uint32_t stage_bytes, uint64_t* full,
+                                      uint64_t* empty, uint64_t* acc_full, uint64_t* acc_empty, uint32_t tmem,
+                                      volatile int* abort_flag) {
+    constexpr uint32_t a_mn = MODE == kWeight ? 1u : 0u;
+    constexpr uint32_t b_mn = MODE == kWeight || MODE == kInput ? 1u : 0u;
+    constexpr uint32_t fmt = BF16 ? 1u : 0u;
+    const uint32_t n = 2u * p.bnc;
+    const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) |
+                           ((2u * kBM >> 4) << 24);
+    auto commit = [&](uint64_t* bar) {
+        ptx::mma_commit_pair(ptx::cluster_addr(bar, 0));
+        ptx::mma_commit_pair(ptx::cluster_addr(bar, 1));
+    };
+    int s = 0, i = 0;
+    uint32_t phase = 0;
+    for (int t = blockIdx.x >> 1; t < p.tiles_total; t += gridDim.x >> 1, ++i) {
+        const Tile w = decode(p, t);
+        const int buf = i & 1;
+        if (!wait_bar(&acc_empty[buf], ((i >> 1) & 1) ^ 1, p.health, abort_flag)) return;
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(buf) * n;
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+            if (!wait_bar(&full[s], phase, p.health, abort_flag)) return;
+            ptx::tc_fence_after();
+            const uint32_t sa = ptx::smem_u32(smem + s * stage_bytes);
+            const uint32_t sb = sa + kBM * 128;
+#pragma unroll
+            for (int j = 0; j < kBK / 16; ++j) {
+                // K-major: 32 bytes further inside the swizzle atom; MN-major: 16 k-rows further
+                const uint64_t da = a_mn ? desc(sa + j * 2048, kBK * 128, 1024) : desc(sa + j * 32, 16, 1024);
+                const uint64_t db = b_mn ? desc(sb + j * 2048, kBK * 128, 1024) : desc(sb + j * 32, 16, 1024);
+                ptx::mma_f16_pair(d, da, db, idesc, kb > w.kb0 || j > 0 ? 1u : 0u);
+            }
+            commit(&empty[s]);
+            if (++s == p.stages) {
+                s = 0;
+                phase ^= 1;
+            }
+        }
+        commit(&acc_full[buf]);
+    }
+}
+
+// Byte offset of 16-byte chunk j of row r in a store box whose rows are 128 bytes (128-byte
+// swizzle) or 64 bytes (64-byte swizzle): lane = row writes without bank conflicts.
+__device__ __forceinline__ uint32_t box_at(int r, int j, bool wide) {
+    return wide ? static_cast<uint32_t>(r * 128 + ((j ^ (r & 7)) << 4))
+                : static_cast<uint32_t>(r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
+}
+
+// Columns [store_cols, out_cols) of this lane's row, if its box (columns col0 .. col0 + box_cols - 1)
+// holds them: the store engine clips a row at 16-byte granules, so it would also write the columns
+// beside a row that ends inside one.
+template <int ELEM>
+__device__ __forceinline__ void store_tail(const Params& p, const uint8_t* box, bool wide, void* base, long long ld,
+                                           int col0, int row0, int lane) {
+    constexpr int kPer = 16 / ELEM;
+    if (p.store_cols >= p.out_cols || p.store_cols < col0 || p.store_cols >= col0 + p.box_cols || row0 + lane >= p.out_rows)
+        return;
+    const uint4 v = *reinterpret_cast<const uint4*>(box + box_at(lane, (p.store_cols - col0) / kPer, wide));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < kPer - 1; ++e) {
+        if (p.store_cols + e >= p.out_cols) break;
+        const long long at = (row0 + lane) * ld + p.store_cols + e;
+        if (ELEM == 4)
+            static_cast<uint32_t*>(base)[at] = w[e];
+        else
+            static_cast<uint16_t*>(base)[at] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+    }
+}
+
+// Epilogue warps: warp w reads TMEM lanes 32 (w % 4) .. + 31 (rows of the tile), the two warps of
+// a lane quarter take half of the tile's output columns each.
+template <int MODE, bool BF16, int ACT, bool OUT32>
+__device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t* boxes, uint64_t* in_full,
+                                      uint64_t* acc_full, uint64_t* acc_empty, uint32_t tmem,
+                                      volatile int* abort_flag) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const int rank = static_cast<int>(blockIdx.x & 1u);
+    uint8_t* box = boxes + (warp - 2) * 2 * kBoxBytes;  // two boxes per warp
+    uint8_t* box1 = box + kBoxBytes;
+    uint64_t* in_bar = in_full + (warp - 2);
+    const uint32_t n = 2u * p.bnc;
+    const bool wide = OUT32 || p.box_cols == 64;
+    int i = 0;
+    uint32_t used = 0;  // boxes handed to the store engine (kForward, kInput, kWeight)
+    for (int t = blockIdx.x >> 1; t < p.tiles_total; t += gridDim.x >> 1, ++i) {
+        const Tile w = decode(p, t);
+        const int buf = i & 1;
+        const int row0 = w.m * 2 * kBM + rank * kBM + q * 32;
+        const int mine = MODE == kForward || MODE == kGate ? p.bnc / 2 : p.bnc;  // this warp's output columns
+        const int col0 = w.n * p.tile_cols + half * mine;
+        if (MODE == kGate) {  // this tile's dh, while the products run
+            if (lane == 0) {
+                ptx::bulk_wait_read0();
+                ptx::mbar_arrive_expect_tx(in_bar, 32u * p.box_cols * 2u);
+                ptx::tma_load_3d(box, &maps.in, in_bar, col0, row0, 0);
+            }
+            __syncwarp();
+        }
+        const bool ready = wait_bar(&acc_full[buf], (i >> 1) & 1, p.health, abort_flag);
+        if (MODE == kGate) {  // the copy has landed before the box (or the CTA) goes on
+            const bool in = wait_bar(in_bar, i & 1, p.health, nullptr);
+            if (!in || !ready) break;
+        } else if (!ready) {
+            break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t base = tmem + static_cast<uint32_t>(buf) * n + (static_cast<uint32_t>(q * 32) << 16);
+        if (MODE == kForward || MODE == kGate) {
+            uint8_t* out0 = box;
+            if (MODE == kForward) {
+                out0 = used & 1 ? box1 : box;
+                if (lane == 0) ptx::bulk_wait_read1();
+                __syncwarp();
+            }
+            for (int c = 0; c < mine; c += 16) {
+                uint32_t gr[16], ur[16];
+                ptx::tmem_ld16_issue(base + half * mine + c, gr);
+                ptx::tmem_ld16_issue(base + p.bnc + half * mine + c, ur);
+                ptx::tmem_ld_wait(gr);
+                ptx::tmem_ld_wait(ur);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t at = box_at(lane, c / 8 + e, wide);
+                    uint32_t o0[4], o1[4];
+                    uint4 in4 = make_uint4(0, 0, 0, 0);
+                    if (MODE == kGate) in4 = *reinterpret_cast<const uint4*>(box + at);
+                    const uint32_t in[4] = {in4.x, in4.y, in4.z, in4.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float g0 = __uint_as_float(gr[8 * e + 2 * k]), g1 = __uint_as_float(gr[8 * e + 2 * k + 1]);
+                        const float u0 = __uint_as_float(ur[8 * e + 2 * k]), u1 = __uint_as_float(ur[8 * e + 2 * k + 1]);
+                        if (MODE == kForward) {
+                            o0[k] = pack2<BF16>(act_value<ACT>(g0) * u0, act_value<ACT>(g1) * u1);
+                        } else {
+                            const float2 dh = unpack2<BF16>(in[k]);
+                            float a0, s0, a1, s1;
+                            act_both<ACT>(g0, a0, s0);
+                            act_both<ACT>(g1, a1, s1);
+                            o0[k] = pack2<BF16>(dh.x * u0 * s0, dh.y * u1 * s1);
+                            o1[k] = pack2<BF16>(dh.x * a0, dh.y * a1);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(out0 + at) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+                    if (MODE == kGate) *reinterpret_cast<uint4*>(box1 + at) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+                }
+            }
+            ptx::tc_fence_before();
+            if (MODE == kForward) store_tail<2>(p, out0, wide, p.out[0], p.ld_out[0], col0, row0, lane);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                ptx::mbar_arrive_cluster(ptx::cluster_addr(&acc_empty[buf], 0));
+                if (col0 < p.store_cols && row0 < p.out_rows) {  // the store engine clips a box, it needs one to start inside
+                    ptx::tma_store_3d(&maps.d0, out0, col0, row0, 0);
+                    if (MODE == kGate) ptx::tma_store_3d(&maps.d0, box1, col0, row0, 1);
+                }
+                ptx::bulk_commit();
+            }
+            ++used;
+        } else {
+            const int z = MODE == kWeight ? (p.splits > 1 ? w.split * 2 + w.z : 0) : 0;
+            const CUtensorMap* dst = MODE == kWeight && p.splits == 1 && w.z ? &maps.d1 : &maps.d0;
+            for (int c = 0; c < mine; c += p.box_cols) {
+                uint8_t* out = used & 1 ? box1 : box;
+                if (lane == 0) ptx::bulk_wait_read1();
+                __syncwarp();
+                for (int e = 0; e < p.box_cols; e += 16) {
+                    uint32_t r[16];
+                    ptx::tmem_ld16_issue(base + half * mine + c + e, r);
+                    ptx::tmem_ld_wait(r);
+                    if (OUT32) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            *reinterpret_cast<uint4*>(out + box_at(lane, e / 4 + k, true)) =
+                                make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                o[j] = pack2<BF16>(__uint_as_float(r[8 * k + 2 * j]), __uint_as_float(r[8 * k + 2 * j + 1]));
+                            *reinterpret_cast<uint4*>(out + box_at(lane, e / 8 + k, wide)) = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                    }
+                }
+                if (c + p.box_cols >= mine) ptx::tc_fence_before();
+                store_tail<OUT32 ? 4 : 2>(p, out, wide, p.out[w.z], p.ld_out[w.z], col0 + c, row0, lane);
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    if (c + p.box_cols >= mine) ptx::mbar_arrive_cluster(ptx::cluster_addr(&acc_empty[buf], 0));
+                    if (col0 + c < p.store_cols && row0 < p.out_rows) ptx::tma_store_3d(dst, out, col0 + c, row0, z);
+                    ptx::bulk_commit();
+                }
+                ++used;
+            }
+        }
+    }
+    if (lane == 0) ptx::bulk_wait0();
+}
+
+template <int MODE, bool BF16, int ACT, bool OUT32>
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+    product_kernel(const __grid_constant__ Maps maps, const Params p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], mma_done, in_full[kEpiWarps];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t stage_bytes = static_cast<uint32_t>(kBM + p.bnc) * 128;
+    uint8_t* boxes = smem + p.stages * stage_bytes;
+    const int warp = threadIdx.x >> 5;
+    const bool leader = (blockIdx.x & 1u) == 0;
+    const uint32_t tmem_cols = 4u * p.bnc;  // two buffers of 2 bnc columns
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            ptx::mbar_init(&acc_full[b], 1);
+            ptx::mbar_init(&acc_empty[b], 2 * kEpiWarps);
+        }
+        for (int e = 0; e < kEpiWarps; ++e) ptx::mbar_init(&in_full[e], 1);
+        ptx::mbar_init(&mma_done, 1);
+        abort_flag = 0;
+        ptx::fence_barrier_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(&tmem_slot, tmem_cols);
+        ptx::tmem_relinquish_pair();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_sync();  // both CTAs' barriers exist before any remote use
+    ptx::tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0) {
+        if (ptx::elect_one()) produce<MODE>(maps, p, smem, stage_bytes, full, empty, &abort_flag);
+    } else if (warp == 1) {
+        if (ptx::elect_one()) {
+            if (leader) {
+                issue<MODE, BF16>(p, smem, stage_bytes, full, empty, acc_full, acc_empty, tmem, &abort_flag);
+                // all MMAs have completed before TMEM is released, also after an abort
+                ptx::mma_commit_pair(ptx::cluster_addr(&mma_done, 0));
+                ptx::mma_commit_pair(ptx::cluster_addr(&mma_done, 1));
+            }
+            wait_bar(&mma_done, 0, p.health, nullptr);
+        }
+    } else {
+        drain<MODE, BF16, ACT, OUT32>(maps, p, boxes, in_full, acc_full, acc_empty, tmem, &abort_flag);
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    __syncwarp();
+    ptx::cluster_sync();  // neither CTA leaves while the other may still address its memory
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc_pair(tmem, tmem_cols);
+    }
+}
+
+// out_z[f][k] = sum over splits, in split order, of part[split][z][f][k]; z = gate, up
+template <typename OUT>
+__device__ __forceinline__ OUT narrow(float v);
+template <>
+__device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename OUT>
+__global__ void reduce_kernel(const float* __restrict__ part, int splits, int rows, int cols, int ld_part,
+                              OUT* __restrict__ gate, long long ld_gate, OUT* __restrict__ up, long long ld_up) {
+    const int quads = (cols + 3) / 4;
+    const long long per = static_cast<long long>(rows) * quads;
+    const long long plane = static_cast<long long>(rows) * ld_part;
+    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < 2 * per;
+         i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const int z = i >= per;
+        const long long j = i - z * per;
+        const long long row = j / quads;
+        const int col = static_cast<int>(j - row * quads) * 4;
+        const float* src = part + z * plane + row * ld_part + col;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+            const float4 v = *reinterpret_cast<const float4*>(src + 2 * s * plane);
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
+        }
+        OUT* dst = (z ? up + row * ld_up : gate + row * ld_gate) + col;
+        dst[0] = narrow<OUT>(sum.x);
+        if (col + 1 < cols) dst[1] = narrow<OUT>(sum.y);
+        if (col + 2 < cols) dst[2] = narrow<OUT>(sum.z);
+        if (col + 3 < cols) dst[3] = narrow<OUT>(sum.w);
+    }
+}
+
+// ---- host ---------------------------------------------------------------------
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+    static const EncodeTiled fn = [] {
+        void* q = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) == cudaSuccess &&
+                       r == cudaDriverEntryPointSuccess
+                   ? reinterpret_cast<EncodeTiled>(q)
+                   : nullptr;
+    }();
+    return fn;
+}
+
+struct Plan {
+    int rows, features, hidden, bf16, act;
+    int device, pairs;  // CTA pairs resident at once
+};
+
+// {inner, outer, depth} elements at base; boxes of box_inner x box_outer
+bool make_map(CUtensorMap* map, const char* what, CUtensorMapDataType type, const void* base, long long inner,
+              long long outer, long long depth, long long ld, long long depth_stride, int box_inner, int box_outer) {
+    const int elem = type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer),
+                                static_cast<cuuint64_t>(depth)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * elem), static_cast<cuuint64_t>(depth_stride * elem)};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer), 1};
+    const cuuint32_t ones[3] = {1, 1, 1};
+    const CUtensorMapSwizzle swizzle = box_inner * elem == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    const CUresult r = encoder()(map, type, 3, const_cast<void*>(base), dims, strides, box, ones,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return true;
+    set_error("gated MLP: tensor map of %s failed (%d) for %lld x %lld", what, static_cast<int>(r), inner, outer);
+    return false;
+}
+
+bool matrix_ok(const char* what, const void* base, long long ld, long long cols, int elem) {
+    if (base && aligned(base, 16) && ld >= cols && (ld * elem) % 16 == 0) return true;
+    set_error("gated MLP: %s must be non-null, 16-byte aligned, with a row stride >= %lld that is a multiple of 16 bytes "
+              "(got stride %lld)", what, cols, ld);
+    return false;
+}
+
+typedef void (*KernelFn)(const Maps, const Params);
+
+template <bool BF16>
+KernelFn gated_kernel(int mode, int act) {
+    if (mode == kForward)
+        return act == kSilu ? product_kernel<kForward, BF16, kSilu, false>
+                            : act == kGelu ? product_kernel<kForward, BF16, kGelu, false>
+                                           : product_kernel<kForward, BF16, kRelu, false>;
+    return act == kSilu ? product_kernel<kGate, BF16, kSilu, false>
+                        : act == kGelu ? product_kernel<kGate, BF16, kGelu, false>
+                                       : product_kernel<kGate, BF16, kRelu, false>;
+}
+
+KernelFn kernel_of(const Plan* plan, int mode, bool out32) {
+    if (mode == kForward || mode == kGate)
+        return plan->bf16 ? gated_kernel<true>(mode, plan->act) : gated_kernel<false>(mode, plan->act);
+    if (mode == kInput) return plan->bf16 ? product_kernel<kInput, true, 0, false> : product_kernel<kInput, false, 0, false>;
+    if (out32) return plan->bf16 ? product_kernel<kWeight, true, 0, true> : product_kernel<kWeight, false, 0, true>;
+    return plan->bf16 ? product_kernel<kWeight, true, 0, false> : product_kernel<kWeight, false, 0, false>;
+}
+
+constexpr int kStaticSmem = 1024;  // room left for the barriers, the TMEM slot and the abort word
+
+int launch(const Plan* plan, int mode, bool out32, Params& p, const Maps& maps, cudaStream_t stream) {
+    const int stage = (kBM + p.bnc) * 128;
+    const int fixed = 1024 + kEpiWarps * 2 * kBoxBytes;
+    p.stages = std::min(kMaxStages, (kMaxSmem - kStaticSmem - fixed) / stage);
+    const long long total = static_cast<long long>(p.tiles_n) * p.tiles_m * p.tiles_z * p.splits;
+    if (total > 0x3FFFFFFF) {
+        set_error("gated MLP: too many output tiles");
+        return -1;
+    }
+    p.tiles_total = static_cast<int>(total);
+    const int pairs = static_cast<int>(std::min<long long>(total, plan->pairs));
+    kernel_of(plan, mode, out32)<<<2 * pairs, kThreads, p.stages * stage + fixed, stream>>>(maps, p);
+    return launch_status("gated MLP product");
+}
+
+// Tile width: 128 B rows per CTA, or 64 when the wider tiles would leave pairs without one.
+int width_for(const Plan* plan, long long row_tiles, long long cols, int per_row) {
+    return row_tiles * ((cols + 128 * per_row - 1) / (128 * per_row)) < plan->pairs ? 64 : 128;
+}
+
+// Splits of the weight gradients' contraction over `rows`: one tile per pair where the splits stay
+// at least 16 k-blocks long; and chains of at most 8192 rows, because the tensor cores' fp32
+// accumulation error grows with the chain (about 7e-9 per product, measured).
+int splits_for(const Plan* plan, int rows) {
+    const long long tiles = 2LL * ((plan->hidden + 255) / 256) * ((plan->features + 255) / 256);
+    const int kblocks = (rows + kBK - 1) / kBK;
+    const long long fill = std::max<long long>(1, std::min<long long>(plan->pairs / tiles, kblocks / 16));
+    return static_cast<int>(std::max<long long>(fill, (kblocks + 127) / 128));
+}
+
+long long pad(long long cols, long long to) { return (cols + to - 1) / to * to; }
+
+// inner extent of an output's tensor map: whole granules (rows shorter than one are not stored by it)
+long long stored(long long cols, long long granule) { return std::max(granule, cols / granule * granule); }
+
+// workspace: dg and du, then (when split) the fp32 partial weight gradients
+long long gate_bytes(const Plan* plan) { return pad(4LL * plan->rows * pad(plan->hidden, 8), 256); }
+long long part_bytes(const Plan* plan) {  // splits grow with the rows
+    const long long s = splits_for(plan, plan->rows);
+    return s > 1 ? s * 2 * plan->hidden * pad(plan->features, 4) * 4 : 0;
+}
+
+bool ready(const Plan* plan, int rows) {
+    if (!plan) {
+        set_error("null gated MLP plan");
+        return false;
+    }
+    if (rows < 0 || rows > plan->rows) {
+        set_error("gated MLP: rows must be 0..%d (got %d)", plan->rows, rows);
+        return false;
+    }
+    int device = -1;
+    if (cudaGetDevice(&device) != cudaSuccess || device != plan->device) {
+        set_error("gated MLP: the plan belongs to device %d, the current device is %d", plan->device, device);
+        return false;
+    }
+    return true;
+}
+
+// The two projections: forward (out = h) or backward (grad_out in, dg and du out).
+int project(const Plan* plan, int rows, const void* x, long long ldx, const void* wg, long long ldg, const void* wu,
+            long long ldu, const void* grad_out, long long ld_grad, void* out, long long ld_out, long long out_plane,
+            int* health, cudaStream_t stream) {
+    const int K = plan->features, F = plan->hidden;
+    const CUtensorMapDataType type = plan->bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const int mode = grad_out ? kGate : kForward;
+    Params p{};
+    p.tiles_m = (rows + 2 * kBM - 1) / (2 * kBM);
+    p.bnc = width_for(plan, p.tiles_m, F, 1);
+    p.tile_cols = p.bnc;
+    p.tiles_n = (F + p.bnc - 1) / p.bnc;
+    p.tiles_z = p.splits = 1;
+    p.kblocks = p.kb_per_split = (K + kBK - 1) / kBK;
+    p.box_cols = p.bnc / 2;
+    p.out_rows = rows;
+    p.out_cols = F;
+    p.store_cols = grad_out ? F : F / 8 * 8;  // the workspace's rows are padded: nothing beside them
+    p.out[0] = out;
+    p.ld_out[0] = ld_out;
+    p.health = health;
+    Maps maps;
+    const long long planes = grad_out ? 2 : 1;
+    if (!make_map(&maps.a, "x", type, x, K, rows, 1, ldx, ldx * rows, kBK, kBM) ||
+        !make_map(&maps.b0, "gate weight", type, wg, K, F, 1, ldg, ldg * F, kBK, p.bnc) ||
+        !make_map(&maps.b1, "up weight", type, wu, K, F, 1, ldu, ldu * F, kBK, p.bnc) ||
+        !make_map(&maps.d0, "output", type, out, grad_out ? F : stored(F, 8), rows, planes, ld_out, out_plane, p.box_cols, 32))
+        return -1;
+    maps.d1 = maps.in = maps.d0;
+    if (grad_out && !make_map(&maps.in, "output gradient", type, grad_out, F, rows, 1, ld_grad, ld_grad * rows, p.box_cols, 32))
+        return -1;
+    return launch(plan, mode, false, p, maps, stream);
+}
+
+int input_gradient(const Plan* plan, const rl2_gated_backward_args* g, cudaStream_t stream) {
+    const int K = plan->features, F = plan->hidden, rows = g->rows;
+    const CUtensorMapDataType type = plan->bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const long long ldw = pad(F, 8);
+    Params p{};
+    p.tiles_m = (rows + 2 * kBM - 1) / (2 * kBM);
+    p.bnc = width_for(plan, p.tiles_m, K, 2);
+    p.tile_cols = 2 * p.bnc;
+    p.tiles_n = (K + p.tile_cols - 1) / p.tile_cols;
+    p.tiles_z = p.splits = 1;
+    p.kb_segment = (F + kBK - 1) / kBK;
+    p.kblocks = p.kb_per_split = 2 * p.kb_segment;
+    p.box_cols = 64;
+    p.out_rows = rows;
+    p.out_cols = K;
+    p.store_cols = K / 8 * 8;
+    p.out[0] = g->grad_x;
+    p.ld_out[0] = g->ld_grad_x;
+    p.health = g->health;
+    Maps maps;
+    if (!make_map(&maps.a, "hidden gradients", type, g->workspace, F, rows, 2, ldw, ldw * rows, kBK, kBM) ||
+        !make_map(&maps.b0, "gate weight", type, g->gate_weight, K, F, 1, g->ld_gate, g->ld_gate * F, 64, kBK) ||
+        !make_map(&maps.b1, "up weight", type, g->up_weight, K, F, 1, g->ld_up, g->ld_up * F, 64, kBK) ||
+        !make_map(&maps.d0, "input gradient", type, g->grad_x, stored(K, 8), rows, 1, g->ld_grad_x, g->ld_grad_x * rows, 64, 32))
+        return -1;
+    maps.d1 = maps.in = maps.d0;
+    return launch(plan, kInput, false, p, maps, stream);
+}
+
+template <typename OUT>
+void reduce(const float* part, int splits, int rows, int cols, int ld, const rl2_gated_backward_args* g, cudaStream_t stream) {
+    const long long quads = 2LL * rows * ((cols + 3) / 4);
+    const int blocks = static_cast<int>(std::min<long long>((quads + 255) / 256, 148 * 8));
+    reduce_kernel<OUT><<<blocks, 256, 0, stream>>>(part, splits, rows, cols, ld, static_cast<OUT*>(g->grad_gate),
+                                                   g->ld_grad_gate, static_cast<OUT*>(g->grad_up), g->ld_grad_up);
+}
+
+int weight_gradients(const Plan* plan, const rl2_gated_backward_args* g, cudaStream_t stream) {
+    const int K = plan->features, F = plan->hidden, rows = g->rows;
+    const CUtensorMapDataType type = plan->bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const long long ldw = pad(F, 8), ldp = pad(K, 4);
+    Params p{};
+    p.tiles_m = (F + 2 * kBM - 1) / (2 * kBM);
+    p.tiles_z = 2;
+    p.kblocks = (rows + kBK - 1) / kBK;
+    p.splits = splits_for(plan, rows);
+    p.kb_per_split = (p.kblocks + p.splits - 1) / p.splits;
+    p.splits = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;  // every split non-empty
+    p.bnc = width_for(plan, 2LL * p.tiles_m * p.splits, K, 2);
+    p.tile_cols = 2 * p.bnc;
+    p.tiles_n = (K + p.tile_cols - 1) / p.tile_cols;
+    p.out_rows = F;
+    p.out_cols = K;
+    p.health = g->health;
+    float* part = reinterpret_cast<float*>(static_cast<char*>(g->workspace) + gate_bytes(plan));
+    const bool out32 = p.splits > 1 || g->grad_weight_fp32;
+    const CUtensorMapDataType out_type = out32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type;
+    p.box_cols = out32 ? 32 : 64;
+    const int granule = out32 ? 4 : 8;
+    p.store_cols = p.splits > 1 ? K : K / granule * granule;
+    p.out[0] = g->grad_gate;
+    p.out[1] = g->grad_up;
+    p.ld_out[0] = g->ld_grad_gate;
+    p.ld_out[1] = g->ld_grad_up;
+    Maps maps;
+    if (!make_map(&maps.a, "hidden gradients", type, g->workspace, F, rows, 2, ldw, ldw * rows, 64, kBK) ||
+        !make_map(&maps.b0, "x", type, g->x, K, rows, 1, g->ldx, g->ldx * rows, 64, kBK))
+        return -1;
+    maps.b1 = maps.b0;
+    if (p.splits > 1) {
+        if (!make_map(&maps.d0, "partial weight gradients", out_type, part, K, F, 2LL * p.splits, ldp, ldp * F, 32, 32)) return -1;
+        maps.d1 = maps.d0;
+    } else if (!make_map(&maps.d0, "gate weight gradient", out_type, g->grad_gate, stored(K, granule), F, 1, g->ld_grad_gate,
+                         g->ld_grad_gate * F, p.box_cols, 32) ||
+               !make_map(&maps.d1, "up weight gradient", out_type, g->grad_up, stored(K, granule), F, 1, g->ld_grad_up,
+                         g->ld_grad_up * F, p.box_cols, 32)) {
+        return -1;
+    }
+    maps.in = maps.d0;
+    if (launch(plan, kWeight, out32, p, maps, stream)) return -1;
+    if (p.splits == 1) return 0;
+    if (g->grad_weight_fp32)
+        reduce<float>(part, p.splits, F, K, static_cast<int>(ldp), g, stream);
+    else if (plan->bf16)
+        reduce<__nv_bfloat16>(part, p.splits, F, K, static_cast<int>(ldp), g, stream);
+    else
+        reduce<__half>(part, p.splits, F, K, static_cast<int>(ldp), g, stream);
+    return launch_status("gated MLP weight-gradient reduction");
+}
+
+}  // namespace gated
+}  // namespace rl2
+
+extern "C" void* rl2_gated_create(const rl2_gated_desc* d) {
+    using namespace rl2;
+    using namespace rl2::gated;
+    clear_error();
+    if (!d || d->rows < 1 || d->features < 1 || d->hidden < 1 || d->rows > (1 << 28) || d->features > (1 << 24) ||
+        d->hidden > (1 << 24)) {
+        set_error("gated MLP: rows (up to 2^28), features and hidden (up to 2^24) must be positive");
+        return nullptr;
+    }
+    if ((d->dtype != 0 && d->dtype != 1) || d->activation < 0 || d->activation > 2) {
+        set_error("gated MLP: dtype must be 0 (fp16) or 1 (bf16), activation 0 (SiLU), 1 (GELU) or 2 (ReLU)");
+        return nullptr;
+    }
+    if (!encoder()) {
+        set_error("cuTensorMapEncodeTiled is unavailable from the driver");
+        return nullptr;
+    }
+    Plan* plan = new (std::nothrow) Plan{d->rows, d->features, d->hidden, d->dtype, d->activation, 0, 0};
+    if (!plan) {
+        set_error("out of host memory");
+        return nullptr;
+    }
+    int sms = 0;
+    bool ok = cudaGetDevice(&plan->device) == cudaSuccess &&
+              cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, plan->device) == cudaSuccess;
+    plan->pairs = sms / 2;
+    for (int i = 0; ok && i < 5; ++i) {
+        const void* fn = reinterpret_cast<const void*>(kernel_of(plan, std::min(i, 3), i == 4));
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3(static_cast<unsigned>(2 * std::max(1, sms / 2)));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = kMaxSmem - kStaticSmem;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        ok = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem - kStaticSmem) == cudaSuccess &&
+             cudaOccupancyMaxActiveClusters(&clusters, fn, &cfg) == cudaSuccess && clusters > 0;
+        plan->pairs = std::min(plan->pairs, clusters);
+    }
+    if (!ok) {
+        set_error("gated MLP: no pair of CTAs fits the current device (%s)", cudaGetErrorString(cudaGetLastError()));
+        delete plan;
+        return nullptr;
+    }
+    return plan;
+}
+
+extern "C" int rl2_gated_destroy(void* plan) {
+    rl2::clear_error();
+    delete static_cast<rl2::gated::Plan*>(plan);
+    return 0;
+}
+
+extern "C" long long rl2_gated_workspace_bytes(void* opaque) {
+    using namespace rl2::gated;
+    const Plan* plan = static_cast<const Plan*>(opaque);
+    return plan ? gate_bytes(plan) + part_bytes(plan) : -1;
+}
+
+extern "C" int rl2_gated_forward(void* opaque, const rl2_gated_forward_args* g, void* stream) {
+    using namespace rl2;
+    using namespace rl2::gated;
+    clear_error();
+    const Plan* plan = static_cast<const Plan*>(opaque);
+    if (!g) {
+        set_error("gated MLP: null arguments");
+        return -1;
+    }
+    if (!ready(plan, g->rows)) return -1;
+    if (g->rows == 0) return 0;
+    if (!matrix_ok("x", g->x, g->ldx, plan->features, 2) ||
+        !matrix_ok("gate weight", g->gate_weight, g->ld_gate, plan->features, 2) ||
+        !matrix_ok("up weight", g->up_weight, g->ld_up, plan->features, 2) ||
+        !matrix_ok("output", g->out, g->ld_out, plan->hidden, 2))
+        return -1;
+    return project(plan, g->rows, g->x, g->ldx, g->gate_weight, g->ld_gate, g->up_weight, g->ld_up, nullptr, 0, g->out,
+                   g->ld_out, g->ld_out * g->rows, g->health, as_stream(stream));
+}
+
+extern "C" int rl2_gated_backward(void* opaque, const rl2_gated_backward_args* g, void* stream) {
+    using namespace rl2;
+    using namespace rl2::gated;
+    clear_error();
+    const Plan* plan = static_cast<const Plan*>(opaque);
+    if (!g) {
+        set_error("gated MLP: null arguments");
+        return -1;
+    }
+    if (!ready(plan, g->rows)) return -1;
+    const int K = plan->features, F = plan->hidden;
+    const int elem = g->grad_weight_fp32 ? 4 : 2;
+    const bool weights = g->grad_gate || g->grad_up;
+    if (!weights && !g->grad_x) {
+        set_error("gated MLP backward: no gradient asked for");
+        return -1;
+    }
+    if (weights && (!matrix_ok("gate weight gradient", g->grad_gate, g->ld_grad_gate, K, elem) ||
+                    !matrix_ok("up weight gradient", g->grad_up, g->ld_grad_up, K, elem)))
+        return -1;
+    cudaStream_t s = as_stream(stream);
+    if (g->rows == 0) {
+        if (weights && (cudaMemset2DAsync(g->grad_gate, g->ld_grad_gate * elem, 0, static_cast<size_t>(K) * elem, F, s) != cudaSuccess ||
+                        cudaMemset2DAsync(g->grad_up, g->ld_grad_up * elem, 0, static_cast<size_t>(K) * elem, F, s) != cudaSuccess)) {
+            set_error("gated MLP backward: clearing the weight gradients failed");
+            return -1;
+        }
+        return 0;
+    }
+    if (!matrix_ok("x", g->x, g->ldx, K, 2) || !matrix_ok("gate weight", g->gate_weight, g->ld_gate, K, 2) ||
+        !matrix_ok("up weight", g->up_weight, g->ld_up, K, 2) || !matrix_ok("output gradient", g->grad_out, g->ld_grad_out, F, 2) ||
+        (g->grad_x && !matrix_ok("input gradient", g->grad_x, g->ld_grad_x, K, 2)))
+        return -1;
+    if (!g->workspace || !aligned(g->workspace, 256)) {
+        set_error("gated MLP backward: the workspace must be non-null and 256-byte aligned");
+        return -1;
+    }
+    if (g->grad_x == g->x) {
+        set_error("gated MLP backward: grad_x may not be x (the weight gradients read x after it is written)");
+        return -1;
+    }
+    const long long ldw = pad(F, 8);
+    if (project(plan, g->rows, g->x, g->ldx, g->gate_weight, g->ld_gate, g->up_weight, g->ld_up, g->grad_out,
+                g->ld_grad_out, g->workspace, ldw, ldw * g->rows, g->health, s))
+        return -1;
+    if (g->grad_x && input_gradient(plan, g, s)) return -1;
+    return weights ? weight_gradients(plan, g, s) : 0;
+}
