@@ -12,7 +12,8 @@
  *    capture; plans are tied to the current device and are not thread-safe;
  *  - device waits inside kernels are bounded: a wait that times out sets a bit
  *    in the caller's int "health" word (1 = timeout, 2 = non-finite value,
- *    4 = fp16 operand overflow) instead of hanging.
+ *    4 = fp16 operand overflow, 8 = index or per-row parameter out of range) instead of
+ *    hanging.
  *
  * All floating-point buffers are fp32 unless a parameter says fp16.
  */
@@ -916,6 +917,90 @@ int rl2_gated_destroy(void* plan);
 long long rl2_gated_workspace_bytes(void* plan);
 int rl2_gated_forward(void* plan, const rl2_gated_forward_args* args, void* stream);
 int rl2_gated_backward(void* plan, const rl2_gated_backward_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * distillation of a head from a teacher's top logits, loss and gradient in one kernel (no
+ * counterpart in the reference). Per row, with T = temperature:
+ *   q = softmax(t / T) over the row's teacher entries, p = softmax(s / T) over its vocab
+ *   logits; row_loss = T^2 sum_k q_k (log q_k - log p[i_k]);
+ *   *loss_out = loss_weight * sum_n w_n row_loss_n, rows added in a fixed order;
+ *   dlogits_j = loss_weight w_n T (p_j - sum_{k: i_k = j} q_k) * *grad_scale, assigned.
+ * teacher_values / teacher_indices [rows][top], 1 <= top <= 1024, any order; an index < 0
+ * marks an absent entry, one >= vocab is left out and sets bit 8 of *health; a token may
+ * appear more than once (its q add up). row_weight null: 1. A row of weight 0 (its logits
+ * are not read), without a teacher entry above -inf or without a logit above -inf has loss 0
+ * and gradient 0; otherwise NaN and +inf give NaN. A token at -inf has p = 0: a teacher entry
+ * on it makes the loss +inf, its gradient stays finite.
+ * Types: 0 = fp32, 1 = fp16, 2 = bf16, each matrix its own; rows contiguous, any row stride
+ * and alignment (16-byte aligned rows, or logits and gradient rows equally misaligned, are
+ * fastest). dlogits, grad_scale (a device float: the loss scale of fp16 gradients),
+ * row_weight, loss_out and health may be null. counter: one zero-initialised unsigned int
+ * that the kernel leaves at zero; calls that overlap need one each.
+ * ------------------------------------------------------------------------- */
+typedef struct rl2_distill_args {
+    int rows, vocab, top;
+    const void* logits;
+    long long ld_logits;
+    int logits_dtype;
+    const void* teacher_values;
+    long long ld_values;
+    int values_dtype;
+    const void* teacher_indices;
+    long long ld_indices;
+    int index_bits;
+    float temperature;
+    const float* row_weight;
+    float loss_weight;
+    float* row_loss;
+    float* loss_out;
+    void* dlogits;
+    long long ld_dlogits;
+    int dlogits_dtype;
+    const float* grad_scale;
+    unsigned* counter;
+    int* health;
+} rl2_distill_args;
+
+int rl2_distill_topk(const rl2_distill_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * drawing one token per row of logits with temperature, top-k, top-p and min-p from given
+ * uniforms (no counterpart in the reference, whose policies act on continuous actions).
+ * Tokens are ordered by logit, descending, equal logits by index; e = exp((l - max) / T),
+ * with (l - max) times the fp32 reciprocal of T; w = round(2^30 e) as an integer. Kept are
+ * the tokens that are among the first top_k (top_k <= 0 or >= vocab: all), have before them
+ * in that order less than top_p of the top-k mass (the first token always; top_p >= 1: all;
+ * <= 0: the first alone) and have e >= min_p. tokens[row] is the first index whose
+ * cumulative w over the kept tokens exceeds floor(u W), W their sum; log_probs[row]
+ * (optional) = log(w / W). Sums are exact integers: the result depends on the inputs alone.
+ * T = 0 (or below the smallest normal float) takes the first best token. NaN logits count as -inf, +inf as the largest float;
+ * a row without a logit above -inf gives token -1 and log-probability -inf, and so does a
+ * row whose own parameters are not valid (temperature negative or NaN, top_p NaN, min_p
+ * above 1 or NaN; bit 8 of *health). A uniform below 0 or NaN
+ * counts as 0, one at or above 1 as just below it.
+ * Scalars apply to all rows; temperatures, top_ks, top_ps and min_ps (device arrays
+ * [rows], each optional) replace them. Logits: 0 = fp32, 1 = fp16, 2 = bf16, contiguous
+ * rows of 1..2^20 tokens, any row stride and alignment.
+ * ------------------------------------------------------------------------- */
+typedef struct rl2_sample_args {
+    int rows, vocab;
+    const void* logits;
+    long long ld_logits;
+    int logits_dtype;
+    const float* uniforms;
+    float temperature;
+    int top_k;
+    float top_p, min_p;
+    const float* temperatures;
+    const int* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    int* tokens;
+    float* log_probs;
+    int* health;
+} rl2_sample_args;
+
+int rl2_sample_tokens(const rl2_sample_args* args, void* stream);
 
 #ifdef __cplusplus
 }

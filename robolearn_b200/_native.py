@@ -431,3 +431,31 @@ SIGNATURES.update({
     "rl2_gated_forward": ([P, ctypes.POINTER(GatedForwardArgs), P], I),
     "rl2_gated_backward": ([P, ctypes.POINTER(GatedBackwardArgs), P], I),
 })
+
+
+class DistillArgs(ctypes.Structure):
+    """``rl2_distill_args`` (include/rl2.h)."""
+
+    _fields_ = [
+        ("rows", I), ("vocab", I), ("top", I), ("logits", P), ("ld_logits", LL), ("logits_dtype", I),
+        ("teacher_values", P), ("ld_values", LL), ("values_dtype", I), ("teacher_indices", P), ("ld_indices", LL),
+        ("index_bits", I), ("temperature", F), ("row_weight", P), ("loss_weight", F), ("row_loss", P),
+        ("loss_out", P), ("dlogits", P), ("ld_dlogits", LL), ("dlogits_dtype", I), ("grad_scale", P),
+        ("counter", P), ("health", P),
+    ]
+
+
+SIGNATURES["rl2_distill_topk"] = ([ctypes.POINTER(DistillArgs), P], I)
+
+
+class SampleArgs(ctypes.Structure):
+    """``rl2_sample_args`` (include/rl2.h)."""
+
+    _fields_ = [
+        ("rows", I), ("vocab", I), ("logits", P), ("ld_logits", LL), ("logits_dtype", I), ("uniforms", P),
+        ("temperature", F), ("top_k", I), ("top_p", F), ("min_p", F), ("temperatures", P), ("top_ks", P),
+        ("top_ps", P), ("min_ps", P), ("tokens", P), ("log_probs", P), ("health", P),
+    ]
+
+
+SIGNATURES["rl2_sample_tokens"] = ([ctypes.POINTER(SampleArgs), P], I)

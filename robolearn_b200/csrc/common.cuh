@@ -42,6 +42,7 @@ constexpr uint32_t kSpinLimit = 1u << 26;
 constexpr int kHealthTimeout = 1;
 constexpr int kHealthNonFinite = 2;
 constexpr int kHealthOverflow = 4;
+constexpr int kHealthIndex = 8;
 
 }  // namespace rl2
 
