@@ -25,6 +25,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 namespace rl2 {
 namespace sample {
@@ -104,6 +105,8 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
 }
 
 struct WarpGroup {
+    __device__ __forceinline__ u64 mass(u64 m) { return warp_sum64(m); }
+    __device__ __forceinline__ uint32_t count(uint32_t c) { return __reduce_add_sync(0xffffffffu, c); }
     __device__ __forceinline__ Sum sum(Sum s) { return Sum{__reduce_add_sync(0xffffffffu, s.count), warp_sum64(s.mass)}; }
     __device__ __forceinline__ uint32_t max_key(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
 };
@@ -287,40 +290,55 @@ __global__ void __launch_bounds__(32 * kRowWarps) warp_kernel(const rl2_sample_a
 // The row is read once. A thread keeps the maxima of small groups of its tokens (16-byte vectors, or
 // several); the k-th largest of all maxima bounds the k-th token from below, so only the groups whose
 // maximum reaches the bound are read again and give a list of a little more than k candidates, on which
-// both cuts are found. The bound comes from a histogram of the maxima over 2048 bins of (l - max) / T,
+// cuts and draw are made. The bound comes from a histogram of the maxima over 2048 bins of (max - l) / T,
 // whose 21.6 cover every token that has a weight. min-p bounds the candidates in the same way.
 // Without a bound (no top-k, or the list does not fit) the cuts come from a histogram of all tokens
-// (count and weight a bin) and the list of those in the bin of the cut.
-// The draw: the kept weight of each stretch of 2^shift tokens, a scan, and one warp on the stretch that
-// holds the target.
+// (count and weight a bin) and the list of those in the bin of the cut, and the draw from the kept
+// weight of each stretch of 2^shift tokens.
+// Histograms leave a bin of a few tokens, which one warp finishes without barriers.
 
 constexpr int kT = 512;
 constexpr int kWarps = kT / 32;
 constexpr int kBins = 2048;
+constexpr int kEach = kBins / kT;
 constexpr float kReach = 21.6f;  // exp(-21.6) 2^30 rounds to 0
-constexpr int kSlots = 16;       // group maxima per thread
 constexpr int kPer = 8;          // list entries per thread
 constexpr int kList = kT * kPer;
+constexpr int kFew = 32 * kPer;  // tokens that one warp takes
 constexpr int kStretches = 1024;
 constexpr int kMaxStretch = 2048;  // tokens: 2^20 of them in fewer than 1024 stretches
 
+// A bin of a histogram (or a stretch): what is in it, what is before it, the whole.
+struct Found {
+    Sum here, before, whole;
+    int bin, pad;
+};
+
 struct Shared {
-    u64 mass[kBins];       // histogram / stretches
-    uint32_t count[kBins];
-    float maxima[kSlots][kT];
+    alignas(16) u64 mass[kBins];  // histogram / stretches
+    alignas(16) uint32_t count[kBins];
+    uint8_t maxima[64 * kT];      // L [slot][thread]
     float value[kList];
     int index[kList];
-    uint32_t slot_w[kMaxStretch];  // the drawn stretch: weight, tie
-    uint8_t slot_tie[kMaxStretch];
+    union {
+        struct {
+            uint32_t slot_w[kMaxStretch];  // the drawn stretch: weight, tie
+            uint8_t slot_tie[kMaxStretch];
+        };
+        struct {
+            float few_value[kFew];
+            int few_index[kFew];
+            uint32_t few_w[kFew];
+        };
+    };
     uint32_t red_count[2][kWarps];
     u64 red_mass[2][kWarps];
+    uint2 red_pair[2][kWarps];
     uint32_t scan_count[kWarps];
     u64 scan_mass[kWarps];
-    int found;
-    u64 found_mass;
-    uint32_t found_count;
-    u64 found_total;
-    int listed;
+    Found found;
+    Cut cut;
+    int listed, groups, few, answer;
 };
 
 __device__ __forceinline__ uint32_t peer(const void* p, uint32_t rank) { return ptx::cluster_addr(p, rank); }
@@ -334,8 +352,63 @@ __device__ __forceinline__ u64 load64(uint32_t at) {
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
     return v;
 }
+__device__ __forceinline__ void store32(uint32_t at, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ void add32(uint32_t at, uint32_t v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ void add64(uint32_t at, u64 v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.add.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+}
 
-// All threads of the cluster's CTAs (of the CTA alone where it has one).
+// A warp's lanes append `mine` entries each to a list: the place of this lane's first.
+__device__ __forceinline__ int append(int* length, int mine) {
+    const int lane = threadIdx.x & 31;
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+    }
+    int base = 0;
+    if (lane == 31 && sum) base = atomicAdd(length, sum);
+    return __shfl_sync(0xffffffffu, base, 31) + sum - mine;
+}
+
+// The threads of one CTA. At most 2^12 tokens of weight up to 2^30 a sum: the count shares a word with
+// the weight's high bits. One barrier a reduction: the slots alternate, and a slot is written again only
+// after the barrier of the reduction between, which every reader has reached.
+struct Block {
+    Shared* sh;
+    int parity;
+    __device__ __forceinline__ Sum sum(Sum s) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        const uint32_t lo = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(s.mass) & 0x3FFFFFFu);
+        uint32_t hi = __reduce_add_sync(0xffffffffu, (s.count << 18) | static_cast<uint32_t>(s.mass >> 26));
+        if (lane == 0) sh->red_pair[parity][warp] = make_uint2(lo, hi);
+        __syncthreads();
+        const uint2 x = lane < kWarps ? sh->red_pair[parity][lane] : make_uint2(0, 0);
+        parity ^= 1;
+        // the warps' low parts have 31 bits: added as two halves
+        const uint32_t l0 = __reduce_add_sync(0xffffffffu, x.x & 0xFFFFu), l1 = __reduce_add_sync(0xffffffffu, x.x >> 16);
+        hi = __reduce_add_sync(0xffffffffu, x.y);
+        return Sum{hi >> 18, (static_cast<u64>(hi & 0x3FFFFu) << 26) + (static_cast<u64>(l1) << 16) + l0};
+    }
+    __device__ __forceinline__ u64 mass(u64 m) { return sum(Sum{0, m}).mass; }
+    __device__ __forceinline__ uint32_t count(uint32_t c) { return sum(Sum{c, 0}).count; }
+    __device__ __forceinline__ uint32_t max_key(uint32_t k) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        k = __reduce_max_sync(0xffffffffu, k);
+        if (lane == 0) sh->red_count[parity][warp] = k;
+        __syncthreads();
+        k = lane < kWarps ? sh->red_count[parity][lane] : 0u;
+        parity ^= 1;
+        return __reduce_max_sync(0xffffffffu, k);
+    }
+};
+
+// The threads of a cluster's CTAs (of the CTA alone where it has one), any number of tokens.
 struct Cluster {
     Shared* sh;
     uint32_t size, rank;
@@ -347,8 +420,6 @@ struct Cluster {
         else
             __syncthreads();
     }
-    // One barrier a reduction: the slots alternate, and a slot is written again only after the
-    // barrier of the reduction between, which every reader has reached.
     __device__ __forceinline__ Sum sum(Sum s) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         s.count = __reduce_add_sync(0xffffffffu, s.count);
@@ -414,360 +485,714 @@ __device__ __forceinline__ Sum block_scan(Shared* sh, Sum s, Sum& all) {
     return before;
 }
 
+__device__ __forceinline__ void clear_histogram(Shared* sh) {
+    for (int i = threadIdx.x; i < kBins / 2; i += kT) reinterpret_cast<uint4*>(sh->mass)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < kBins / 4; i += kT) reinterpret_cast<uint4*>(sh->count)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// Of a complete histogram: into sh->found the first bin up to which (itself included) the count, or the
+// weight, reaches the limit (kBins where none does). All threads; a barrier before it is read.
+__device__ __forceinline__ void find_bin(Shared* sh, bool by_mass, double limit, const Sum (&mine)[kEach], Sum at) {
+    auto value = [&](Sum x) { return by_mass ? static_cast<double>(x.mass) : static_cast<double>(x.count); };
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const Sum next{at.count + mine[e].count, at.mass + mine[e].mass};
+        if (value(at) < limit && value(next) >= limit) {
+            sh->found.bin = threadIdx.x * kEach + e;
+            sh->found.here = mine[e];
+            sh->found.before = at;
+        }
+        at = next;
+    }
+}
+
+// This thread's bins and what is before them.
+__device__ __forceinline__ Sum scan_histogram(Shared* sh, Sum (&mine)[kEach], Sum& whole) {
+    Sum s{0, 0};
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        mine[e] = Sum{sh->count[threadIdx.x * kEach + e], sh->mass[threadIdx.x * kEach + e]};
+        s.count += mine[e].count;
+        s.mass += mine[e].mass;
+    }
+    return block_scan(sh, s, whole);
+}
+
+// ---- a row from its list ------------------------------------------------------------
+
+// The last of the first `ties` indexes among the tokens marked, which are more than that.
+template <int N, typename Group>
+__device__ __forceinline__ int last_of(Group& group, const int (&token)[N], const bool (&marked)[N], u64 ties, int vocab) {
+    int lo = -1, hi = vocab - 1;  // more than `ties` through hi, not through lo
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c += marked[i] && token[i] <= mid;
+        (group.count(c) > ties ? hi : lo) = mid;
+    }
+    return lo;
+}
+
+// The first index through which the tokens' weight and what is before them exceeds the target.
+template <int N, typename Group>
+__device__ __forceinline__ int first_over(Group& group, const int (&token)[N], const uint32_t (&w)[N], u64 before, u64 target,
+                                          int vocab) {
+    int lo = -1, hi = vocab - 1;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        u64 m = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) m += token[i] <= mid ? w[i] : 0u;
+        (before + group.mass(m) > target ? hi : lo) = mid;
+    }
+    return hi;
+}
+
+// Up to kFew candidates: one warp, no barriers.
+__device__ __noinline__ void draw_few(Shared* sh, int n, const Row r, int vocab, float best, const rl2_sample_args& a, long long row) {
+    const int lane = threadIdx.x & 31;
+    WarpGroup group;
+    float v[kPer];
+    uint32_t w[kPer];
+    int token[kPer];
+    Sum all{0, 0};
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int at = i * 32 + lane;
+        v[i] = at < n ? sh->value[at] : -INFINITY;
+        token[i] = at < n ? sh->index[at] : vocab;
+        w[i] = at < n ? static_cast<uint32_t>(weight_of(exp_of(v[i], best, r.inverse))) : 0u;
+        all.count += w[i] != 0;
+        all.mass += w[i];
+    }
+    all = group.sum(all);
+    const Kept kept = both_cuts(group, r, vocab, best, v, w, all);
+    bool tie[kPer];
+    uint32_t ties = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) ties += tie[i] = v[i] == kept.cut && w[i] != 0;
+    const int last = group.count(ties) > kept.ties ? last_of(group, token, tie, kept.ties, vocab) : vocab;
+    u64 total = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const bool in = v[i] > kept.cut || (tie[i] && token[i] <= last);
+        if (!in || (!r.greedy && exp_of(v[i], best, r.inverse) < r.min_p)) w[i] = 0;
+        total += w[i];
+    }
+    total = group.mass(total);
+    const int chosen = first_over(group, token, w, 0, target_of(r.uniform, total), vocab);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (token[i] == chosen && w[i]) {
+            a.tokens[row] = chosen;
+            if (a.log_probs) a.log_probs[row] = log_share(w[i], total);
+        }
+}
+
+// A longer list: histograms of it (by value for the cuts, by index for the draw), one warp on the bin found.
+// `fine` bins a unit of value below the best spread the list over all bins.
+__device__ __noinline__ void draw_many(Shared* sh, int n, const Row r, int vocab, float best, float fine, const rl2_sample_args& a,
+                                       long long row) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    Block group{sh, 0};
+    float v[kPer];
+    uint32_t w[kPer];
+    int token[kPer];
+    auto bin_of = [&](float x) {
+        const float at = (best - x) * fine;
+        return at < kBins - 1 ? static_cast<int>(at) : kBins - 1;
+    };
+    clear_histogram(sh);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int at = i * kT + tid;
+        v[i] = at < n ? sh->value[at] : -INFINITY;
+        token[i] = at < n ? sh->index[at] : vocab;
+        w[i] = at < n ? static_cast<uint32_t>(weight_of(exp_of(v[i], best, r.inverse))) : 0u;
+        if (w[i]) {
+            atomicAdd(&sh->count[bin_of(v[i])], 1u);
+            atomicAdd(&sh->mass[bin_of(v[i])], static_cast<u64>(w[i]));
+        }
+    }
+    __syncthreads();
+    Sum mine[kEach], whole;
+    const Sum at = scan_histogram(sh, mine, whole);
+    // the cut whose limit the histogram reaches
+    auto cut_of = [&](auto by_mass, double limit) {
+        constexpr bool kMass = decltype(by_mass)::value;
+        if (tid == 0) sh->few = 0;
+        find_bin(sh, kMass, limit, mine, at);
+        __syncthreads();
+        const int bin = sh->found.bin;
+        const Sum before = sh->found.before;
+        if (sh->found.here.count <= kFew) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (w[i] && bin_of(v[i]) == bin) {
+                    const int to = atomicAdd(&sh->few, 1);
+                    sh->few_value[to] = v[i];
+                    sh->few_w[to] = w[i];
+                }
+            __syncthreads();
+            if (warp == 0) {
+                float x[kPer];
+                uint32_t y[kPer];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    x[i] = i * 32 + lane < sh->few ? sh->few_value[i * 32 + lane] : -INFINITY;
+                    y[i] = i * 32 + lane < sh->few ? sh->few_w[i * 32 + lane] : 0u;
+                }
+                WarpGroup own;
+                const Cut c = find_cut<kMass>(own, x, y, limit, before);
+                if (lane == 0) sh->cut = c;
+            }
+            __syncthreads();
+            const Cut c = sh->cut;
+            __syncthreads();
+            return c;
+        }
+        uint32_t y[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) y[i] = bin_of(v[i]) == bin ? w[i] : 0u;
+        return find_cut<kMass>(group, v, y, limit, before);
+    };
+    Kept kept{-INFINITY, 0};
+    if (r.greedy || r.top_p <= 0.0f) {
+        kept = Kept{best, 1};
+    } else {
+        Sum above = whole;
+        u64 total = whole.mass;
+        if (r.top_k > 0 && r.top_k < vocab && whole.count > static_cast<uint32_t>(r.top_k)) {
+            const Cut c = cut_of(std::false_type{}, r.top_k);
+            kept = Kept{c.value, static_cast<u64>(r.top_k) - c.above.count};
+            above = c.above;
+            total = above.mass + kept.ties * weight_of(exp_of(kept.cut, best, r.inverse));
+        }
+        if (r.top_p < 1.0f) {
+            const double limit = static_cast<double>(r.top_p) * static_cast<double>(total);
+            u64 most = kept.ties;
+            if (!(static_cast<double>(above.mass) < limit)) {
+                const Cut c = cut_of(std::true_type{}, limit);
+                kept.cut = c.value;
+                above = c.above;
+                most = ~0ull;
+            }
+            if (kept.cut != -INFINITY)
+                kept.ties = kept_of_last(above.mass, weight_of(exp_of(kept.cut, best, r.inverse)), limit, most);
+        }
+    }
+    // ---- what is kept, by index ----
+    bool tie[kPer];
+    uint32_t ties = 0;
+    __syncthreads();  // sh->few and the histogram are read
+    if (tid == 0) sh->few = 0;
+    clear_histogram(sh);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) ties += tie[i] = v[i] == kept.cut && w[i] != 0;
+    ties = group.count(ties);
+    int last = vocab;
+    if (ties > kept.ties) {
+        if (ties <= kFew) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (tie[i]) sh->few_index[atomicAdd(&sh->few, 1)] = token[i];
+            __syncthreads();
+            if (warp == 0) {
+                int x[kPer];
+                bool y[kPer];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    y[i] = i * 32 + lane < sh->few;
+                    x[i] = y[i] ? sh->few_index[i * 32 + lane] : vocab;
+                }
+                WarpGroup own;
+                const int l = last_of(own, x, y, kept.ties, vocab);
+                if (lane == 0) sh->answer = l;
+            }
+            __syncthreads();
+            last = sh->answer;
+        } else {
+            last = last_of(group, token, tie, kept.ties, vocab);
+        }
+    }
+    int shift = 0;
+    while ((vocab - 1) >> shift >= kBins) ++shift;
+    __syncthreads();  // the histogram is clear, sh->answer and sh->few are read
+    if (tid == 0) sh->few = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const bool in = v[i] > kept.cut || (tie[i] && token[i] <= last);
+        if (!in || (!r.greedy && exp_of(v[i], best, r.inverse) < r.min_p)) w[i] = 0;
+        if (w[i]) {
+            atomicAdd(&sh->count[token[i] >> shift], 1u);
+            atomicAdd(&sh->mass[token[i] >> shift], static_cast<u64>(w[i]));
+        }
+    }
+    __syncthreads();
+    Sum kept_all;
+    const Sum kept_at = scan_histogram(sh, mine, kept_all);
+    const u64 target = target_of(r.uniform, kept_all.mass);
+    find_bin(sh, true, static_cast<double>(target + 1), mine, kept_at);
+    __syncthreads();
+    const int bin = sh->found.bin;
+    const u64 before = sh->found.before.mass;
+    int chosen;
+    if (sh->found.here.count <= kFew) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (w[i] && token[i] >> shift == bin) {
+                const int to = atomicAdd(&sh->few, 1);
+                sh->few_index[to] = token[i];
+                sh->few_w[to] = w[i];
+            }
+        __syncthreads();
+        if (warp != 0) return;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const bool in = i * 32 + lane < sh->few;
+            token[i] = in ? sh->few_index[i * 32 + lane] : vocab;
+            w[i] = in ? sh->few_w[i * 32 + lane] : 0u;
+        }
+        WarpGroup own;
+        chosen = first_over(own, token, w, before, target, vocab);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (token[i] >> shift != bin) w[i] = 0;
+        chosen = first_over(group, token, w, before, target, vocab);
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (token[i] == chosen && w[i]) {
+            a.tokens[row] = chosen;
+            if (a.log_probs) a.log_probs[row] = log_share(w[i], kept_all.mass);
+        }
+}
+
+// ---- reading a row ------------------------------------------------------------------
+
 template <typename L>
 struct Reader {
     static constexpr int kN = 16 / sizeof(L);
-    const L* s;     // the row
-    int vocab, mis; // elements between the 16-byte boundary at or before the row and the row
+    const L* s;      // the row
+    int vocab, mis;  // elements between the 16-byte boundary at or before the row and the row
     int vectors;
 
     __device__ __forceinline__ Reader(const L* row, int v) : s(row), vocab(v) {
         mis = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(L));
         vectors = (mis + vocab + kN - 1) / kN;
     }
-    // token of element e of vector b: b kN + e - mis; elements outside the row are -inf
+    // token of the first element of vector b; whether the vector lies in the row, and the 32 from b on
+    __device__ __forceinline__ int first(int b) const { return b * kN - mis; }
+    __device__ __forceinline__ bool whole(int j) const { return j >= 0 && j + kN <= vocab; }
+    __device__ __forceinline__ bool inside(int b) const { return b * kN >= mis && (b + 32) * kN - mis <= vocab; }
+    __device__ __forceinline__ uint4 raw(int b) const { return __ldg(reinterpret_cast<const uint4*>(s + first(b))); }
+    __device__ __forceinline__ float at(int j) const { return clean(to_float(s[j])); }
+    // elements outside the row are -inf
     __device__ __forceinline__ void load(int b, float (&v)[kN]) const {
-        const int j = b * kN - mis;
-        if (j >= 0 && j + kN <= vocab) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(s + j));
-            L x[kN];
-            *reinterpret_cast<uint4*>(x) = raw;
+        const int j = first(b);
+        if (whole(j)) {
+            const uint4 x = raw(b);
+            L y[kN];
+            *reinterpret_cast<uint4*>(y) = x;
 #pragma unroll
-            for (int e = 0; e < kN; ++e) v[e] = clean(to_float(x[e]));
+            for (int e = 0; e < kN; ++e) v[e] = clean(to_float(y[e]));
         } else {
 #pragma unroll
-            for (int e = 0; e < kN; ++e) v[e] = j + e >= 0 && j + e < vocab ? clean(to_float(s[j + e])) : -INFINITY;
+            for (int e = 0; e < kN; ++e) v[e] = j + e >= 0 && j + e < vocab ? at(j + e) : -INFINITY;
         }
     }
 };
 
+// Maximum of a 16-byte vector's elements, NaN left out (not cleaned otherwise).
 template <typename L>
-__global__ void __launch_bounds__(kT, 2) row_kernel(const rl2_sample_args a, const int size, const int shift) {
-    extern __shared__ __align__(16) uint8_t raw[];
-    Shared* sh = reinterpret_cast<Shared*>(raw);
-    constexpr int kN = Reader<L>::kN;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int V = a.vocab;
-    Cluster group{sh, static_cast<uint32_t>(size), size > 1 ? ptx::cluster_rank() : 0u, 0};
-    const int per = (1 << shift) / (32 * kN);  // vectors a lane has in a stretch
-    for (long long row = blockIdx.x / size; row < a.rows; row += gridDim.x / size) {
-        const Reader<L> in(static_cast<const L*>(a.logits) + row * a.ld_logits, V);
-        const Row r = row_of(a, row);
-        const int stretches = (in.vectors + 32 * per - 1) / (32 * per);
-        // this CTA's stretches, a warp each in turn
-        const int from = static_cast<int>(static_cast<long long>(stretches) * group.rank / size);
-        const int to = static_cast<int>(static_cast<long long>(stretches) * (group.rank + 1) / size);
-        const int steps = max(0, (to - from - warp + kWarps - 1) / kWarps) * per;  // vectors of this lane
-        const int slot_steps = (((to - from + kWarps - 1) / kWarps) * per + kSlots - 1) / kSlots;
-        auto vector_of = [&](int step) {
-            return ((from + warp + kWarps * (step / per)) * per + step % per) * 32 + lane;
-        };
-        // ---- the one pass over the row: group maxima and the maximum ----
-        float best = -INFINITY;
-        for (int slot = 0; slot < kSlots; ++slot) {
-            float m = -INFINITY;
-            const int end = min(steps, (slot + 1) * slot_steps);
-#pragma unroll 4
-            for (int i = slot * slot_steps; i < end; ++i) {
-                const int b = vector_of(i);
-                if (b < in.vectors) {
-                    float v[kN];
-                    in.load(b, v);
-#pragma unroll
-                    for (int e = 0; e < kN; ++e) m = fmaxf(m, v[e]);
-                }
-            }
-            sh->maxima[slot][tid] = m;
-            best = fmaxf(best, m);
-        }
-        best = value_of(group.max_key(key_of(best)));
-        if (best == -INFINITY || !r.valid) {
-            if (tid == 0 && group.rank == 0) {
-                a.tokens[row] = -1;
-                if (a.log_probs) a.log_probs[row] = -INFINITY;
-                if (!r.valid && a.health) atomicOr(a.health, kHealthIndex);
-            }
-            continue;
-        }
-        const float per_bin = kBins / kReach;
-        auto bin_of = [&](float v) {  // bin 0 holds the best token; -inf and what has no weight: the last
-            const float at = (best - v) * r.inverse * per_bin;
-            return at < kBins - 1 ? static_cast<int>(at) : kBins - 1;
-        };
-        auto clear = [&]() {
-            for (int i = tid; i < kBins; i += kT) {
-                sh->mass[i] = 0;
-                sh->count[i] = 0;
-            }
-        };
-        // totals of a bin over the cluster
-        auto bin_total = [&](int i) {
-            Sum t{sh->count[i], sh->mass[i]};
-            if (size > 1) {
-                t = Sum{0, 0};
-                for (int c = 0; c < size; ++c) {
-                    t.count += load32(peer(&sh->count[i], c));
-                    t.mass += load64(peer(&sh->mass[i], c));
-                }
-            }
-            return t;
-        };
-        // The first bin up to which (itself included) the count, or the weight, reaches the limit; what is before
-        // it; the whole. kBins where none does. The histogram is complete and stays.
-        auto find_bin = [&](bool by_mass, double limit, Sum& before, Sum& whole) {
-            constexpr int kEach = kBins / kT;
-            Sum mine[kEach], s{0, 0};
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                mine[e] = bin_total(tid * kEach + e);
-                s.count += mine[e].count;
-                s.mass += mine[e].mass;
-            }
-            if (tid == 0) sh->found = kBins;
-            Sum at = block_scan(sh, s, whole);
-            auto value = [&](Sum x) { return by_mass ? static_cast<double>(x.mass) : static_cast<double>(x.count); };
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const Sum next{at.count + mine[e].count, at.mass + mine[e].mass};
-                if (value(at) < limit && value(next) >= limit) {
-                    sh->found = tid * kEach + e;
-                    sh->found_count = at.count;
-                    sh->found_mass = at.mass;
-                }
-                at = next;
-            }
-            __syncthreads();
-            before = Sum{sh->found_count, sh->found_mass};
-            const int bin = sh->found;
-            __syncthreads();
-            return bin;
-        };
-        // List of the tokens of weight in a range of values; false where it does not fit on some CTA.
-        auto push = [&](float v, int token) {
-            const int at = atomicAdd(&sh->listed, 1);
-            if (at < kList) {
-                sh->value[at] = v;
-                sh->index[at] = token;
-            }
-        };
-        const bool cut_k = r.top_k > 0 && r.top_k < V;
-        const bool first_only = r.greedy || r.top_p <= 0.0f || (cut_k && r.top_k == 1);
+__device__ __forceinline__ L most(uint4 x);
+template <>
+__device__ __forceinline__ float most<float>(uint4 x) {
+    return fmaxf(fmaxf(__uint_as_float(x.x), __uint_as_float(x.y)), fmaxf(__uint_as_float(x.z), __uint_as_float(x.w)));
+}
+template <>
+__device__ __forceinline__ __half most<__half>(uint4 x) {
+    const __half2* h = reinterpret_cast<const __half2*>(&x);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return __hmax(__low2half(m), __high2half(m));
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 most<__nv_bfloat16>(uint4 x) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return __hmax(__low2bfloat16(m), __high2bfloat16(m));
+}
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ __half larger(__half a, __half b) { return __hmax(a, b); }
+__device__ __forceinline__ __nv_bfloat16 larger(__nv_bfloat16 a, __nv_bfloat16 b) { return __hmax(a, b); }
 
-        // ---- the bound on the candidates ----
-        int bound = kBins - 1;
-        Sum before, whole;
-        if (first_only) {
-            bound = 0;
-        } else {
-            if (cut_k) {
-                clear();
-                group.sync();
-                for (int slot = 0; slot < kSlots; ++slot) {
-                    const float m = sh->maxima[slot][tid];
-                    if (m != -INFINITY) atomicAdd(&sh->count[bin_of(m)], 1u);
-                }
-                group.sync();
-                bound = min(bound, find_bin(false, r.top_k, before, whole));
-                group.sync();
-            }
-            if (r.top_p >= 1.0f && r.min_p > 0.0f)  // one bin of slack for the rounding of the logarithm
-                bound = min(bound, static_cast<int>(min(-logf(r.min_p) * per_bin + 1.0f, kBins - 1.0f)));
+// One row as a CTA of its cluster sees it: stretches [from, to) are this CTA's, a warp each in turn.
+template <typename L>
+struct Work {
+    static constexpr int kN = Reader<L>::kN;
+    static constexpr int kSlots = 64 / sizeof(L);  // group maxima per thread: 64 bytes of them
+    Shared* sh;
+    Cluster group;
+    Reader<L> in;
+    Row r;
+    int shift, log_per;    // log2 of the tokens of a stretch, and of a lane's vectors in it
+    int from, to;
+    int steps, slot_steps; // vectors of this lane; of one of its groups
+    float best, per_value; // bins a unit of value below the best
+    bool cut_k, first_only;
+
+    __device__ __forceinline__ int vectors_of(int warp) const { return max(0, (to - from - warp + kWarps - 1) / kWarps) << log_per; }
+    __device__ __forceinline__ int vector_of(int warp, int lane, int step) const {
+        return (((from + warp + kWarps * (step >> log_per)) << log_per) + (step & ((1 << log_per) - 1))) * 32 + lane;
+    }
+    // bin 0 holds the best token; -inf and what has no weight: the last
+    __device__ __forceinline__ int bin_of(float v) const {
+        const float at = (best - v) * per_value;
+        return at < kBins - 1 ? static_cast<int>(at) : kBins - 1;
+    }
+    template <typename F>
+    __device__ __forceinline__ void every(F&& f) const {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        for (int i = 0; i < steps; ++i) {
+            const int b = vector_of(warp, lane, i);
+            if (b >= in.vectors) break;
+            float x[kN];
+            in.load(b, x);
+#pragma unroll
+            for (int e = 0; e < kN; ++e) f(x[e], in.first(b) + e);
         }
-        float v[kPer];
-        uint32_t w[kPer];
-        auto take_list = [&]() {
+    }
+    // hands the first CTA's sh->found to the others; a barrier
+    __device__ __forceinline__ void share_found() {
+        __syncthreads();
+        if (group.size > 1) {
+            constexpr int kWords = sizeof(Found) / 4;
+            if (group.rank == 0)
+                for (int i = threadIdx.x; i < kWords * static_cast<int>(group.size - 1); i += kT) {
+                    const uint32_t* word = reinterpret_cast<const uint32_t*>(&sh->found) + i % kWords;
+                    store32(peer(word, 1 + i / kWords), *word);
+                }
+            group.sync();
+        }
+    }
+    // adds the cluster's histograms on its first CTA: bins [0, n); a barrier
+    __device__ __forceinline__ void merge(int n) {
+        group.sync();
+        if (group.size > 1) {
+            if (group.rank != 0)
+                for (int i = threadIdx.x; i < n; i += kT) {
+                    if (const uint32_t c = sh->count[i]) add32(peer(&sh->count[i], 0), c);
+                    if (const u64 m = sh->mass[i]) add64(peer(&sh->mass[i], 0), m);
+                }
+            group.sync();
+        }
+    }
+    // The bin of the merged histogram at which the limit (or `share` of the whole weight) is reached; on every CTA.
+    __device__ __forceinline__ Found search(bool by_mass, double limit, bool share) {
+        if (group.rank == 0) {
+            Sum mine[kEach], whole;
+            const Sum at = scan_histogram(sh, mine, whole);
+            if (threadIdx.x == 0) {
+                sh->found.bin = kBins;
+                sh->found.whole = whole;
+            }
+            __syncthreads();
+            find_bin(sh, by_mass, share ? limit * static_cast<double>(whole.mass) : limit, mine, at);
+        }
+        share_found();
+        const Found f = sh->found;
+        group.sync();  // read by all before it is written again
+        return f;
+    }
+};
+
+// Group maxima and the row's maximum: the one pass over the row.
+template <typename L>
+__device__ __forceinline__ float read_row(const Work<L>& work) {
+    constexpr int kN = Work<L>::kN, kSlots = Work<L>::kSlots;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    L* maxima = reinterpret_cast<L*>(work.sh->maxima);
+    const Reader<L>& in = work.in;
+    const L none = L(-INFINITY);
+    L m = none, all = none;
+    int slot = 0, left = work.slot_steps;
+    auto put = [&](L x) {
+        m = larger(m, x);
+        if (--left == 0) {
+            all = larger(all, m);
+            maxima[slot++ * kT + tid] = m;
+            m = none;
+            left = work.slot_steps;
+        }
+    };
+    auto edge = [&](int i) {  // a vector that may lie across an end of the row
+        const int j = in.first(work.vector_of(warp, lane, i));
+        L x = none;
+        for (int e = max(0, -j); e < kN && j + e < in.vocab; ++e) x = larger(x, in.s[j + e]);
+        return x;
+    };
+    constexpr int kAhead = 8;  // loads in flight
+    int i = 0;
+    for (; i + kAhead <= work.steps; i += kAhead) {
+        if (in.inside(work.vector_of(warp, 0, i)) && in.inside(work.vector_of(warp, 0, i + kAhead - 1))) {
+            uint4 x[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) x[k] = in.raw(work.vector_of(warp, lane, i + k));
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) put(most<L>(x[k]));
+        } else {
+            for (int k = 0; k < kAhead; ++k) put(edge(i + k));
+        }
+    }
+    for (; i < work.steps; ++i) put(in.inside(work.vector_of(warp, 0, i)) ? most<L>(in.raw(work.vector_of(warp, lane, i))) : edge(i));
+    all = larger(all, m);
+    for (; slot < kSlots; ++slot) {
+        maxima[slot * kT + tid] = m;
+        m = none;
+    }
+    return clean(to_float(all));
+}
+
+// The list of the tokens in bins [0, bound], on the cluster's first CTA: whether it fits.
+template <typename L>
+__device__ __forceinline__ bool build_list(Work<L>& work, int bound) {
+    constexpr int kN = Work<L>::kN, kSlots = Work<L>::kSlots;
+    const int tid = threadIdx.x;
+    Shared* sh = work.sh;
+    const Reader<L>& in = work.in;
+    const L* maxima = reinterpret_cast<const L*>(sh->maxima);
+    uint16_t* groups = reinterpret_cast<uint16_t*>(sh->mass);
+    const float best = work.best, per_value = work.per_value, limit = static_cast<float>(bound + 1);
+    // bin_of(v) <= bound, without cleaning: NaN fails, +inf passes
+    auto passes = [&](float v) { return (best - v) * per_value < limit; };
+    if (tid == 0) sh->listed = sh->groups = 0;
+    __syncthreads();
+    // groups with a candidate, then their tokens, both appended a warp at a time
+    uint32_t passed = 0;
+#pragma unroll
+    for (int slot = 0; slot < kSlots; ++slot) passed |= (passes(to_float(maxima[slot * kT + tid])) ? 1u : 0u) << slot;
+    int at = append(&sh->groups, __popc(passed));
+    for (; passed; passed &= passed - 1, ++at)
+        if (at < kList) groups[at] = static_cast<uint16_t>((__ffs(passed) - 1) * kT + tid);
+    __syncthreads();
+    if (sh->groups <= kList) {  // each group has a token
+        const int n = sh->groups * work.slot_steps;  // vectors to read again
+        constexpr int kAhead = 4;
+        for (int i0 = 0; i0 < n; i0 += kAhead * kT) {
+            uint4 x[kAhead];
+            int first[kAhead];  // token of the vector's first element
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = i0 + k * kT + tid;
+                first[k] = in.vocab;
+                if (i < n) {
+                    const int g = work.slot_steps == 1 ? groups[i] : groups[i / work.slot_steps];
+                    const int step = (g / kT) * work.slot_steps + (work.slot_steps == 1 ? 0 : i % work.slot_steps);
+                    const int its_warp = (g & (kT - 1)) >> 5;
+                    if (step < work.vectors_of(its_warp)) {
+                        const int b = work.vector_of(its_warp, g & 31, step);
+                        first[k] = in.first(b);
+                        if (in.whole(first[k])) x[k] = in.raw(b);
+                    }
+                }
+            }
+            uint32_t has = 0;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (in.whole(first[k])) {
+                    L y[kN];
+                    *reinterpret_cast<uint4*>(y) = x[k];
+#pragma unroll
+                    for (int e = 0; e < kN; ++e) has |= (passes(to_float(y[e])) ? 1u : 0u) << (k * kN + e);
+                } else {
+                    for (int e = max(0, -first[k]); e < kN && first[k] + e < in.vocab; ++e)
+                        has |= (passes(to_float(in.s[first[k] + e])) ? 1u : 0u) << (k * kN + e);
+                }
+            }
+            int slot = append(&sh->listed, __popc(has));
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                for (uint32_t here = (has >> (k * kN)) & ((1u << kN) - 1); here; here &= here - 1, ++slot)
+                    if (slot < kList) {
+                        const int j = first[k] + __ffs(here) - 1;
+                        sh->value[slot] = in.at(j);
+                        sh->index[slot] = j;
+                    }
+        }
+    } else if (tid == 0) {
+        sh->listed = kList + 1;
+    }
+    work.group.sync();
+    const int size = static_cast<int>(work.group.size);
+    if (size == 1) return sh->listed <= kList;
+    int before = 0, all = 0;
+    for (int c = 0; c < size; ++c) {
+        const int n_c = static_cast<int>(load32(peer(&sh->listed, c)));
+        if (c < static_cast<int>(work.group.rank)) before += n_c;
+        all = min(all + n_c, kList + 1);
+    }
+    const int own = sh->listed;
+    if (all <= kList && work.group.rank != 0)
+        for (int i = tid; i < own; i += kT) {
+            store32(peer(&sh->value[before + i], 0), __float_as_uint(sh->value[i]));
+            store32(peer(&sh->index[before + i], 0), static_cast<uint32_t>(sh->index[i]));
+        }
+    work.group.sync();
+    if (tid == 0) sh->listed = all;
+    __syncthreads();
+    return all <= kList;
+}
+
+// The cut of all tokens: histogram, then the list of the cut's bin; a bin that does not fit is divided
+// again between its own extremes, by keys. `limit` receives the limit (a share: of the whole weight).
+template <typename L>
+__device__ __noinline__ Cut wide_cut(Work<L>& work, bool by_mass, double& limit, bool share) {
+    Shared* sh = work.sh;
+    const int tid = threadIdx.x;
+    const float best = work.best, inverse = work.r.inverse;
+    float high = best, low = -INFINITY;
+    uint32_t width = 1;  // keys a bin, after the first division
+    Sum above{0, 0};
+    for (bool first = true;; first = false) {
+        // bin of a token of weight in the range divided; -1 elsewhere
+        auto bin_in = [&](float x, uint32_t& w) {
+            if (!(x >= low && x <= high)) return -1;
+            w = static_cast<uint32_t>(weight_of(exp_of(x, best, inverse)));
+            if (!w) return -1;
+            return first ? work.bin_of(x) : static_cast<int>((key_of(high) - key_of(x)) / width);
+        };
+        clear_histogram(sh);
+        work.group.sync();
+        work.every([&](float x, int) {
+            uint32_t w;
+            const int bin = bin_in(x, w);
+            if (bin < 0) return;
+            atomicAdd(&sh->count[bin], 1u);
+            atomicAdd(&sh->mass[bin], static_cast<u64>(w));
+        });
+        work.merge(kBins);
+        const Found f = work.search(by_mass, first ? limit : limit - (by_mass ? static_cast<double>(above.mass) : static_cast<double>(above.count)),
+                                    first && share);
+        if (first && share) limit *= static_cast<double>(f.whole.mass);
+        if (f.bin == kBins) return Cut{-INFINITY, f.whole};  // fewer tokens of weight than top-k asks for
+        above.count += f.before.count;
+        above.mass += f.before.mass;
+        if (tid == 0) sh->listed = 0;
+        work.group.sync();
+        if (f.here.count <= kList) {
+            work.every([&](float x, int) {
+                uint32_t w;
+                if (bin_in(x, w) != f.bin) return;
+                sh->value[atomicAdd(&sh->listed, 1)] = x;
+            });
+            __syncthreads();
+            float v[kPer];
+            uint32_t w[kPer];
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int at = i * kT + tid;
                 v[i] = at < sh->listed ? sh->value[at] : -INFINITY;
-                w[i] = at < sh->listed ? static_cast<uint32_t>(weight_of(exp_of(v[i], best, r.inverse))) : 0u;
+                w[i] = at < sh->listed ? static_cast<uint32_t>(weight_of(exp_of(v[i], best, inverse))) : 0u;
             }
-        };
-        bool listed = false;
-        if (bound < kBins - 1) {
-            if (tid == 0) sh->listed = 0;
-            __syncthreads();
-            for (int slot = 0; slot < kSlots; ++slot) {
-                if (bin_of(sh->maxima[slot][tid]) > bound) continue;
-                const int end = min(steps, (slot + 1) * slot_steps);
-                for (int i = slot * slot_steps; i < end; ++i) {
-                    const int b = vector_of(i);
-                    if (b >= in.vectors) break;
-                    float x[kN];
-                    in.load(b, x);
-#pragma unroll
-                    for (int e = 0; e < kN; ++e)
-                        if (bin_of(x[e]) <= bound) push(x[e], b * kN + e - in.mis);
-                }
-            }
-            __syncthreads();
-            listed = group.max_key(sh->listed > kList ? 1u : 0u) == 0;
+            return by_mass ? find_cut<true>(work.group, v, w, limit, above) : find_cut<false>(work.group, v, w, limit, above);
         }
-        Kept kept{-INFINITY, 0};
-        if (listed) {
-            take_list();
-            Sum all{0, 0};
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                all.count += w[i] != 0;
-                all.mass += w[i];
+        uint32_t up = 0, down = 0;
+        work.every([&](float x, int) {
+            uint32_t w;
+            if (bin_in(x, w) != f.bin) return;
+            up = max(up, key_of(x));
+            down = max(down, ~key_of(x));
+        });
+        high = value_of(work.group.max_key(up));
+        low = value_of(~work.group.max_key(down));
+        if (high == low) return Cut{high, above};
+        width = (key_of(high) - key_of(low)) / kBins + 1;  // the ends never share a bin: each division gains
+    }
+}
+
+// Cuts and draw from the whole row.
+template <typename L>
+__device__ __noinline__ void draw_wide(Work<L>& work, const rl2_sample_args& a, long long row) {
+    constexpr int kN = Work<L>::kN;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    Shared* sh = work.sh;
+    const Row r = work.r;
+    const float best = work.best;
+    const Reader<L>& in = work.in;
+    const int shift = work.shift, per = 1 << work.log_per;
+    Kept kept{-INFINITY, 0};
+    if (work.first_only) {
+        kept = Kept{best, 1};
+    } else {
+        Sum above{0, 0};
+        u64 total = 0;
+        double limit = 0.0;
+        bool have_k = false;
+        if (work.cut_k) {
+            limit = r.top_k;
+            const Cut c = wide_cut(work, false, limit, false);
+            above = c.above;
+            total = c.above.mass;
+            if (c.value != -INFINITY) {
+                have_k = true;
+                kept = Kept{c.value, static_cast<u64>(r.top_k) - c.above.count};
+                total += kept.ties * weight_of(exp_of(kept.cut, best, r.inverse));
             }
-            all = group.sum(all);
-            kept = both_cuts(group, r, V, best, v, w, all);
-        } else if (first_only) {
-            kept = Kept{best, 1};
-        } else if (cut_k || r.top_p < 1.0f) {
-            // ---- cuts from a histogram of every token ----
-            auto every = [&](auto&& f) {
-                for (int i = 0; i < steps; ++i) {
-                    const int b = vector_of(i);
-                    if (b >= in.vectors) break;
-                    float x[kN];
-                    in.load(b, x);
-#pragma unroll
-                    for (int e = 0; e < kN; ++e) f(x[e], b * kN + e - in.mis);
-                }
-            };
-            // The cut of all tokens: histogram over [.., high], then the list of the cut's bin; a bin that does
-            // not fit is divided again between its own extremes.
-            auto wide_cut = [&](bool by_mass, double limit_or_share, bool is_share, double& limit) {
-                float high = best, low = -INFINITY, scale = r.inverse * per_bin;
-                Sum above{0, 0};
-                for (bool first = true;; first = false) {
-                    auto bin_in = [&](float x) {
-                        const float at = (high - x) * scale;
-                        return at < kBins - 1 ? static_cast<int>(at) : kBins - 1;
-                    };
-                    auto inside = [&](float x) { return x >= low && x <= high; };
-                    clear();
-                    group.sync();
-                    every([&](float x, int) {
-                        if (!inside(x)) return;
-                        const u64 weight = weight_of(exp_of(x, best, r.inverse));
-                        if (!weight) return;
-                        const int bin = bin_in(x);
-                        atomicAdd(&sh->count[bin], 1u);
-                        atomicAdd(&sh->mass[bin], weight);
-                    });
-                    group.sync();
-                    Sum part, all;
-                    if (first && is_share) {
-                        find_bin(by_mass, 0.0, part, all);
-                        limit = limit_or_share * static_cast<double>(all.mass);
-                    } else if (first) {
-                        limit = limit_or_share;
-                    }
-                    const double rest = limit - (by_mass ? static_cast<double>(above.mass) : static_cast<double>(above.count));
-                    const int bin = find_bin(by_mass, rest, part, all);
-                    if (bin == kBins) {  // fewer tokens of weight than top-k asks for
-                        group.sync();
-                        return Cut{-INFINITY, all};
-                    }
-                    above.count += part.count;
-                    above.mass += part.mass;
-                    const Sum here = bin_total(bin);
-                    if (tid == 0) sh->listed = 0;
-                    group.sync();
-                    if (here.count <= kList) {
-                        every([&](float x, int token) {
-                            if (inside(x) && bin_in(x) == bin && weight_of(exp_of(x, best, r.inverse))) push(x, token);
-                        });
-                        __syncthreads();
-                        take_list();
-                        return by_mass ? find_cut<true>(group, v, w, limit, above) : find_cut<false>(group, v, w, limit, above);
-                    }
-                    uint32_t up = 0, down = 0;
-                    every([&](float x, int) {
-                        if (inside(x) && bin_in(x) == bin && weight_of(exp_of(x, best, r.inverse))) {
-                            up = max(up, key_of(x));
-                            down = max(down, ~key_of(x));
-                        }
-                    });
-                    high = value_of(group.max_key(up));
-                    low = value_of(~group.max_key(down));
-                    if (high == low) return Cut{high, above};
-                    // at most kBins - 1 for the lowest, so the ends never share a bin
-                    scale = fminf((kBins - 1) / (high - low), FLT_MAX);
-                }
-            };
-            Sum above{0, 0};
-            u64 total = 0;
-            double limit = 0.0;
-            bool have_k = false;
-            if (cut_k) {
-                const Cut c = wide_cut(false, r.top_k, false, limit);
+        }
+        if (r.top_p < 1.0f) {
+            u64 most = kept.ties;
+            limit = static_cast<double>(r.top_p) * (work.cut_k ? static_cast<double>(total) : 1.0);
+            if (!have_k || !(static_cast<double>(above.mass) < limit)) {
+                const Cut c = wide_cut(work, true, limit, !work.cut_k);
+                kept.cut = c.value;
                 above = c.above;
-                total = c.above.mass;
-                if (c.value != -INFINITY) {
-                    have_k = true;
-                    kept = Kept{c.value, static_cast<u64>(r.top_k) - c.above.count};
-                    total += kept.ties * weight_of(exp_of(kept.cut, best, r.inverse));
-                }
+                most = ~0ull;
             }
-            if (r.top_p < 1.0f) {
-                u64 most = kept.ties;
-                limit = static_cast<double>(r.top_p) * static_cast<double>(total);
-                if (!have_k || !(static_cast<double>(above.mass) < limit)) {
-                    const Cut c = have_k || cut_k ? wide_cut(true, limit, false, limit) : wide_cut(true, r.top_p, true, limit);
-                    kept.cut = c.value;
-                    above = c.above;
-                    most = ~0ull;
-                }
-                if (kept.cut != -INFINITY)
-                    kept.ties = kept_of_last(above.mass, weight_of(exp_of(kept.cut, best, r.inverse)), limit, most);
+            if (kept.cut != -INFINITY)
+                kept.ties = kept_of_last(above.mass, weight_of(exp_of(kept.cut, best, r.inverse)), limit, most);
+        }
+    }
+    // kept weight above the cut and tokens at it, by stretch
+    auto weigh = [&](float x) {
+        if (r.greedy) return static_cast<u64>(1);
+        const float e = exp_of(x, best, r.inverse);
+        return e >= r.min_p ? weight_of(e) : 0;
+    };
+    const u64 tie_weight = kept.ties ? weigh(kept.cut) : 0;
+    work.group.sync();
+    clear_histogram(sh);
+    work.group.sync();
+    for (int st = work.from + warp; st < work.to; st += kWarps) {
+        u64 mass = 0;
+        uint32_t ties = 0;
+        for (int i = 0; i < per; ++i) {
+            const int b = (st * per + i) * 32 + lane;
+            if (b >= in.vectors) break;
+            float x[kN];
+            in.load(b, x);
+#pragma unroll
+            for (int e = 0; e < kN; ++e) {
+                if (x[e] > kept.cut) mass += weigh(x[e]);
+                ties += x[e] == kept.cut;
             }
         }
-        // ---- the draw: kept weight above the cut and tokens at it, by stretch ----
-        auto weigh = [&](float x) {
-            if (r.greedy) return static_cast<u64>(1);
-            const float e = exp_of(x, best, r.inverse);
-            return e >= r.min_p ? weight_of(e) : 0;
-        };
-        const u64 tie_weight = kept.ties ? weigh(kept.cut) : 0;
-        group.sync();
-        clear();
-        group.sync();
-        if (listed) {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int at = i * kT + tid;
-                if (at < sh->listed && v[i] >= kept.cut) {
-                    const int b = (sh->index[at] + in.mis) >> shift;
-                    if (v[i] == kept.cut)
-                        atomicAdd(&sh->count[b], 1u);
-                    else
-                        atomicAdd(&sh->mass[b], weigh(v[i]));
-                }
-            }
-        } else {
-            for (int st = from + warp; st < to; st += kWarps) {
-                u64 mass = 0;
-                uint32_t ties = 0;
-                for (int i = 0; i < per; ++i) {
-                    const int b = (st * per + i) * 32 + lane;
-                    if (b >= in.vectors) break;
-                    float x[kN];
-                    in.load(b, x);
-#pragma unroll
-                    for (int e = 0; e < kN; ++e) {
-                        if (x[e] > kept.cut) mass += weigh(x[e]);
-                        ties += x[e] == kept.cut;
-                    }
-                }
-                mass = warp_sum64(mass);
-                ties = __reduce_add_sync(0xffffffffu, ties);
-                if (lane == 0) {
-                    sh->mass[st] = mass;
-                    sh->count[st] = ties;
-                }
-            }
+        mass = warp_sum64(mass);
+        ties = __reduce_add_sync(0xffffffffu, ties);
+        if (lane == 0) {
+            sh->mass[st] = mass;
+            sh->count[st] = ties;
         }
-        group.sync();
-        constexpr int kEach = kStretches / kT;
-        Sum mine[kEach], s{0, 0}, all;
+    }
+    work.merge(kStretches);
+    if (work.group.rank == 0) {
+        constexpr int kEachStretch = kStretches / kT;
+        Sum mine[kEachStretch], s{0, 0}, all;
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            mine[e] = bin_total(tid * kEach + e);
+        for (int e = 0; e < kEachStretch; ++e) {
+            mine[e] = Sum{sh->count[tid * kEachStretch + e], sh->mass[tid * kEachStretch + e]};
             s.count += mine[e].count;
             s.mass += mine[e].mass;
         }
@@ -775,80 +1200,129 @@ __global__ void __launch_bounds__(kT, 2) row_kernel(const rl2_sample_args a, con
         const u64 total = all.mass + min(static_cast<u64>(all.count), kept.ties) * tie_weight;
         const u64 target = target_of(r.uniform, total);
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            // before this stretch, and through it
+        for (int e = 0; e < kEachStretch; ++e) {
+            // kept weight before this stretch, and through it
             const u64 cum = at.mass + min(static_cast<u64>(at.count), kept.ties) * tie_weight;
-            at.count += mine[e].count;
-            at.mass += mine[e].mass;
-            const u64 next = at.mass + min(static_cast<u64>(at.count), kept.ties) * tie_weight;
-            if (cum <= target && target < next) {
-                sh->found = tid * kEach + e;
-                sh->found_mass = cum;
-                sh->found_count = at.count - mine[e].count;
-            }
+            const Sum next{at.count + mine[e].count, at.mass + mine[e].mass};
+            if (cum <= target && target < next.mass + min(static_cast<u64>(next.count), kept.ties) * tie_weight)
+                sh->found = Found{mine[e], Sum{at.count, cum}, Sum{0, total}, tid * kEachStretch + e, 0};
+            at = next;
         }
-        __syncthreads();
-        const int chosen = sh->found;
-        const u64 start = sh->found_mass;
-        const u64 ties_seen = sh->found_count;
-        // the CTA that owns the stretch draws within it
-        if (chosen >= from && chosen < to) {
-            for (int i = tid; i < (1 << shift); i += kT) {
-                sh->slot_w[i] = 0;
-                sh->slot_tie[i] = 0;
-            }
-            __syncthreads();
-            if (listed) {
-                for (int i = tid; i < sh->listed; i += kT) {
-                    const float x = sh->value[i];
-                    const int j = sh->index[i] + in.mis;
-                    if ((j >> shift) == chosen && x >= kept.cut) {
-                        sh->slot_w[j & ((1 << shift) - 1)] = static_cast<uint32_t>(weigh(x));
-                        sh->slot_tie[j & ((1 << shift) - 1)] = x == kept.cut;
-                    }
-                }
-            } else {
-                for (int i = tid; i < 32 * per; i += kT) {
-                    const int b = chosen * per * 32 + i;
-                    if (b >= in.vectors) break;
-                    float x[kN];
-                    in.load(b, x);
+    }
+    work.share_found();
+    const int chosen = sh->found.bin;
+    const u64 start = sh->found.before.mass, ties_seen = sh->found.before.count, total = sh->found.whole.mass;
+    const u64 target = target_of(r.uniform, total);
+    if (chosen < work.from || chosen >= work.to) return;
+    // the CTA that owns the stretch draws within it
+    for (int i = tid; i < (1 << shift); i += kT) {
+        sh->slot_w[i] = 0;
+        sh->slot_tie[i] = 0;
+    }
+    __syncthreads();
+    for (int i = tid; i < 32 * per; i += kT) {
+        const int b = chosen * per * 32 + i;
+        if (b >= in.vectors) break;
+        float x[kN];
+        in.load(b, x);
 #pragma unroll
-                    for (int e = 0; e < kN; ++e) {
-                        sh->slot_w[i * kN + e] = x[e] > kept.cut || (x[e] == kept.cut && kept.ties) ? static_cast<uint32_t>(weigh(x[e])) : 0u;
-                        sh->slot_tie[i * kN + e] = x[e] == kept.cut;
-                    }
-                }
-            }
-            __syncthreads();
-            if (warp == 0) {
-                u64 cum = start, left = kept.ties - min(kept.ties, ties_seen);
-                for (int i = lane; i < (1 << shift); i += 32) {
-                    uint32_t mine_w = sh->slot_w[i];
-                    const bool tie = sh->slot_tie[i];
-                    const uint32_t tied = __ballot_sync(0xffffffffu, tie);
-                    if (tie && __popc(tied & ((1u << lane) - 1)) >= left) mine_w = 0;
-                    left -= min(left, static_cast<u64>(__popc(tied)));
-                    const u64 step = warp_sum64(mine_w);
-                    if (cum + step > target) {
-                        u64 sum = mine_w;
-#pragma unroll
-                        for (int o = 1; o < 32; o <<= 1) {
-                            const u64 up = __shfl_up_sync(0xffffffffu, sum, o);
-                            if (lane >= o) sum += up;
-                        }
-                        const uint32_t hit = __ballot_sync(0xffffffffu, cum + sum > target);
-                        if (lane == __ffs(hit) - 1) {
-                            a.tokens[row] = (chosen << shift) + i - in.mis;
-                            if (a.log_probs) a.log_probs[row] = log_share(mine_w, total);
-                        }
-                        break;
-                    }
-                    cum += step;
-                }
-            }
+        for (int e = 0; e < kN; ++e) {
+            sh->slot_w[i * kN + e] = x[e] > kept.cut || (x[e] == kept.cut && kept.ties) ? static_cast<uint32_t>(weigh(x[e])) : 0u;
+            sh->slot_tie[i * kN + e] = x[e] == kept.cut;
         }
-        group.sync();
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    u64 cum = start, left = kept.ties - min(kept.ties, ties_seen);
+    for (int i = lane; i < (1 << shift); i += 32) {
+        uint32_t mine = sh->slot_w[i];
+        const bool tie = sh->slot_tie[i];
+        const uint32_t tied = __ballot_sync(0xffffffffu, tie);
+        if (tie && __popc(tied & ((1u << lane) - 1)) >= left) mine = 0;
+        left -= min(left, static_cast<u64>(__popc(tied)));
+        const u64 step = warp_sum64(mine);
+        if (cum + step > target) {
+            u64 sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 up = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += up;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, cum + sum > target);
+            if (lane == __ffs(hit) - 1) {
+                a.tokens[row] = (chosen << shift) + i - in.mis;
+                if (a.log_probs) a.log_probs[row] = log_share(mine, total);
+            }
+            return;
+        }
+        cum += step;
+    }
+}
+
+template <typename L>
+__global__ void __launch_bounds__(kT, 2) row_kernel(const rl2_sample_args a, const int size, const int shift) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    Shared* sh = reinterpret_cast<Shared*>(raw);
+    constexpr int kN = Work<L>::kN, kSlots = Work<L>::kSlots;
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const int V = a.vocab;
+    const uint32_t rank = size > 1 ? ptx::cluster_rank() : 0u;
+    for (long long row = blockIdx.x / size; row < a.rows; row += gridDim.x / size) {
+        const Reader<L> in(static_cast<const L*>(a.logits) + row * a.ld_logits, V);
+        const int log_per = shift - 5 - (kN == 8 ? 3 : 2);
+        const int stretches = (in.vectors + (32 << log_per) - 1) >> (5 + log_per);
+        Work<L> work{sh, Cluster{sh, static_cast<uint32_t>(size), rank, 0}, in, row_of(a, row), shift, log_per,
+                     static_cast<int>(static_cast<long long>(stretches) * rank / size),
+                     static_cast<int>(static_cast<long long>(stretches) * (rank + 1) / size), 0, 0, 0.0f, 0.0f, false, false};
+        work.steps = work.vectors_of(warp);
+        work.slot_steps = max(1, (work.vectors_of(0) + kSlots - 1) / kSlots);
+        work.best = value_of(work.group.max_key(key_of(read_row(work))));
+        if (work.best == -INFINITY || !work.r.valid) {
+            if (tid == 0 && rank == 0) {
+                a.tokens[row] = -1;
+                if (a.log_probs) a.log_probs[row] = -INFINITY;
+                if (!work.r.valid && a.health) atomicOr(a.health, kHealthIndex);
+            }
+            work.group.sync();
+            continue;
+        }
+        const Row& r = work.r;
+        work.per_value = fminf(r.inverse * (kBins / kReach), FLT_MAX);
+        work.cut_k = r.top_k > 0 && r.top_k < V;
+        work.first_only = r.greedy || r.top_p <= 0.0f || (work.cut_k && r.top_k == 1);
+        // ---- the bound on the candidates ----
+        int bound = kBins - 1;
+        if (work.first_only) {
+            bound = 0;
+        } else {
+            if (work.cut_k) {
+                clear_histogram(sh);
+                work.group.sync();
+                const L* maxima = reinterpret_cast<const L*>(sh->maxima);
+#pragma unroll
+                for (int slot = 0; slot < kSlots; ++slot) {
+                    const int bin = work.bin_of(clean(to_float(maxima[slot * kT + tid])));
+                    if (bin < kBins - 1) atomicAdd(&sh->count[bin], 1u);
+                }
+                work.merge(kBins);
+                bound = min(bound, work.search(false, r.top_k, false).bin);
+            }
+            if (r.top_p >= 1.0f && r.min_p > 0.0f)  // one bin of slack for the rounding of the logarithm
+                bound = min(bound, static_cast<int>(min(-logf(r.min_p) * (kBins / kReach) + 1.0f, kBins - 1.0f)));
+        }
+        if (bound < kBins - 1 && build_list(work, bound)) {
+            if (rank == 0) {
+                const int n = sh->listed;
+                if (n <= kFew) {
+                    if (warp == 0) draw_few(sh, n, r, V, work.best, a, row);
+                } else {
+                    draw_many(sh, n, r, V, work.best, fminf(work.per_value * (static_cast<float>(kBins) / (bound + 1)), FLT_MAX), a, row);
+                }
+            }
+        } else {
+            draw_wide(work, a, row);
+        }
+        work.group.sync();
     }
     if (size > 1) ptx::cluster_sync();  // no CTA leaves while another may read its shared memory
 }

@@ -130,6 +130,27 @@ def test_masks(vocab, dtype):
         assert tokens[0] == -1 and tokens[1] == -1 and tokens[3] == 0 and tokens[10] == vocab - 1
 
 
+@pytest.mark.parametrize("rows,vocab", [(5, 300), (3, 6000), (200, 20000), (2, 140000)])
+def test_temperatures_at_the_ends(rows, vocab):
+    """So low that only the best count, so high that all weigh the same, and what is no normal number."""
+    logits, u = draws(rows, vocab, seed=vocab)
+    for t in (1e-45, 1e-38, 1.5e-38, 1e-36, 1e-30, 1e-4, 1e4, 1e30, INF):
+        gone = dict(temperature=0.0) if t < 2.0 ** -126 else dict(temperature=t)
+        tokens = torch.empty(rows, dtype=torch.int32, device="cuda")
+        for f in (dict(), dict(top_k=7), dict(top_p=0.5), dict(top_k=min(vocab, 900), top_p=0.9), dict(min_p=0.5)):
+            want, _ = check(logits, u, **gone, **f)
+            TokenSampler(rows, vocab).run(logits=logits, uniforms=u, tokens=tokens, temperature=t, **f)
+            assert torch.equal(tokens, want)
+
+
+@pytest.mark.parametrize("rows,vocab,spread", [(2, 20000, 1e-4), (200, 9000, 1e-3), (2, 200000, 1e-38), (100, 70000, 0.5), (1, 50000, 100.0)])
+def test_narrow_and_wide_rows(rows, vocab, spread):
+    """All tokens near one another (one histogram bin holds more than a list), and very far."""
+    logits, u = draws(rows, vocab, seed=3, scale=spread)
+    for f in (dict(), dict(top_k=vocab // 3), dict(top_p=0.5), dict(top_k=5000, top_p=0.3), dict(top_k=100, top_p=0.999), dict(min_p=0.9)):
+        check(logits, u, **f)
+
+
 @pytest.mark.parametrize("vocab", [5, 777, 33333, 150000])
 def test_probabilities_in_64_bits(vocab):
     """The drawn token's interval of the cumulative probabilities, in 64 bits from the definition, holds the
