@@ -268,6 +268,16 @@ def stream_ptr(stream=None) -> int:
     return s.cuda_stream
 
 
+def raw_stream(stream, device_index: int) -> int:
+    """Address of ``stream``, or of the current stream of a device (without building a Stream object: about
+    3 us less a call than ``stream_ptr``)."""
+    if stream is not None:
+        return stream.cuda_stream
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 class ReplayIngestArgs(ctypes.Structure):
     """``rl2_replay_ingest_args`` (include/rl2.h)."""
 

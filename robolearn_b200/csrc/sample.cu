@@ -24,6 +24,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <type_traits>
 
@@ -71,13 +72,14 @@ __device__ __forceinline__ Row row_of(const rl2_sample_args& a, long long row) {
 __device__ __forceinline__ float exp_of(float v, float best, float inverse) { return expf((v - best) * inverse); }
 __device__ __forceinline__ u64 weight_of(float e) { return __float2uint_rn(e * kUnit); }
 
+// The share p of a weight as an integer: a sum is below the product exactly if it is below this.
+__device__ __forceinline__ u64 share_of(float p, u64 total) {
+    return static_cast<u64>(ceil(static_cast<double>(p) * static_cast<double>(total)));
+}
+
 // tokens of the last value that P keeps: those before which less than `limit` of mass stands
-__device__ __forceinline__ u64 kept_of_last(u64 before, u64 w, double limit, u64 count) {
-    if (w == 0) return count;
-    u64 n = static_cast<u64>((limit - static_cast<double>(before)) / static_cast<double>(w));
-    while (n > 0 && static_cast<double>(before + (n - 1) * w) >= limit) --n;
-    while (n < count && static_cast<double>(before + n * w) < limit) ++n;
-    return min(n, count);
+__device__ __forceinline__ u64 kept_of_last(u64 before, u64 w, u64 limit, u64 count) {
+    return w == 0 ? count : min((limit - before + w - 1) / w, count);
 }
 
 __device__ __forceinline__ u64 target_of(float u, u64 total) {
@@ -121,7 +123,7 @@ struct Cut {
 // are not among them. The limit is not reached by `above` alone, and is by all of them. MASS: the
 // limit is on the weight above, else on the count.
 template <bool MASS, int N, typename Group>
-__device__ __forceinline__ Cut find_cut(Group& group, const float (&v)[N], const uint32_t (&w)[N], double limit, Sum above) {
+__device__ __forceinline__ Cut find_cut(Group& group, const float (&v)[N], const uint32_t (&w)[N], u64 limit, Sum above) {
     auto over = [&](float x) {
         Sum s{0, 0};
 #pragma unroll
@@ -133,7 +135,7 @@ __device__ __forceinline__ Cut find_cut(Group& group, const float (&v)[N], const
         s = group.sum(s);
         return Sum{s.count + above.count, s.mass + above.mass};
     };
-    auto less = [&](Sum s) { return (MASS ? static_cast<double>(s.mass) : static_cast<double>(s.count)) < limit; };
+    auto less = [&](Sum s) { return (MASS ? s.mass : static_cast<u64>(s.count)) < limit; };
     // highest and lowest token, as keys (the lowest through the complement)
     auto extremes = [&](float lo, float hi, float& least, float& most) {
         uint32_t up = 0, down = 0;
@@ -177,25 +179,25 @@ struct Kept {
     u64 ties;
 };
 
-// Both cuts of a row whose tokens (at least those that the cuts can reach) are N a thread.
-template <int N, typename Group>
-__device__ __forceinline__ Kept both_cuts(Group& group, const Row& r, int vocab, float best, const float (&v)[N],
-                                          const uint32_t (&w)[N], Sum all) {
-    Kept kept{-INFINITY, 0};
+// Both cuts of a row whose tokens (at least those that the cuts can reach) are N a thread. `given`: the
+// limit of the second where the tokens are not all that weigh, else 0. CUT(by_mass, limit) finds a cut.
+template <typename CUT>
+__device__ __forceinline__ Kept both_cuts(const Row& r, int vocab, float best, Sum all, u64 given, CUT&& cut) {
     if (r.greedy || r.top_p <= 0.0f) return Kept{best, 1};
+    Kept kept{-INFINITY, 0};
     Sum above = all;  // above -inf
     u64 total = all.mass;
     if (r.top_k > 0 && r.top_k < vocab && all.count > static_cast<uint32_t>(r.top_k)) {
-        const Cut c = find_cut<false>(group, v, w, static_cast<double>(r.top_k), Sum{0, 0});
+        const Cut c = cut(std::false_type{}, static_cast<u64>(r.top_k));
         kept = Kept{c.value, static_cast<u64>(r.top_k) - c.above.count};
         above = c.above;
         total = above.mass + kept.ties * weight_of(exp_of(kept.cut, best, r.inverse));
     }
     if (r.top_p < 1.0f) {
-        const double limit = static_cast<double>(r.top_p) * static_cast<double>(total);
+        const u64 limit = given ? given : share_of(r.top_p, total);
         u64 most = kept.ties;
-        if (!(static_cast<double>(above.mass) < limit)) {
-            const Cut c = find_cut<true>(group, v, w, limit, Sum{0, 0});
+        if (above.mass >= limit) {
+            const Cut c = cut(std::true_type{}, limit);
             kept.cut = c.value;
             above = c.above;
             most = ~0ull;
@@ -206,23 +208,66 @@ __device__ __forceinline__ Kept both_cuts(Group& group, const Row& r, int vocab,
     return kept;
 }
 
-// ---- up to 1024 tokens: a warp per row, N tokens a lane (token i * 32 + lane) --------------
+// ---- up to 1024 tokens: a warp per row, N tokens a lane (token lane * N + i) -----------------
+//
+// A cut comes from a histogram of the row over 128 bins of (max - l) / T in shared memory (count, and weight
+// as a low and a high word), then from counting among the tokens of its bin.
 
 constexpr int kRowWarps = 4;
+constexpr int kRowBins = 128;
+constexpr float kReach = 21.6f;  // exp(-21.6) 2^30 rounds to 0: what is further from the best has no weight
+
+struct RowShared {
+    alignas(16) uint32_t count[kRowBins], low[kRowBins], high[kRowBins];
+    float few_value[32];
+    uint32_t few_w[32];
+};
+
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v) {  // exclusive
+    const int lane = threadIdx.x & 31;
+    uint32_t in = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, in, o);
+        if (lane >= o) in += up;
+    }
+    return in - v;
+}
+__device__ __forceinline__ u64 warp_scan64(u64 v) {  // exclusive
+    const int lane = threadIdx.x & 31;
+    u64 in = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 up = __shfl_up_sync(0xffffffffu, in, o);
+        if (lane >= o) in += up;
+    }
+    return in - v;
+}
 
 template <typename L, int N>
 __global__ void __launch_bounds__(32 * kRowWarps) warp_kernel(const rl2_sample_args a) {
+    __shared__ RowShared all_shared[kRowWarps];
+    RowShared& sh = all_shared[threadIdx.x >> 5];
     const int lane = threadIdx.x & 31;
     const int V = a.vocab;
     WarpGroup group;
     for (long long row = static_cast<long long>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); row < a.rows;
          row += static_cast<long long>(gridDim.x) * kRowWarps) {
-        const L* s = static_cast<const L*>(a.logits) + row * a.ld_logits;
+        const L* s = static_cast<const L*>(a.logits) + row * a.ld_logits + lane * N;
+        const int here = V - lane * N;  // tokens of this lane (more than N: N)
         float v[N];
+        constexpr int kVec = N * sizeof(L) >= 16 ? 16 / sizeof(L) : 1;
+        if (kVec > 1 && here >= N && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int j = i * 32 + lane;
-            v[i] = j < V ? clean(to_float(s[j])) : -INFINITY;
+            for (int i = 0; i < N; i += kVec) {
+                L x[kVec];
+                *reinterpret_cast<uint4*>(x) = __ldg(reinterpret_cast<const uint4*>(s + i));
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) v[i + k] = clean(to_float(x[k]));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = i < here ? clean(to_float(s[i])) : -INFINITY;
         }
         const Row r = row_of(a, row);
         float best = v[0];
@@ -246,41 +291,122 @@ __global__ void __launch_bounds__(32 * kRowWarps) warp_kernel(const rl2_sample_a
             all.mass += w[i];
         }
         all = group.sum(all);
-        const Kept kept = both_cuts(group, r, V, best, v, w, all);
-        u64 ties_left = kept.ties, total = 0;
+        const float per_value = fminf(r.inverse * (kRowBins / kReach), FLT_MAX);
+        auto bin_of = [&](float x) {
+            const float at = (best - x) * per_value;
+            return at < kRowBins - 1 ? static_cast<int>(at) : kRowBins - 1;
+        };
+        bool counted = false;
+        auto cut_of = [&](auto by_mass, u64 limit) {
+            constexpr bool kMass = decltype(by_mass)::value;
+            static_assert(kRowBins == 128, "four bins a lane");
+            if (!counted) {
+                counted = true;
+                __syncwarp();
+                reinterpret_cast<uint4*>(sh.count)[lane] = make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(sh.low)[lane] = make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(sh.high)[lane] = make_uint4(0, 0, 0, 0);
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (w[i]) {
+                        const int bin = bin_of(v[i]);
+                        atomicAdd(&sh.count[bin], 1u);
+                        atomicAdd(&sh.low[bin], w[i] & 0xFFFFu);  // 1024 tokens at most: neither word overflows
+                        atomicAdd(&sh.high[bin], w[i] >> 16);
+                    }
+                __syncwarp();
+            }
+            Sum mine[4], sum{0, 0};
+            const uint4 c = reinterpret_cast<const uint4*>(sh.count)[lane], lo = reinterpret_cast<const uint4*>(sh.low)[lane],
+                        hi = reinterpret_cast<const uint4*>(sh.high)[lane];
+            mine[0] = Sum{c.x, (static_cast<u64>(hi.x) << 16) + lo.x};
+            mine[1] = Sum{c.y, (static_cast<u64>(hi.y) << 16) + lo.y};
+            mine[2] = Sum{c.z, (static_cast<u64>(hi.z) << 16) + lo.z};
+            mine[3] = Sum{c.w, (static_cast<u64>(hi.w) << 16) + lo.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sum.count += mine[e].count;
+                sum.mass += mine[e].mass;
+            }
+            Sum at{warp_scan(sum.count), warp_scan64(sum.mass)};
+            // the bin at which the limit is reached: in one lane
+            int bin = -1;
+            uint32_t inside = 0;
+            Sum before{0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const Sum next{at.count + mine[e].count, at.mass + mine[e].mass};
+                if ((kMass ? at.mass : at.count) < limit && (kMass ? next.mass : next.count) >= limit) {
+                    bin = lane * 4 + e;
+                    inside = mine[e].count;
+                    before = at;
+                }
+                at = next;
+            }
+            const int from = __ffs(__ballot_sync(0xffffffffu, bin >= 0)) - 1;
+            bin = __shfl_sync(0xffffffffu, bin, from);
+            inside = __shfl_sync(0xffffffffu, inside, from);
+            before.count = __shfl_sync(0xffffffffu, before.count, from);
+            before.mass = __shfl_sync(0xffffffffu, before.mass, from);
+            if (inside > 32) {
+                uint32_t y[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) y[i] = bin_of(v[i]) == bin ? w[i] : 0u;
+                return find_cut<kMass>(group, v, y, limit, before);
+            }
+            // what is above each of the bin's tokens; the cut is the lowest that has less than the limit there
+            uint32_t own = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) own |= (w[i] && bin_of(v[i]) == bin ? 1u : 0u) << i;
+            uint32_t to = warp_scan(__popc(own));
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (own >> i & 1u) {
+                    sh.few_value[to] = v[i];
+                    sh.few_w[to++] = w[i];
+                }
+            __syncwarp();
+            const float x = lane < inside ? sh.few_value[lane] : INFINITY;
+            Sum above = before;
+            for (uint32_t k = 0; k < inside; ++k)
+                if (sh.few_value[k] > x) {
+                    above.count += 1;
+                    above.mass += sh.few_w[k];
+                }
+            const bool less = lane < inside && (kMass ? above.mass : static_cast<u64>(above.count)) < limit;
+            const uint32_t lowest = ~__reduce_max_sync(0xffffffffu, less ? ~key_of(x) : 0u);
+            const int owner = __ffs(__ballot_sync(0xffffffffu, less && key_of(x) == lowest)) - 1;
+            __syncwarp();
+            return Cut{value_of(lowest), Sum{__shfl_sync(0xffffffffu, above.count, owner), __shfl_sync(0xffffffffu, above.mass, owner)}};
+        };
+        const Kept kept = both_cuts(r, V, best, all, 0, cut_of);
+        // the first ties by index, then the kept weights in order
+        uint32_t ties = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) ties += v[i] == kept.cut && w[i] != 0;
+        uint32_t rank = kept.cut != -INFINITY ? warp_scan(ties) : 0u;
+        u64 sum = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const bool tie = v[i] == kept.cut && w[i] != 0;
-            const uint32_t tied = __ballot_sync(0xffffffffu, tie);
-            const bool in = v[i] > kept.cut || (tie && __popc(tied & ((1u << lane) - 1)) < ties_left);
-            ties_left -= min(ties_left, static_cast<u64>(__popc(tied)));
-            if (!in || (!r.greedy && exp_of(v[i], best, r.inverse) < r.min_p)) w[i] = 0;
-            total += w[i];
+            const bool in = v[i] > kept.cut || (tie && rank < kept.ties);
+            rank += tie;
+            if (!in || (!r.greedy && r.min_p > 0.0f && exp_of(v[i], best, r.inverse) < r.min_p)) w[i] = 0;
+            sum += w[i];
         }
-        total = warp_sum64(total);
+        const u64 total = warp_sum64(sum);
         const u64 target = target_of(r.uniform, total);
-        u64 cum = 0;
-        for (int i = 0; i < N; ++i) {
-            uint32_t mine = 0;
+        u64 cum = warp_scan64(sum);
+        if (cum <= target && target < cum + sum) {
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (k == i) mine = w[k];
-            const u64 step = warp_sum64(mine);
-            if (cum + step > target) {  // the token is one of these 32
-                u64 sum = mine;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 up = __shfl_up_sync(0xffffffffu, sum, o);
-                    if (lane >= o) sum += up;
+            for (int i = 0; i < N; ++i) {
+                if (cum <= target && target < cum + w[i]) {
+                    a.tokens[row] = lane * N + i;
+                    if (a.log_probs) a.log_probs[row] = log_share(w[i], total);
                 }
-                const uint32_t hit = __ballot_sync(0xffffffffu, cum + sum > target);
-                if (lane == __ffs(hit) - 1) {
-                    a.tokens[row] = i * 32 + lane;
-                    if (a.log_probs) a.log_probs[row] = log_share(mine, total);
-                }
-                break;
+                cum += w[i];
             }
-            cum += step;
         }
     }
 }
@@ -301,10 +427,10 @@ constexpr int kT = 512;
 constexpr int kWarps = kT / 32;
 constexpr int kBins = 2048;
 constexpr int kEach = kBins / kT;
-constexpr float kReach = 21.6f;  // exp(-21.6) 2^30 rounds to 0
 constexpr int kPer = 8;          // list entries per thread
 constexpr int kList = kT * kPer;
-constexpr int kFew = 32 * kPer;  // tokens that one warp takes
+constexpr int kFewPer = 8;
+constexpr int kFew = 32 * kFewPer;  // tokens that one warp takes
 constexpr int kStretches = 1024;
 constexpr int kMaxStretch = 2048;  // tokens: 2^20 of them in fewer than 1024 stretches
 
@@ -485,15 +611,36 @@ __device__ __forceinline__ Sum block_scan(Shared* sh, Sum s, Sum& all) {
     return before;
 }
 
+__device__ __forceinline__ uint32_t block_scan(Shared* sh, uint32_t s) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t in = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, in, o);
+        if (lane >= o) in += up;
+    }
+    if (lane == 31) sh->scan_count[warp] = in;
+    __syncthreads();
+    return in - s + __reduce_add_sync(0xffffffffu, lane < warp ? sh->scan_count[lane] : 0u);
+}
+
 __device__ __forceinline__ void clear_histogram(Shared* sh) {
     for (int i = threadIdx.x; i < kBins / 2; i += kT) reinterpret_cast<uint4*>(sh->mass)[i] = make_uint4(0, 0, 0, 0);
     for (int i = threadIdx.x; i < kBins / 4; i += kT) reinterpret_cast<uint4*>(sh->count)[i] = make_uint4(0, 0, 0, 0);
 }
 
+// Adds a weight to a bin: its low word, and the carry where there is one. (A 64-bit add in shared memory is a
+// loop of compare and swap.)
+__device__ __forceinline__ void add_mass(Shared* sh, int bin, uint32_t w) {
+    uint32_t* word = reinterpret_cast<uint32_t*>(&sh->mass[bin]);
+    const uint32_t old = atomicAdd(word, w);
+    if (old + w < old) atomicAdd(word + 1, 1u);
+}
+
 // Of a complete histogram: into sh->found the first bin up to which (itself included) the count, or the
 // weight, reaches the limit (kBins where none does). All threads; a barrier before it is read.
-__device__ __forceinline__ void find_bin(Shared* sh, bool by_mass, double limit, const Sum (&mine)[kEach], Sum at) {
-    auto value = [&](Sum x) { return by_mass ? static_cast<double>(x.mass) : static_cast<double>(x.count); };
+__device__ __forceinline__ void find_bin(Shared* sh, bool by_mass, u64 limit, const Sum (&mine)[kEach], Sum at) {
+    auto value = [&](Sum x) { return by_mass ? x.mass : static_cast<u64>(x.count); };
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
         const Sum next{at.count + mine[e].count, at.mass + mine[e].mass};
@@ -520,114 +667,125 @@ __device__ __forceinline__ Sum scan_histogram(Shared* sh, Sum (&mine)[kEach], Su
 
 // ---- a row from its list ------------------------------------------------------------
 
-// The last of the first `ties` indexes among the tokens marked, which are more than that.
-template <int N, typename Group>
-__device__ __forceinline__ int last_of(Group& group, const int (&token)[N], const bool (&marked)[N], u64 ties, int vocab) {
-    int lo = -1, hi = vocab - 1;  // more than `ties` through hi, not through lo
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        uint32_t c = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) c += marked[i] && token[i] <= mid;
-        (group.count(c) > ties ? hi : lo) = mid;
-    }
-    return lo;
-}
-
-// The first index through which the tokens' weight and what is before them exceeds the target.
-template <int N, typename Group>
-__device__ __forceinline__ int first_over(Group& group, const int (&token)[N], const uint32_t (&w)[N], u64 before, u64 target,
-                                          int vocab) {
-    int lo = -1, hi = vocab - 1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        u64 m = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) m += token[i] <= mid ? w[i] : 0u;
-        (before + group.mass(m) > target ? hi : lo) = mid;
-    }
-    return hi;
-}
-
-// Up to kFew candidates: one warp, no barriers.
-__device__ __noinline__ void draw_few(Shared* sh, int n, const Row r, int vocab, float best, const rl2_sample_args& a, long long row) {
-    const int lane = threadIdx.x & 31;
+// One warp on a few tokens of the list: value, weight and index of entry i * 32 + lane in each lane.
+template <int N>
+struct Few {
+    float v[N];
+    uint32_t w[N];
+    int token[N];
     WarpGroup group;
-    float v[kPer];
-    uint32_t w[kPer];
-    int token[kPer];
+
+    __device__ __forceinline__ Cut cut(bool by_mass, u64 limit, Sum before) {
+        return by_mass ? find_cut<true>(group, v, w, limit, before) : find_cut<false>(group, v, w, limit, before);
+    }
+    // the last of the first `ties` indexes (in lo .. hi] among the tokens marked, which are more than that
+    __device__ __forceinline__ int last_of(const bool (&marked)[N], u64 ties, int lo, int hi) {
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            uint32_t c = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) c += marked[i] && token[i] <= mid;
+            (group.count(c) > ties ? hi : lo) = mid;
+        }
+        return lo;
+    }
+    // the first index (in lo .. hi] through which the tokens' weight and what is before them exceeds the target
+    __device__ __forceinline__ int first_over(u64 before, u64 target, int lo, int hi) {
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            u64 m = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) m += token[i] <= mid ? w[i] : 0u;
+            (before + group.mass(m) > target ? hi : lo) = mid;
+        }
+        return hi;
+    }
+    __device__ __forceinline__ void write(const rl2_sample_args& a, long long row, int chosen, u64 total) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (token[i] == chosen && w[i]) {
+                a.tokens[row] = chosen;
+                if (a.log_probs) a.log_probs[row] = log_share(w[i], total);
+            }
+    }
+};
+
+// A list of up to 32 N candidates: one warp, no barriers.
+template <int N>
+__device__ __noinline__ void draw_few(Shared* sh, int n, const Row r, int vocab, float best, u64 given, const rl2_sample_args& a,
+                                      long long row) {
+    const int lane = threadIdx.x & 31;
+    Few<N> few;
     Sum all{0, 0};
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < N; ++i) {
         const int at = i * 32 + lane;
-        v[i] = at < n ? sh->value[at] : -INFINITY;
-        token[i] = at < n ? sh->index[at] : vocab;
-        w[i] = at < n ? static_cast<uint32_t>(weight_of(exp_of(v[i], best, r.inverse))) : 0u;
-        all.count += w[i] != 0;
-        all.mass += w[i];
+        few.v[i] = at < n ? sh->value[at] : -INFINITY;
+        few.token[i] = at < n ? sh->index[at] : vocab;
+        few.w[i] = at < n ? static_cast<uint32_t>(weight_of(exp_of(few.v[i], best, r.inverse))) : 0u;
+        all.count += few.w[i] != 0;
+        all.mass += few.w[i];
     }
-    all = group.sum(all);
-    const Kept kept = both_cuts(group, r, vocab, best, v, w, all);
-    bool tie[kPer];
+    all = few.group.sum(all);
+    const Kept kept = both_cuts(r, vocab, best, all, given,
+                                [&](auto by_mass, u64 limit) { return few.cut(decltype(by_mass)::value, limit, Sum{0, 0}); });
+    bool tie[N];
     uint32_t ties = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) ties += tie[i] = v[i] == kept.cut && w[i] != 0;
-    const int last = group.count(ties) > kept.ties ? last_of(group, token, tie, kept.ties, vocab) : vocab;
+    for (int i = 0; i < N; ++i) ties += tie[i] = few.v[i] == kept.cut && few.w[i] != 0;
+    const int last = few.group.count(ties) > kept.ties ? few.last_of(tie, kept.ties, -1, vocab - 1) : vocab;
     u64 total = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const bool in = v[i] > kept.cut || (tie[i] && token[i] <= last);
-        if (!in || (!r.greedy && exp_of(v[i], best, r.inverse) < r.min_p)) w[i] = 0;
-        total += w[i];
+    for (int i = 0; i < N; ++i) {
+        const bool in = few.v[i] > kept.cut || (tie[i] && few.token[i] <= last);
+        if (!in || (!r.greedy && exp_of(few.v[i], best, r.inverse) < r.min_p)) few.w[i] = 0;
+        total += few.w[i];
     }
-    total = group.mass(total);
-    const int chosen = first_over(group, token, w, 0, target_of(r.uniform, total), vocab);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-        if (token[i] == chosen && w[i]) {
-            a.tokens[row] = chosen;
-            if (a.log_probs) a.log_probs[row] = log_share(w[i], total);
-        }
+    total = few.group.mass(total);
+    few.write(a, row, few.first_over(0, target_of(r.uniform, total), -1, vocab - 1), total);
 }
 
 // A longer list: histograms of it (by value for the cuts, by index for the draw), one warp on the bin found.
-// `fine` bins a unit of value below the best spread the list over all bins.
-__device__ __noinline__ void draw_many(Shared* sh, int n, const Row r, int vocab, float best, float fine, const rl2_sample_args& a,
-                                       long long row) {
+// `fine` bins a unit of value below the best spread the list over all bins. A bin with more tokens than one
+// warp takes is halved by the block.
+__device__ __noinline__ void draw_many(Shared* sh, int n, const Row r, int vocab, float best, float fine, u64 given,
+                                       const rl2_sample_args& a, long long row) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Block group{sh, 0};
     float v[kPer];
     uint32_t w[kPer];
-    int token[kPer];
     auto bin_of = [&](float x) {
         const float at = (best - x) * fine;
         return at < kBins - 1 ? static_cast<int>(at) : kBins - 1;
     };
+    auto token_of = [&](int i) { return i * kT + tid < n ? sh->index[i * kT + tid] : vocab; };
     clear_histogram(sh);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int at = i * kT + tid;
-        v[i] = at < n ? sh->value[at] : -INFINITY;
-        token[i] = at < n ? sh->index[at] : vocab;
-        w[i] = at < n ? static_cast<uint32_t>(weight_of(exp_of(v[i], best, r.inverse))) : 0u;
-        if (w[i]) {
-            atomicAdd(&sh->count[bin_of(v[i])], 1u);
-            atomicAdd(&sh->mass[bin_of(v[i])], static_cast<u64>(w[i]));
+        v[i] = -INFINITY;
+        w[i] = 0;
+        if (i * kT + tid < n) {
+            v[i] = sh->value[i * kT + tid];
+            w[i] = static_cast<uint32_t>(weight_of(exp_of(v[i], best, r.inverse)));
+            if (w[i]) {
+                atomicAdd(&sh->count[bin_of(v[i])], 1u);
+                add_mass(sh, bin_of(v[i]), w[i]);
+            }
         }
     }
     __syncthreads();
     Sum mine[kEach], whole;
     const Sum at = scan_histogram(sh, mine, whole);
     // the cut whose limit the histogram reaches
-    auto cut_of = [&](auto by_mass, double limit) {
+    auto cut_of = [&](auto by_mass, u64 limit) {
         constexpr bool kMass = decltype(by_mass)::value;
         if (tid == 0) sh->few = 0;
         find_bin(sh, kMass, limit, mine, at);
         __syncthreads();
         const int bin = sh->found.bin;
         const Sum before = sh->found.before;
-        if (sh->found.here.count <= kFew) {
+        if (sh->found.here.count <= 32) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
                 if (w[i] && bin_of(v[i]) == bin) {
@@ -637,16 +795,18 @@ __device__ __noinline__ void draw_many(Shared* sh, int n, const Row r, int vocab
                 }
             __syncthreads();
             if (warp == 0) {
-                float x[kPer];
-                uint32_t y[kPer];
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    x[i] = i * 32 + lane < sh->few ? sh->few_value[i * 32 + lane] : -INFINITY;
-                    y[i] = i * 32 + lane < sh->few ? sh->few_w[i * 32 + lane] : 0u;
-                }
-                WarpGroup own;
-                const Cut c = find_cut<kMass>(own, x, y, limit, before);
-                if (lane == 0) sh->cut = c;
+                // what is above each of the few; the cut is the lowest that has less than the limit there
+                const int few = sh->few;
+                const float x = lane < few ? sh->few_value[lane] : INFINITY;
+                Sum above = before;
+                for (int k = 0; k < few; ++k)
+                    if (sh->few_value[k] > x) {
+                        above.count += 1;
+                        above.mass += sh->few_w[k];
+                    }
+                const bool less = lane < few && (kMass ? above.mass : static_cast<u64>(above.count)) < limit;
+                const uint32_t lowest = ~__reduce_max_sync(0xffffffffu, less ? ~key_of(x) : 0u);
+                if (less && key_of(x) == lowest) sh->cut = Cut{x, above};  // equal values write the same
             }
             __syncthreads();
             const Cut c = sh->cut;
@@ -658,63 +818,42 @@ __device__ __noinline__ void draw_many(Shared* sh, int n, const Row r, int vocab
         for (int i = 0; i < kPer; ++i) y[i] = bin_of(v[i]) == bin ? w[i] : 0u;
         return find_cut<kMass>(group, v, y, limit, before);
     };
-    Kept kept{-INFINITY, 0};
-    if (r.greedy || r.top_p <= 0.0f) {
-        kept = Kept{best, 1};
-    } else {
-        Sum above = whole;
-        u64 total = whole.mass;
-        if (r.top_k > 0 && r.top_k < vocab && whole.count > static_cast<uint32_t>(r.top_k)) {
-            const Cut c = cut_of(std::false_type{}, r.top_k);
-            kept = Kept{c.value, static_cast<u64>(r.top_k) - c.above.count};
-            above = c.above;
-            total = above.mass + kept.ties * weight_of(exp_of(kept.cut, best, r.inverse));
-        }
-        if (r.top_p < 1.0f) {
-            const double limit = static_cast<double>(r.top_p) * static_cast<double>(total);
-            u64 most = kept.ties;
-            if (!(static_cast<double>(above.mass) < limit)) {
-                const Cut c = cut_of(std::true_type{}, limit);
-                kept.cut = c.value;
-                above = c.above;
-                most = ~0ull;
-            }
-            if (kept.cut != -INFINITY)
-                kept.ties = kept_of_last(above.mass, weight_of(exp_of(kept.cut, best, r.inverse)), limit, most);
-        }
-    }
+    const Kept kept = both_cuts(r, vocab, best, whole, given, cut_of);
     // ---- what is kept, by index ----
-    bool tie[kPer];
     uint32_t ties = 0;
     __syncthreads();  // sh->few and the histogram are read
     if (tid == 0) sh->few = 0;
     clear_histogram(sh);
+    auto tie = [&](int i) { return v[i] == kept.cut && w[i] != 0; };
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) ties += tie[i] = v[i] == kept.cut && w[i] != 0;
+    for (int i = 0; i < kPer; ++i) ties += tie(i);
     ties = group.count(ties);
     int last = vocab;
     if (ties > kept.ties) {
-        if (ties <= kFew) {
+        if (ties <= 32) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
-                if (tie[i]) sh->few_index[atomicAdd(&sh->few, 1)] = token[i];
+                if (tie(i)) sh->few_index[atomicAdd(&sh->few, 1)] = token_of(i);
             __syncthreads();
             if (warp == 0) {
-                int x[kPer];
-                bool y[kPer];
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    y[i] = i * 32 + lane < sh->few;
-                    x[i] = y[i] ? sh->few_index[i * 32 + lane] : vocab;
-                }
-                WarpGroup own;
-                const int l = last_of(own, x, y, kept.ties, vocab);
-                if (lane == 0) sh->answer = l;
+                // rank among the few by index; the one of rank ties - 1 is the last kept
+                const int mine_index = lane < sh->few ? sh->few_index[lane] : vocab;
+                int rank = 0;
+                for (int k = 0; k < sh->few; ++k) rank += sh->few_index[k] < mine_index;
+                if (lane < sh->few && rank + 1 == static_cast<int>(kept.ties)) sh->answer = mine_index;
             }
             __syncthreads();
             last = sh->answer;
         } else {
-            last = last_of(group, token, tie, kept.ties, vocab);
+            int lo = -1, hi = vocab - 1;  // more than kept.ties through hi, not through lo
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                uint32_t c = 0;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) c += tie(i) && token_of(i) <= mid;
+                (group.count(c) > kept.ties ? hi : lo) = mid;
+            }
+            last = lo;
         }
     }
     int shift = 0;
@@ -723,50 +862,61 @@ __device__ __noinline__ void draw_many(Shared* sh, int n, const Row r, int vocab
     if (tid == 0) sh->few = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const bool in = v[i] > kept.cut || (tie[i] && token[i] <= last);
-        if (!in || (!r.greedy && exp_of(v[i], best, r.inverse) < r.min_p)) w[i] = 0;
-        if (w[i]) {
-            atomicAdd(&sh->count[token[i] >> shift], 1u);
-            atomicAdd(&sh->mass[token[i] >> shift], static_cast<u64>(w[i]));
+        if (!w[i]) continue;
+        const int token = token_of(i);
+        const bool in = v[i] > kept.cut || (v[i] == kept.cut && token <= last);
+        if (!in || (!r.greedy && r.min_p > 0.0f && exp_of(v[i], best, r.inverse) < r.min_p)) {
+            w[i] = 0;
+        } else {
+            atomicAdd(&sh->count[token >> shift], 1u);
+            add_mass(sh, token >> shift, w[i]);
         }
     }
     __syncthreads();
     Sum kept_all;
     const Sum kept_at = scan_histogram(sh, mine, kept_all);
     const u64 target = target_of(r.uniform, kept_all.mass);
-    find_bin(sh, true, static_cast<double>(target + 1), mine, kept_at);
+    find_bin(sh, true, target + 1, mine, kept_at);
     __syncthreads();
     const int bin = sh->found.bin;
     const u64 before = sh->found.before.mass;
-    int chosen;
-    if (sh->found.here.count <= kFew) {
+    const int lo = (bin << shift) - 1, hi = min(vocab, (bin + 1) << shift) - 1;
+    if (sh->found.here.count <= 32) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-            if (w[i] && token[i] >> shift == bin) {
+            if (w[i] && token_of(i) >> shift == bin) {
                 const int to = atomicAdd(&sh->few, 1);
-                sh->few_index[to] = token[i];
+                sh->few_index[to] = token_of(i);
                 sh->few_w[to] = w[i];
             }
         __syncthreads();
-        if (warp != 0) return;
+        const int few = sh->few;
+        if (warp != 0 || lane >= few) return;
+        const int mine_index = sh->few_index[lane];
+        u64 cum = before;
+        for (int k = 0; k < few; ++k)
+            if (sh->few_index[k] < mine_index) cum += sh->few_w[k];
+        if (cum <= target && target < cum + sh->few_w[lane]) {
+            a.tokens[row] = mine_index;
+            if (a.log_probs) a.log_probs[row] = log_share(sh->few_w[lane], kept_all.mass);
+        }
+        return;
+    }
+    int from = lo, to = hi;
+    while (to - from > 1) {
+        const int mid = (from + to) >> 1;
+        u64 m = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const bool in = i * 32 + lane < sh->few;
-            token[i] = in ? sh->few_index[i * 32 + lane] : vocab;
-            w[i] = in ? sh->few_w[i * 32 + lane] : 0u;
+            const int token = token_of(i);
+            m += token > lo && token <= mid ? w[i] : 0u;
         }
-        WarpGroup own;
-        chosen = first_over(own, token, w, before, target, vocab);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (token[i] >> shift != bin) w[i] = 0;
-        chosen = first_over(group, token, w, before, target, vocab);
+        (before + group.mass(m) > target ? to : from) = mid;
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-        if (token[i] == chosen && w[i]) {
-            a.tokens[row] = chosen;
+        if (token_of(i) == to && w[i]) {
+            a.tokens[row] = to;
             if (a.log_probs) a.log_probs[row] = log_share(w[i], kept_all.mass);
         }
 }
@@ -853,17 +1003,47 @@ struct Work {
         const float at = (best - v) * per_value;
         return at < kBins - 1 ? static_cast<int>(at) : kBins - 1;
     }
+    // f(step, token of the first element, elements) for every vector of this lane, whole warps in step;
+    // elements outside the row are -inf
+    template <typename F>
+    __device__ __forceinline__ void every_vector(F&& f) const {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        constexpr int kAhead = 4;  // loads in flight
+        int i = 0;
+        for (; i + kAhead <= steps; i += kAhead) {
+            if (in.inside(vector_of(warp, 0, i)) && in.inside(vector_of(warp, 0, i + kAhead - 1))) {
+                uint4 raw[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) raw[k] = in.raw(vector_of(warp, lane, i + k));
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    L y[kN];
+                    *reinterpret_cast<uint4*>(y) = raw[k];
+                    float x[kN];
+#pragma unroll
+                    for (int e = 0; e < kN; ++e) x[e] = clean(to_float(y[e]));
+                    f(i + k, in.first(vector_of(warp, lane, i + k)), x);
+                }
+            } else {
+                for (int k = 0; k < kAhead; ++k) {
+                    float x[kN];
+                    in.load(vector_of(warp, lane, i + k), x);
+                    f(i + k, in.first(vector_of(warp, lane, i + k)), x);
+                }
+            }
+        }
+        for (; i < steps; ++i) {
+            float x[kN];
+            in.load(vector_of(warp, lane, i), x);
+            f(i, in.first(vector_of(warp, lane, i)), x);
+        }
+    }
     template <typename F>
     __device__ __forceinline__ void every(F&& f) const {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        for (int i = 0; i < steps; ++i) {
-            const int b = vector_of(warp, lane, i);
-            if (b >= in.vectors) break;
-            float x[kN];
-            in.load(b, x);
+        every_vector([&](int, int, const float(&x)[kN]) {
 #pragma unroll
-            for (int e = 0; e < kN; ++e) f(x[e], in.first(b) + e);
-        }
+            for (int e = 0; e < kN; ++e) f(x[e]);
+        });
     }
     // hands the first CTA's sh->found to the others; a barrier
     __device__ __forceinline__ void share_found() {
@@ -890,8 +1070,8 @@ struct Work {
             group.sync();
         }
     }
-    // The bin of the merged histogram at which the limit (or `share` of the whole weight) is reached; on every CTA.
-    __device__ __forceinline__ Found search(bool by_mass, double limit, bool share) {
+    // The bin of the merged histogram at which the limit is reached; on every CTA.
+    __device__ __forceinline__ Found search(bool by_mass, u64 limit) {
         if (group.rank == 0) {
             Sum mine[kEach], whole;
             const Sum at = scan_histogram(sh, mine, whole);
@@ -900,7 +1080,7 @@ struct Work {
                 sh->found.whole = whole;
             }
             __syncthreads();
-            find_bin(sh, by_mass, share ? limit * static_cast<double>(whole.mass) : limit, mine, at);
+            find_bin(sh, by_mass, limit, mine, at);
         }
         share_found();
         const Found f = sh->found;
@@ -1012,16 +1192,22 @@ __device__ __forceinline__ bool build_list(Work<L>& work, int bound) {
                         has |= (passes(to_float(in.s[first[k] + e])) ? 1u : 0u) << (k * kN + e);
                 }
             }
+            // indexes first, values once the list is whole: a lane has its tokens in any of the vectors
             int slot = append(&sh->listed, __popc(has));
+            for (; has; has &= has - 1, ++slot) {
+                const int bit = __ffs(has) - 1;
+                int j = first[0];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k)
-                for (uint32_t here = (has >> (k * kN)) & ((1u << kN) - 1); here; here &= here - 1, ++slot)
-                    if (slot < kList) {
-                        const int j = first[k] + __ffs(here) - 1;
-                        sh->value[slot] = in.at(j);
-                        sh->index[slot] = j;
-                    }
+                for (int k = 1; k < kAhead; ++k)
+                    if (bit / kN == k) j = first[k];
+                if (slot < kList) sh->index[slot] = j + bit % kN;
+            }
         }
+        __syncthreads();
+        const int listed = min(sh->listed, kList);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (i * kT + tid < listed) sh->value[i * kT + tid] = in.at(sh->index[i * kT + tid]);
     } else if (tid == 0) {
         sh->listed = kList + 1;
     }
@@ -1047,9 +1233,9 @@ __device__ __forceinline__ bool build_list(Work<L>& work, int bound) {
 }
 
 // The cut of all tokens: histogram, then the list of the cut's bin; a bin that does not fit is divided
-// again between its own extremes, by keys. `limit` receives the limit (a share: of the whole weight).
+// again between its own extremes, by keys.
 template <typename L>
-__device__ __noinline__ Cut wide_cut(Work<L>& work, bool by_mass, double& limit, bool share) {
+__device__ __noinline__ Cut wide_cut(Work<L>& work, bool by_mass, u64 limit, const Found* known) {
     Shared* sh = work.sh;
     const int tid = threadIdx.x;
     const float best = work.best, inverse = work.r.inverse;
@@ -1064,31 +1250,35 @@ __device__ __noinline__ Cut wide_cut(Work<L>& work, bool by_mass, double& limit,
             if (!w) return -1;
             return first ? work.bin_of(x) : static_cast<int>((key_of(high) - key_of(x)) / width);
         };
-        clear_histogram(sh);
-        work.group.sync();
-        work.every([&](float x, int) {
-            uint32_t w;
-            const int bin = bin_in(x, w);
-            if (bin < 0) return;
-            atomicAdd(&sh->count[bin], 1u);
-            atomicAdd(&sh->mass[bin], static_cast<u64>(w));
-        });
-        work.merge(kBins);
-        const Found f = work.search(by_mass, first ? limit : limit - (by_mass ? static_cast<double>(above.mass) : static_cast<double>(above.count)),
-                                    first && share);
-        if (first && share) limit *= static_cast<double>(f.whole.mass);
+        Found f;
+        if (first && known) {
+            f = *known;
+        } else {
+            clear_histogram(sh);
+            work.group.sync();
+            work.every([&](float x) {
+                uint32_t w;
+                const int bin = bin_in(x, w);
+                if (bin < 0) return;
+                atomicAdd(&sh->count[bin], 1u);
+                add_mass(sh, bin, w);
+            });
+            work.merge(kBins);
+            f = work.search(by_mass, limit - (by_mass ? above.mass : static_cast<u64>(above.count)));
+        }
         if (f.bin == kBins) return Cut{-INFINITY, f.whole};  // fewer tokens of weight than top-k asks for
         above.count += f.before.count;
         above.mass += f.before.mass;
         if (tid == 0) sh->listed = 0;
         work.group.sync();
-        if (f.here.count <= kList) {
-            work.every([&](float x, int) {
-                uint32_t w;
-                if (bin_in(x, w) != f.bin) return;
-                sh->value[atomicAdd(&sh->listed, 1)] = x;
-            });
-            __syncthreads();
+        work.every([&](float x) {
+            uint32_t w;
+            if (bin_in(x, w) != f.bin) return;
+            const int at = atomicAdd(&sh->listed, 1);
+            if (at < kList) sh->value[at] = x;
+        });
+        __syncthreads();
+        if (work.group.max_key(static_cast<uint32_t>(sh->listed)) <= kList) {
             float v[kPer];
             uint32_t w[kPer];
 #pragma unroll
@@ -1100,7 +1290,7 @@ __device__ __noinline__ Cut wide_cut(Work<L>& work, bool by_mass, double& limit,
             return by_mass ? find_cut<true>(work.group, v, w, limit, above) : find_cut<false>(work.group, v, w, limit, above);
         }
         uint32_t up = 0, down = 0;
-        work.every([&](float x, int) {
+        work.every([&](float x) {
             uint32_t w;
             if (bin_in(x, w) != f.bin) return;
             up = max(up, key_of(x));
@@ -1113,9 +1303,38 @@ __device__ __noinline__ Cut wide_cut(Work<L>& work, bool by_mass, double& limit,
     }
 }
 
+// Weight of the whole row, and the bin of its tokens up to which a share p < 1 of it stands. Tokens that all
+// together weigh less than the rest, 1 - p, cannot reach the share: they are left out of the histogram. The
+// weight's lower bound is that of the group maxima.
+template <typename L>
+__device__ __noinline__ Found share_bin(Work<L>& work, u64& limit) {
+    constexpr int kSlots = Work<L>::kSlots;
+    Shared* sh = work.sh;
+    const float best = work.best, inverse = work.r.inverse;
+    const L* maxima = reinterpret_cast<const L*>(sh->maxima);
+    clear_histogram(sh);
+    u64 mass = 0;
+#pragma unroll 4
+    for (int slot = 0; slot < kSlots; ++slot)
+        mass += weight_of(exp_of(clean(to_float(maxima[slot * kT + threadIdx.x])), best, inverse));
+    const u64 least = work.group.sum(Sum{0, mass}).mass;
+    // token weights below this sum to less than half of the rest (the other half is slack for roundings to weights)
+    const float rest = (1.0f - work.r.top_p) * 0.5f * static_cast<float>(least) / static_cast<float>(work.in.vocab);
+    const uint32_t floor_w = rest > 2.0f ? static_cast<uint32_t>(fminf(rest, kUnit)) : 1u;
+    mass = 0;
+    work.every([&](float x) {
+        const uint32_t w = static_cast<uint32_t>(weight_of(exp_of(x, best, inverse)));
+        mass += w;
+        if (w >= floor_w) add_mass(sh, work.bin_of(x), w);
+    });
+    limit = share_of(work.r.top_p, work.group.sum(Sum{0, mass}).mass);
+    work.merge(kBins);
+    return work.search(true, limit);
+}
+
 // Cuts and draw from the whole row.
 template <typename L>
-__device__ __noinline__ void draw_wide(Work<L>& work, const rl2_sample_args& a, long long row) {
+__device__ __noinline__ void draw_wide(Work<L>& work, u64 given, const Found* known, const rl2_sample_args& a, long long row) {
     constexpr int kN = Work<L>::kN;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Shared* sh = work.sh;
@@ -1127,26 +1346,22 @@ __device__ __noinline__ void draw_wide(Work<L>& work, const rl2_sample_args& a, 
     if (work.first_only) {
         kept = Kept{best, 1};
     } else {
-        Sum above{0, 0};
+        Sum above{~0u, ~0ull};
         u64 total = 0;
-        double limit = 0.0;
-        bool have_k = false;
         if (work.cut_k) {
-            limit = r.top_k;
-            const Cut c = wide_cut(work, false, limit, false);
+            const Cut c = wide_cut(work, false, static_cast<u64>(r.top_k), nullptr);
             above = c.above;
             total = c.above.mass;
             if (c.value != -INFINITY) {
-                have_k = true;
                 kept = Kept{c.value, static_cast<u64>(r.top_k) - c.above.count};
                 total += kept.ties * weight_of(exp_of(kept.cut, best, r.inverse));
             }
         }
         if (r.top_p < 1.0f) {
             u64 most = kept.ties;
-            limit = static_cast<double>(r.top_p) * (work.cut_k ? static_cast<double>(total) : 1.0);
-            if (!have_k || !(static_cast<double>(above.mass) < limit)) {
-                const Cut c = wide_cut(work, true, limit, !work.cut_k);
+            const u64 limit = given ? given : share_of(r.top_p, total);
+            if (above.mass >= limit) {
+                const Cut c = wide_cut(work, true, limit, known);
                 kept.cut = c.value;
                 above = c.above;
                 most = ~0ull;
@@ -1165,26 +1380,35 @@ __device__ __noinline__ void draw_wide(Work<L>& work, const rl2_sample_args& a, 
     work.group.sync();
     clear_histogram(sh);
     work.group.sync();
-    for (int st = work.from + warp; st < work.to; st += kWarps) {
-        u64 mass = 0;
-        uint32_t ties = 0;
-        for (int i = 0; i < per; ++i) {
-            const int b = (st * per + i) * 32 + lane;
-            if (b >= in.vectors) break;
-            float x[kN];
-            in.load(b, x);
+    u64 mass = 0;
+    uint32_t ties = 0;
+    auto end_of_step = [&](int step) {
+        if (((step + 1) & (per - 1)) != 0) return;  // not the stretch's last
+        mass = warp_sum64(mass);
+        ties = __reduce_add_sync(0xffffffffu, ties);
+        if (lane == 0) {
+            const int st = work.from + warp + kWarps * (step >> work.log_per);
+            sh->mass[st] = mass;
+            sh->count[st] = ties;
+        }
+        mass = 0;
+        ties = 0;
+    };
+    if (kept.cut == -INFINITY && !(r.min_p > 0.0f)) {  // all that weighs
+        work.every_vector([&](int step, int, const float(&x)[kN]) {
+#pragma unroll
+            for (int e = 0; e < kN; ++e) mass += weight_of(exp_of(x[e], best, r.inverse));
+            end_of_step(step);
+        });
+    } else {
+        work.every_vector([&](int step, int, const float(&x)[kN]) {
 #pragma unroll
             for (int e = 0; e < kN; ++e) {
                 if (x[e] > kept.cut) mass += weigh(x[e]);
                 ties += x[e] == kept.cut;
             }
-        }
-        mass = warp_sum64(mass);
-        ties = __reduce_add_sync(0xffffffffu, ties);
-        if (lane == 0) {
-            sh->mass[st] = mass;
-            sh->count[st] = ties;
-        }
+            end_of_step(step);
+        });
     }
     work.merge(kStretches);
     if (work.group.rank == 0) {
@@ -1297,30 +1521,57 @@ __global__ void __launch_bounds__(kT, 2) row_kernel(const rl2_sample_args a, con
         } else {
             if (work.cut_k) {
                 clear_histogram(sh);
-                work.group.sync();
+                __syncthreads();
                 const L* maxima = reinterpret_cast<const L*>(sh->maxima);
 #pragma unroll
                 for (int slot = 0; slot < kSlots; ++slot) {
                     const int bin = work.bin_of(clean(to_float(maxima[slot * kT + tid])));
                     if (bin < kBins - 1) atomicAdd(&sh->count[bin], 1u);
                 }
-                work.merge(kBins);
-                bound = min(bound, work.search(false, r.top_k, false).bin);
+                static_assert(kEach == 4, "four bins a thread");
+                if (size == 1 || r.top_k <= kList / 2 / size) {
+                    // each CTA's own bound is one of the whole row (and the list still short)
+                    if (tid == 0) sh->found.bin = kBins;
+                    __syncthreads();
+                    const uint4 mine = *reinterpret_cast<const uint4*>(&sh->count[tid * kEach]);
+                    const uint32_t in_order[kEach] = {mine.x, mine.y, mine.z, mine.w};
+                    uint32_t at = block_scan(sh, mine.x + mine.y + mine.z + mine.w);
+                    const uint32_t k = static_cast<uint32_t>(r.top_k);
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) {
+                        if (at < k && at + in_order[e] >= k) sh->found.bin = tid * kEach + e;
+                        at += in_order[e];
+                    }
+                    __syncthreads();
+                    bound = min(bound, sh->found.bin);
+                    if (size > 1) bound = static_cast<int>(~work.group.max_key(~static_cast<uint32_t>(bound)));
+                } else {
+                    work.merge(kBins);
+                    bound = min(bound, work.search(false, static_cast<u64>(r.top_k)).bin);
+                }
             }
             if (r.top_p >= 1.0f && r.min_p > 0.0f)  // one bin of slack for the rounding of the logarithm
                 bound = min(bound, static_cast<int>(min(-logf(r.min_p) * (kBins / kReach) + 1.0f, kBins - 1.0f)));
         }
+        u64 given = 0;
+        Found share;
+        if (!work.cut_k && !work.first_only && r.top_p < 1.0f) {
+            share = share_bin(work, given);
+            bound = min(bound, share.bin);
+        }
         if (bound < kBins - 1 && build_list(work, bound)) {
             if (rank == 0) {
                 const int n = sh->listed;
-                if (n <= kFew) {
-                    if (warp == 0) draw_few(sh, n, r, V, work.best, a, row);
+                if (n <= 64) {
+                    if (warp == 0) draw_few<2>(sh, n, r, V, work.best, given, a, row);
+                } else if (n <= kFew) {
+                    if (warp == 0) draw_few<kFewPer>(sh, n, r, V, work.best, given, a, row);
                 } else {
-                    draw_many(sh, n, r, V, work.best, fminf(work.per_value * (static_cast<float>(kBins) / (bound + 1)), FLT_MAX), a, row);
+                    draw_many(sh, n, r, V, work.best, fminf(work.per_value * (static_cast<float>(kBins) / (bound + 1)), FLT_MAX), given, a, row);
                 }
             }
         } else {
-            draw_wide(work, a, row);
+            draw_wide(work, given, given ? &share : nullptr, a, row);
         }
         work.group.sync();
     }
@@ -1369,8 +1620,14 @@ int launch(const rl2_sample_args& a, cudaStream_t stream) {
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(row_kernel<L>),
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+    static std::atomic<unsigned long long> allowed{0};  // devices (up to 64) whose limit is raised
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && (device > 63 || !(allowed.load() >> device & 1))) {
+        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(row_kernel<L>), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 sizeof(Shared));
+        if (e == cudaSuccess && device <= 63) allowed.fetch_or(1ull << device);
+    }
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, row_kernel<L>, a, size, shift);
     if (e != cudaSuccess) {
         set_error("token sampling: %s", cudaGetErrorString(e));

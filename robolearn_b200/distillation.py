@@ -61,4 +61,4 @@ class TopKDistillation:
             a.dlogits, a.ld_dlogits, a.dlogits_dtype = self._matrix("dlogits", dlogits, n, self.vocab, DTYPES)
         if grad_scale is not None:
             a.grad_scale = self._vector("grad_scale", grad_scale, 1)
-        N.check(self._lib.rl2_distill_topk(ctypes.byref(a), N.stream_ptr(stream)), "distillation objective")
+        N.check(self._lib.rl2_distill_topk(ctypes.byref(a), N.raw_stream(stream, self.device.index)), "distillation objective")

@@ -79,7 +79,7 @@ class GatedMLP:
         _matrix("out", out, rows, F, dt, dev)
         a = N.GatedForwardArgs(rows, x.data_ptr(), _ld(x), gate_weight.data_ptr(), _ld(gate_weight),
                                up_weight.data_ptr(), _ld(up_weight), out.data_ptr(), _ld(out), N.ptr(health))
-        N.check(self._lib.rl2_gated_forward(self.handle, ctypes.byref(a), N.stream_ptr(stream)), "gated MLP forward")
+        N.check(self._lib.rl2_gated_forward(self.handle, ctypes.byref(a), N.raw_stream(stream, self.device.index)), "gated MLP forward")
 
     def backward(self, *, x, gate_weight, up_weight, grad_out, grad_x=None, grad_gate=None, grad_up=None, health=None,
                  stream=None) -> None:
@@ -108,7 +108,7 @@ class GatedMLP:
             a.grad_gate, a.ld_grad_gate = grad_gate.data_ptr(), _ld(grad_gate)
             a.grad_up, a.ld_grad_up = grad_up.data_ptr(), _ld(grad_up)
             a.grad_weight_fp32 = int(wt == torch.float32)
-        N.check(self._lib.rl2_gated_backward(self.handle, ctypes.byref(a), N.stream_ptr(stream)), "gated MLP backward")
+        N.check(self._lib.rl2_gated_backward(self.handle, ctypes.byref(a), N.raw_stream(stream, self.device.index)), "gated MLP backward")
 
     def close(self) -> None:
         if self.handle:

@@ -53,4 +53,4 @@ class TokenSampler:
                 setattr(a, name + "s", self._vector(name, value, n, dtype))
             else:
                 setattr(a, name, value)
-        N.check(self._lib.rl2_sample_tokens(ctypes.byref(a), N.stream_ptr(stream)), "token sampling")
+        N.check(self._lib.rl2_sample_tokens(ctypes.byref(a), N.raw_stream(stream, self.device.index)), "token sampling")
