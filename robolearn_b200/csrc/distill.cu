@@ -356,13 +356,20 @@ struct Entries {
     }
 };
 
+// A row's softmax after the first pass: p = 2^(s c - o) / sum where tame, else 2^((s - base) c) / sum.
+struct Softmax {
+    float o, base, sum;
+    bool tame;
+};
+
 struct Stream {
     uint64_t full[kMaxSlots], empty[kMaxSlots];
-    uint64_t teacher_full[2], teacher_empty[2];
+    uint64_t teacher_full[2], passed[2], written[2];
     uint64_t met[2];
     float2 meet[2][kMaxCluster];
-    float red[2][kConsumers / 32], red2[2][kConsumers / 32], loss[kConsumers / 32];
+    float red[2][kConsumers / 32], red2[2][kConsumers / 32];
     float some[2];  // sum of the teacher's weights: 0 without an entry
+    Softmax softmax[2];
     int abort;
 };
 
@@ -409,8 +416,9 @@ struct Slice {
         head = min(a.vocab, mis ? kN - mis : 0);
         vectors = (a.vocab - head) / kN;
         tail = head + vectors * kN;
-        from = static_cast<int>(static_cast<long long>(vectors) * rank / size);
-        count = static_cast<int>(static_cast<long long>(vectors) * (rank + 1) / size) - from;
+        const int shift = 31 - __clz(size);  // a power of two
+        from = static_cast<int>(static_cast<unsigned long long>(vectors) * rank >> shift);
+        count = static_cast<int>(static_cast<unsigned long long>(vectors) * (rank + 1) >> shift) - from;
         chunks = (count * 16 + kChunk - 1) / kChunk;
     }
 };
@@ -561,7 +569,8 @@ __global__ void __launch_bounds__(kConsumers + 64, 2) stream_kernel(const rl2_di
         }
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&sh.teacher_full[i], 1);
-            ptx::mbar_init(&sh.teacher_empty[i], kConsumers / 32);
+            ptx::mbar_init(&sh.passed[i], 1);
+            ptx::mbar_init(&sh.written[i], kConsumers / 32);
             ptx::mbar_init(&sh.met[i], size);
         }
         sh.abort = 0;
@@ -571,18 +580,63 @@ __global__ void __launch_bounds__(kConsumers + 64, 2) stream_kernel(const rl2_di
     if (size > 1) ptx::cluster_sync();
     const long long first_row = blockIdx.x / size, step = gridDim.x / size;
 
-    if (tid >= kConsumers + 32) {  // ---- teacher warp: a row ahead ----
+    const float grad_factor = a.loss_weight * a.temperature * (a.grad_scale ? *a.grad_scale : 1.0f);
+    if (tid >= kConsumers + 32) {
+        // ---- teacher warp: the next row's teacher, then the row's loss and its teacher's tokens ----
+        const int lane = tid & 31;
+        auto next_row = [&](long long row) {
+            while (row < a.rows && a.row_weight && a.row_weight[row] == 0.0f) row += step;
+            return row;
+        };
         int n = 0;
-        for (long long row = first_row; row < a.rows; row += step) {
-            if (a.row_weight && a.row_weight[row] == 0.0f) continue;
-            const int buf = n & 1;
-            wait_bar(&sh.teacher_empty[buf], ((n >> 1) & 1) ^ 1, a.health, abort_flag);
-            __syncwarp();
+        auto prepare = [&](long long row, int buf) {
             const float total = prepare_teacher<L>(a, row, entries[buf], scale);
-            if ((tid & 31) == 0) {
+            if (lane == 0) {
                 sh.some[buf] = total;
                 ptx::mbar_arrive(&sh.teacher_full[buf]);
             }
+        };
+        long long row = next_row(first_row);
+        if (row < a.rows) prepare(row, 0);
+        while (row < a.rows) {
+            const long long after = next_row(row + step);
+            const int buf = n & 1;
+            const Entries& entry = entries[buf];
+            if (after < a.rows) prepare(after, buf ^ 1);  // its last user was this warp
+            wait_bar(&sh.passed[buf], (n >> 1) & 1, a.health, abort_flag);
+            __syncwarp();
+            const Softmax soft = sh.softmax[buf];
+            const bool some = sh.some[buf] != 0.0f && soft.sum != 0.0f;
+            if (rank == 0) {
+                const float log_sum = logf(soft.sum);
+                float loss = 0.0f;
+                for (int k = lane; k < a.top; k += 32) {
+                    const float q = entry.q[k], v = entry.value[k];
+                    const float log_p = (soft.tame ? fmaf(v, scale, -soft.o) : (v - soft.base) * scale) * kLn2 - log_sum;
+                    if (some && q != 0.0f) loss += q * (logf(q) - log_p);
+                }
+                loss = warp_sum(loss);
+                if (lane == 0) a.row_loss[row] = some ? a.temperature * a.temperature * loss : 0.0f;
+            }
+            wait_bar(&sh.written[buf], (n >> 1) & 1, a.health, abort_flag);
+            __syncwarp();
+            if (a.dlogits && some) {
+                // over what the pass wrote: each CTA the tokens of its own slice
+                const Slice<L> in(a, row, rank, size);
+                const int lo = rank == 0 ? 0 : in.head + in.from * kN, hi = static_cast<int>(rank) == size - 1 ? in.tail : in.head + (in.from + in.count) * kN;
+                const float factor = (a.row_weight ? a.row_weight[row] : 1.0f) * grad_factor;
+                const float f = factor / soft.sum;
+                G* ds = static_cast<G*>(a.dlogits) + row * a.ld_dlogits;
+                for (int k = lane; k < a.top; k += 32) {
+                    const int token = entry.token[k];
+                    const float q = entry.all_q[k], v = entry.value[k];
+                    const bool own = (token >= lo && token < hi) || (rank == 0 && token >= in.tail);
+                    const float p = exp2_fast(soft.tame ? fmaf(v, scale, -soft.o) : (v - soft.base) * scale) * f;
+                    if (q != -1.0f && own) ds[token] = narrow<G>(p - factor * q);
+                }
+            }
+            __syncwarp();
+            row = after;
             ++n;
         }
     } else if (tid >= kConsumers) {  // ---- producer warp: one lane ----
@@ -620,51 +674,53 @@ __global__ void __launch_bounds__(kConsumers + 64, 2) stream_kernel(const rl2_di
         int slot = 0, n = 0, meeting = 0;
         uint32_t phase = 0;
         // A wait that fails (bounded, then the abort word) does not change the path: every barrier keeps its threads.
-        // over the CTA, then the cluster: a maximum and, unless `plain`, sums relative to it (as powers of two)
+        // over the CTA, then the cluster: a maximum and the sum (unless `plain`, relative to it as powers of two)
         auto meet = [&](float top, float sum, bool plain) {
-            auto join = [&](float& t, float& s2, float t2, float s3) {
-                const float m = fmaxf(t, t2);
-                if (!plain) s2 = s2 * exp2_fast(t - m) + s3 * exp2_fast(t2 - m);
-                t = m;
-            };
-            auto add = [&](float& t, float& s2, float t2, float s3) {
-                if (plain) {
-                    t = fmaxf(t, t2);
-                    s2 += s3;
-                } else {
-                    join(t, s2, t2, s3);
-                }
-            };
-#pragma unroll
-            for (int o = 16; o; o >>= 1) add(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o));
+            auto relative = [&](float t, float all) { return plain ? 1.0f : exp2_fast(t - all); };
+            float all = warp_max(top);
+            sum = warp_sum(sum * relative(top, all));
             const int buf = meeting & 1;
             if (lane == 0) {
-                sh.red[buf][warp] = top;
+                sh.red[buf][warp] = all;
                 sh.red2[buf][warp] = sum;
             }
             consumer_sync();
             top = sh.red[buf][lane & 15];
-            sum = sh.red2[buf][lane & 15];
-#pragma unroll
-            for (int o = 8; o; o >>= 1) add(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o));
+            all = warp_max(top);
+            sum = warp_sum(lane < kConsumers / 32 ? sh.red2[buf][lane & 15] * relative(top, all) : 0.0f);
             if (size > 1) {
                 if (warp == 0 && lane < size) {
                     const uint32_t to = ptx::cluster_addr(&sh.meet[buf][rank], lane);
-                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(top), "f"(sum) : "memory");
+                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(all), "f"(sum) : "memory");
                     ptx::mbar_arrive_cluster(ptx::cluster_addr(&sh.met[buf], lane));
                 }
                 wait_bar(&sh.met[buf], (meeting >> 1) & 1, a.health, abort_flag, true);
-                top = sh.meet[buf][0].x;
-                sum = sh.meet[buf][0].y;
-                for (int c = 1; c < size; ++c) add(top, sum, sh.meet[buf][c].x, sh.meet[buf][c].y);
+                const float2 x = sh.meet[buf][lane & (size - 1)];
+                all = warp_max(x.x);
+                sum = warp_sum(lane < size ? x.y * relative(x.x, all) : 0.0f);
             }
             ++meeting;
-            return make_float2(top, sum);
+            return make_float2(all, sum);
         };
+        // the next row's weight and edge, loaded while this row is worked on
+        struct Ahead {
+            float weight, edge;
+        };
+        auto load_ahead = [&](long long row) {
+            Ahead x{0.0f, -INFINITY};
+            if (row < a.rows) {
+                const Slice<L> in(a, row, rank, size);
+                x.weight = a.row_weight ? a.row_weight[row] : 1.0f;
+                if (rank == 0 && tid < in.head + (a.vocab - in.tail)) x.edge = to_float(in.s[tid < in.head ? tid : in.tail + tid - in.head]);
+            }
+            return x;
+        };
+        Ahead ahead = load_ahead(first_row);
         for (long long row = first_row; row < a.rows; row += step) {
             const Slice<L> in(a, row, rank, size);
             G* ds = a.dlogits ? static_cast<G*>(a.dlogits) + row * a.ld_dlogits : nullptr;
-            const float weight = a.row_weight ? a.row_weight[row] : 1.0f;
+            const float weight = ahead.weight, edge_now = ahead.edge;
+            ahead = load_ahead(row + step);
             if (weight == 0.0f) {
                 if (ds) {
                     const int lo = rank == 0 ? 0 : in.head + in.from * kN, hi = static_cast<int>(rank) == size - 1 ? a.vocab : in.head + (in.from + in.count) * kN;
@@ -677,7 +733,7 @@ __global__ void __launch_bounds__(kConsumers + 64, 2) stream_kernel(const rl2_di
             const int outside = in.head + (a.vocab - in.tail);
             const bool has_edge = rank == 0 && tid < outside;
             const int edge_at = tid < in.head ? tid : in.tail + tid - in.head;
-            const float edge = has_edge ? to_float(in.s[edge_at]) : -INFINITY;
+            const float edge = has_edge ? edge_now : -INFINITY;
             // f(vector of the slice, its elements) for this thread's vectors of chunk c in ring slot `at`
             auto chunk = [&](int c, int at, auto&& f) {
                 const uint4* data = reinterpret_cast<const uint4*>(ring + at * kChunk);
@@ -749,25 +805,17 @@ __global__ void __launch_bounds__(kConsumers + 64, 2) stream_kernel(const rl2_di
                 again([&](float v) { sum += exp2_fast((v - base) * scale); });
                 sum = meet(0.0f, sum, true).y;
             }
-            // ---- loss ----
             const int buf = n & 1;
+            // the teacher warp arrives here for a row once it is done with the row before the last, so the
+            // slots of that one are free
             wait_bar(&sh.teacher_full[buf], (n >> 1) & 1, a.health, abort_flag);
-            const Entries& entry = entries[buf];
-            const bool some = sh.some[buf] != 0.0f && sum != 0.0f;
-            const float log_sum = logf(sum);
-            auto log_p = [&](float v) { return (tame ? fmaf(v, scale, -o) : (v - base) * scale) * kLn2 - log_sum; };
-            if (rank == 0) {
-                float loss = 0.0f;
-                for (int k = tid; k < a.top; k += kConsumers) {
-                    const float q = entry.q[k];
-                    if (some && q != 0.0f) loss += q * (logf(q) - log_p(entry.value[k]));
-                }
-                loss = warp_sum(loss);
-                if (lane == 0) sh.loss[warp] = loss;
+            if (tid == 0) {
+                sh.softmax[buf] = Softmax{o, base, sum, tame};
+                ptx::mbar_arrive(&sh.passed[buf]);
             }
             // ---- gradient ----
-            const float factor = weight * a.loss_weight * a.temperature * (a.grad_scale ? *a.grad_scale : 1.0f);
-            const float f = factor / sum;
+            const bool some = sh.some[buf] != 0.0f && sum != 0.0f;
+            const float f = weight * grad_factor / sum;
             auto grad = [&](float v) {
                 if (tame) return exp2_fast(fmaf(v, scale, -o)) * f;
                 return exp2_fast((v - base) * scale) * f;
@@ -801,23 +849,8 @@ __global__ void __launch_bounds__(kConsumers + 64, 2) stream_kernel(const rl2_di
                 write(std::true_type{});
             else
                 write(std::false_type{});
-            // the teacher's tokens, over what the pass wrote: each CTA those of its own slice
-            consumer_sync();
-            if (tid < 32 && rank == 0) {
-                const float loss = warp_sum(lane < kConsumers / 32 ? sh.loss[lane] : 0.0f);
-                if (lane == 0) a.row_loss[row] = some ? a.temperature * a.temperature * loss : 0.0f;
-            }
-            if (ds && some) {
-                const int lo = rank == 0 ? 0 : in.head + in.from * kN, hi = static_cast<int>(rank) == size - 1 ? in.tail : in.head + (in.from + in.count) * kN;
-                for (int k = tid; k < a.top; k += kConsumers) {
-                    const int token = entry.token[k];
-                    const float q = entry.all_q[k];
-                    const bool own = (token >= lo && token < hi) || (rank == 0 && token >= in.tail);
-                    if (q != -1.0f && own) ds[token] = narrow<G>(grad(entry.value[k]) - factor * q);
-                }
-            }
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&sh.teacher_empty[buf]);
+            if (lane == 0) ptx::mbar_arrive(&sh.written[buf]);
             ++n;
         }
     }
