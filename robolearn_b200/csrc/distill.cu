@@ -7,8 +7,8 @@
 //   ds_j     = c w_n T (p_j - sum_{k: i_k = j} q_k) (* *grad_scale)
 //
 // A row is read from memory once and stays on the chip between its two passes (running maximum and
-// sum of the softmax; gradient): in a warp's registers up to 1024 tokens, in L1 / L2 behind a CTA up to
-// 8192, and above that in the shared memory of a CTA or of a cluster of CTAs (stream_kernel). All sums
+// sum of the softmax; gradient): in L1 behind a warp (up to 1024 tokens) or a CTA (up to
+// 2048), and above that in the registers of a CTA or of a cluster of CTAs (long_kernel). All sums
 // are fp32; exponentials are the hardware's exp2 of s log2(e) / T less the same of the maximum, so every
 // value is within a few units in the last place of fp32 times 1 + its argument.
 
@@ -18,7 +18,6 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 namespace rl2 {
@@ -321,66 +320,37 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const rl2_distill_args a) 
     finish(a);
 }
 
-// ---- long rows: streamed through shared memory -------------------------------------------
+// ---- long rows: in the registers of a CTA or a cluster ----------------------------------
 //
-// A cluster of CTAs holds a row, each CTA a slice of its 16-byte vectors, in a ring of 16 KB chunks that a
-// producer warp fills with bulk copies: while the second pass over a row frees chunks, the next row's are on
-// their way. Another warp prepares the next row's teacher (softmax, first entry of each token). 512 consumer
-// threads make the two passes; the CTAs of a cluster exchange their maxima and sums through shared
-// memory with one barrier a row. The few elements of a row outside its 16-byte vectors are read where they lie.
+// A cluster of CTAs holds a row, VPT 16-byte vectors a thread, all of them loaded at once: one read of the row,
+// no staging, and two (VPT 8) or three CTAs an SM, so that one loads while another computes. The CTAs of a
+// cluster exchange their maxima and sums through shared memory. The teacher's entries are a thread's each: their
+// loads and their softmax go along with the row's. The first entry of each token writes the token's gradient
+// over what the second pass wrote. The few elements of a row outside its 16-byte vectors are one thread's each.
 //
-// The passes keep the offset o = max log2(e) / T instead of the maximum: p = 2^(s c - o) / sum needs one
-// multiply-add and one exp2 an element, and the rounding of o cancels. Rows where that does not hold (no logit
-// above -1e30, or one above 1e30 after scaling, or NaN) are done again from (s - max) c.
+// The passes use the offset o = max log2(e) / T: p = 2^(s c - o) / sum needs one multiply-add and one exp2 an
+// element, and the rounding of o cancels. Rows where that does not hold (no logit above -1e30, or one above
+// 1e30 after scaling, or NaN) are done again from (s - max) c.
 
-constexpr int kChunk = 16384;
-constexpr int kConsumers = 512;
-constexpr int kMaxSlots = 13;
+constexpr int kLong = 512;  // threads of a CTA
+constexpr int kLongWarps = kLong / 32;
 constexpr int kMaxCluster = 8;
 constexpr float kTame = 1e30f;
 
-// A row's teacher entries, in arrays of kMaxTop or fewer (a multiple of 4).
-struct Entries {
-    int* token;    // -1: absent
-    float* q;      // this entry's
-    float* all_q;  // of all entries of the token, at its first entry; -1 elsewhere
-    float* value;  // the student's logit
-
-    __host__ __device__ static constexpr int padded(int top) { return (top + 3) / 4 * 4; }
-    __host__ __device__ static constexpr int bytes(int top) { return padded(top) * 16; }
-    __device__ __forceinline__ Entries(uint8_t* at, int top) {
-        token = reinterpret_cast<int*>(at);
-        q = reinterpret_cast<float*>(token + padded(top));
-        all_q = q + padded(top);
-        value = all_q + padded(top);
-    }
-};
-
-// A row's softmax after the first pass: p = 2^(s c - o) / sum where tame, else 2^((s - base) c) / sum.
-struct Softmax {
-    float o, base, sum;
-    bool tame;
-};
-
-struct Stream {
-    uint64_t full[kMaxSlots], empty[kMaxSlots];
-    uint64_t teacher_full[2], passed[2], written[2];
+struct Meeting {
     uint64_t met[2];
     float2 meet[2][kMaxCluster];
-    float red[2][kConsumers / 32], red2[2][kConsumers / 32];
-    float some[2];  // sum of the teacher's weights: 0 without an entry
-    Softmax softmax[2];
-    int abort;
+    float top[2][kLongWarps], sum[2][kLongWarps];
+    Running teacher[kLongWarps];
+    float loss[kLongWarps];
 };
 
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, int* health, volatile int* abort_flag, bool cluster = false) {
+// mbarrier that other CTAs of the cluster arrive on; bounded to 4 s (then the timeout bit of *health)
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, int* health) {
     auto done = [&] {
         uint32_t ok;
-        if (cluster)
-            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                         : "=r"(ok) : "r"(ptx::smem_u32(bar)), "r"(phase) : "memory");
-        else
-            ok = ptx::mbar_try_wait(bar, phase);
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(ptx::smem_u32(bar)), "r"(phase) : "memory");
         return ok != 0;
     };
     if (done()) return true;
@@ -389,18 +359,14 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, int* hea
     for (uint32_t i = 1;; ++i) {
         if (done()) return true;
         if ((i & 1023u) == 0) {
-            if (*abort_flag) return false;
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
             if (now - start > 4000000000ull) {
                 if (health) atomicOr(health, kHealthTimeout);
-                *abort_flag = 1;
                 return false;
             }
         }
     }
 }
-
-__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); }
 
 // A row's 16-byte vectors and the slice of them that this CTA holds.
 template <typename L>
@@ -408,7 +374,7 @@ struct Slice {
     static constexpr int kN = 16 / sizeof(L);
     const L* s;
     int head, vectors, tail;  // elements before the first vector, vectors, first element after them
-    int from, count, chunks;
+    int from, count;
 
     __device__ __forceinline__ Slice(const rl2_distill_args& a, long long row, uint32_t rank, uint32_t size) {
         s = static_cast<const L*>(a.logits) + row * a.ld_logits;
@@ -419,7 +385,6 @@ struct Slice {
         const int shift = 31 - __clz(size);  // a power of two
         from = static_cast<int>(static_cast<unsigned long long>(vectors) * rank >> shift);
         count = static_cast<int>(static_cast<unsigned long long>(vectors) * (rank + 1) >> shift) - from;
-        chunks = (count * 16 + kChunk - 1) / kChunk;
     }
 };
 
@@ -439,6 +404,11 @@ __device__ __forceinline__ void unpack_as(uint4 x, float (&v)[8], __nv_bfloat16)
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[2 * k] = __uint_as_float(w[k] << 16), v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
 }
+// a vector of -inf
+__device__ __forceinline__ uint4 nothing(float) { return make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u); }
+__device__ __forceinline__ uint4 nothing(__half) { return make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u); }
+__device__ __forceinline__ uint4 nothing(__nv_bfloat16) { return make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u); }
+
 template <typename L>
 __device__ __forceinline__ void unpack(uint4 x, float (&v)[16 / sizeof(L)]) {
     unpack_as(x, v, L(0.0f));
@@ -469,394 +439,257 @@ __device__ __forceinline__ void store_vector(G* to, const float (&y)[N]) {
     }
 }
 
-// One warp: the row's teacher; returns the sum of its weights. Entries go four to a lane, so that the loads of
-// 128 are in flight together.
-template <typename L>
-__device__ __forceinline__ float prepare_teacher(const rl2_distill_args& a, long long row, const Entries entry, float scale) {
-    constexpr int kEach = 4;
-    const int lane = threadIdx.x & 31;
-    const int K = a.top, padded = Entries::padded(K);
-    const L* s = static_cast<const L*>(a.logits) + row * a.ld_logits;
-    float top = -INFINITY;
-    bool bad = false;
-    for (int k0 = 0; k0 < padded; k0 += 32 * kEach) {
-        long long i[kEach];
-        float v[kEach], z[kEach];
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int k = k0 + e * 32 + lane;
-            i[e] = k < K ? teacher_index(a, row, k) : -1;
-            v[e] = k < K ? teacher_value(a, row, k) : -INFINITY;
-        }
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) z[e] = i[e] >= 0 && i[e] < a.vocab ? to_float(s[i[e]]) : 0.0f;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int k = k0 + e * 32 + lane;
-            const bool here = i[e] >= 0 && i[e] < a.vocab;
-            bad |= i[e] >= a.vocab;
-            if (!here) v[e] = -INFINITY;
-            top = fmaxf(top, v[e]);
-            if (k < padded) {
-                entry.token[k] = here ? static_cast<int>(i[e]) : -1;
-                entry.q[k] = v[e];
-                entry.value[k] = z[e];
-            }
-        }
-    }
-    if (bad && a.health) atomicOr(a.health, kHealthIndex);
-    top = warp_max(top);
-    float total = 0.0f;
-    for (int k = lane; k < K; k += 32)
-        if (entry.q[k] != -INFINITY) total += exp2_fast((entry.q[k] - top) * scale);
-    total = warp_sum(total);
-    const float inverse = 1.0f / total;
-    bool repeated = false;
-    __syncwarp();
-    for (int k0 = 0; k0 < K; k0 += 32 * kEach) {
-        int token[kEach], same[kEach];
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int k = k0 + e * 32 + lane;
-            token[e] = k < K ? entry.token[k] : -1;
-            same[e] = 0;
-            if (k < K) {
-                const float q = entry.q[k] == -INFINITY ? 0.0f : exp2_fast((entry.q[k] - top) * scale) * inverse;
-                entry.q[k] = q;
-                entry.all_q[k] = token[e] >= 0 ? q : -1.0f;
-            }
-        }
-#pragma unroll 4
-        for (int j = 0; j < padded; j += 4) {
-            const int4 t = *reinterpret_cast<const int4*>(entry.token + j);
-#pragma unroll
-            for (int e = 0; e < kEach; ++e)
-                same[e] += (t.x == token[e]) + (t.y == token[e]) + (t.z == token[e]) + (t.w == token[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) repeated |= token[e] >= 0 && same[e] > 1;
-    }
-    if (__any_sync(0xffffffffu, repeated)) {
-        for (int k = lane; k < K; k += 32) {
-            float q = 0.0f;
-            bool first = entry.token[k] >= 0;
-            for (int j = 0; j < K; ++j)
-                if (entry.token[j] == entry.token[k]) {
-                    first &= j >= k;
-                    q += entry.q[j];
-                }
-            entry.all_q[k] = first ? q : -1.0f;
-        }
-    }
-    __syncwarp();
-    return total;
-}
-
-template <typename L, typename G>
-__global__ void __launch_bounds__(kConsumers + 64, 2) stream_kernel(const rl2_distill_args a, const int size, const int slots) {
-    extern __shared__ __align__(128) uint8_t ring[];  // chunks, then two rows' teacher entries
-    __shared__ Stream sh;
+template <typename L, typename G, int VPT>
+__global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kernel(const rl2_distill_args a, const int size) {
+    extern __shared__ __align__(16) uint8_t raw[];  // the teacher's entries
+    __shared__ Meeting sh;
     constexpr int kN = Slice<L>::kN;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = size > 1 ? ptx::cluster_rank() : 0u;
-    volatile int* abort_flag = &sh.abort;
+    const long long row = blockIdx.x / size;
+    const Slice<L> in(a, row, rank, size);
+    const int K = a.top, padded = (K + 3) / 4 * 4;
+    int* token = reinterpret_cast<int*>(raw);                  // -1: absent
+    float* given = reinterpret_cast<float*>(token + padded);   // the teacher's value
+    float* own = given + padded;                               // the student's
     const float scale = kLog2e / a.temperature;
-    const Entries entries[2] = {Entries(ring + slots * kChunk, a.top), Entries(ring + slots * kChunk + Entries::bytes(a.top), a.top)};
+    const float weight = a.row_weight ? a.row_weight[row] : 1.0f;
+    G* ds = a.dlogits ? static_cast<G*>(a.dlogits) + row * a.ld_dlogits : nullptr;
+    if (weight == 0.0f) {
+        const int lo = rank == 0 ? 0 : in.head + in.from * kN, hi = static_cast<int>(rank) == size - 1 ? a.vocab : in.head + (in.from + in.count) * kN;
+        if (ds)
+            for (int j = lo + tid; j < hi; j += kLong) ds[j] = narrow<G>(0.0f);
+        if (tid == 0 && rank == 0) a.row_loss[row] = 0.0f;
+        finish(a);
+        return;
+    }
     if (tid == 0) {
-        for (int i = 0; i < slots; ++i) {
-            ptx::mbar_init(&sh.full[i], 1);
-            ptx::mbar_init(&sh.empty[i], kConsumers / 32);
-        }
-        for (int i = 0; i < 2; ++i) {
-            ptx::mbar_init(&sh.teacher_full[i], 1);
-            ptx::mbar_init(&sh.passed[i], 1);
-            ptx::mbar_init(&sh.written[i], kConsumers / 32);
-            ptx::mbar_init(&sh.met[i], size);
-        }
-        sh.abort = 0;
+        for (int i = 0; i < 2; ++i) ptx::mbar_init(&sh.met[i], size);
         ptx::fence_barrier_init();
     }
-    __syncthreads();
-    if (size > 1) ptx::cluster_sync();
-    const long long first_row = blockIdx.x / size, step = gridDim.x / size;
-
-    const float grad_factor = a.loss_weight * a.temperature * (a.grad_scale ? *a.grad_scale : 1.0f);
-    if (tid >= kConsumers + 32) {
-        // ---- teacher warp: the next row's teacher, then the row's loss and its teacher's tokens ----
-        const int lane = tid & 31;
-        auto next_row = [&](long long row) {
-            while (row < a.rows && a.row_weight && a.row_weight[row] == 0.0f) row += step;
-            return row;
-        };
-        int n = 0;
-        auto prepare = [&](long long row, int buf) {
-            const float total = prepare_teacher<L>(a, row, entries[buf], scale);
-            if (lane == 0) {
-                sh.some[buf] = total;
-                ptx::mbar_arrive(&sh.teacher_full[buf]);
-            }
-        };
-        long long row = next_row(first_row);
-        if (row < a.rows) prepare(row, 0);
-        while (row < a.rows) {
-            const long long after = next_row(row + step);
-            const int buf = n & 1;
-            const Entries& entry = entries[buf];
-            if (after < a.rows) prepare(after, buf ^ 1);  // its last user was this warp
-            wait_bar(&sh.passed[buf], (n >> 1) & 1, a.health, abort_flag);
-            __syncwarp();
-            const Softmax soft = sh.softmax[buf];
-            const bool some = sh.some[buf] != 0.0f && soft.sum != 0.0f;
-            if (rank == 0) {
-                const float log_sum = logf(soft.sum);
-                float loss = 0.0f;
-                for (int k = lane; k < a.top; k += 32) {
-                    const float q = entry.q[k], v = entry.value[k];
-                    const float log_p = (soft.tame ? fmaf(v, scale, -soft.o) : (v - soft.base) * scale) * kLn2 - log_sum;
-                    if (some && q != 0.0f) loss += q * (logf(q) - log_p);
-                }
-                loss = warp_sum(loss);
-                if (lane == 0) a.row_loss[row] = some ? a.temperature * a.temperature * loss : 0.0f;
-            }
-            wait_bar(&sh.written[buf], (n >> 1) & 1, a.health, abort_flag);
-            __syncwarp();
-            if (a.dlogits && some) {
-                // over what the pass wrote: each CTA the tokens of its own slice
-                const Slice<L> in(a, row, rank, size);
-                const int lo = rank == 0 ? 0 : in.head + in.from * kN, hi = static_cast<int>(rank) == size - 1 ? in.tail : in.head + (in.from + in.count) * kN;
-                const float factor = (a.row_weight ? a.row_weight[row] : 1.0f) * grad_factor;
-                const float f = factor / soft.sum;
-                G* ds = static_cast<G*>(a.dlogits) + row * a.ld_dlogits;
-                for (int k = lane; k < a.top; k += 32) {
-                    const int token = entry.token[k];
-                    const float q = entry.all_q[k], v = entry.value[k];
-                    const bool own = (token >= lo && token < hi) || (rank == 0 && token >= in.tail);
-                    const float p = exp2_fast(soft.tame ? fmaf(v, scale, -soft.o) : (v - soft.base) * scale) * f;
-                    if (q != -1.0f && own) ds[token] = narrow<G>(p - factor * q);
-                }
-            }
-            __syncwarp();
-            row = after;
-            ++n;
-        }
-    } else if (tid >= kConsumers) {  // ---- producer warp: one lane ----
-        if (tid == kConsumers) {
-            long long issued = 0;
-            int slot = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (long long row = first_row; row < a.rows && ok; row += step) {
-                if (a.row_weight && a.row_weight[row] == 0.0f) continue;
-                const Slice<L> in(a, row, rank, size);
-                const uint8_t* from = reinterpret_cast<const uint8_t*>(in.s + in.head) + in.from * 16ll;
-                for (int c = 0; c < in.chunks; ++c) {
-                    ok = wait_bar(&sh.empty[slot], phase ^ 1, a.health, abort_flag);
-                    if (!ok) break;
-                    const uint32_t bytes = static_cast<uint32_t>(min(kChunk, in.count * 16 - c * kChunk));
-                    ptx::mbar_arrive_expect_tx(&sh.full[slot], bytes);
-                    ptx::bulk_load(ring + slot * kChunk, from + c * static_cast<long long>(kChunk), bytes, &sh.full[slot]);
-                    ++issued;
-                    if (++slot == slots) {
-                        slot = 0;
-                        phase ^= 1;
-                    }
-                }
-            }
-            // every chunk asked for has landed before the CTA may end, also after an abort
-            for (int i = 0; i < slots; ++i) {
-                const long long armed = issued > i ? (issued - 1 - i) / slots + 1 : 0;
-                volatile int none = 0;
-                if (armed > 0) wait_bar(&sh.full[i], static_cast<uint32_t>((armed - 1) & 1), a.health, &none);
-            }
-        }
-    } else {  // ---- consumers ----
-        const int lane = tid & 31, warp = tid >> 5;
-        int slot = 0, n = 0, meeting = 0;
-        uint32_t phase = 0;
-        // A wait that fails (bounded, then the abort word) does not change the path: every barrier keeps its threads.
-        // over the CTA, then the cluster: a maximum and the sum (unless `plain`, relative to it as powers of two)
-        auto meet = [&](float top, float sum, bool plain) {
-            auto relative = [&](float t, float all) { return plain ? 1.0f : exp2_fast(t - all); };
-            float all = warp_max(top);
-            sum = warp_sum(sum * relative(top, all));
-            const int buf = meeting & 1;
-            if (lane == 0) {
-                sh.red[buf][warp] = all;
-                sh.red2[buf][warp] = sum;
-            }
-            consumer_sync();
-            top = sh.red[buf][lane & 15];
-            all = warp_max(top);
-            sum = warp_sum(lane < kConsumers / 32 ? sh.red2[buf][lane & 15] * relative(top, all) : 0.0f);
-            if (size > 1) {
-                if (warp == 0 && lane < size) {
-                    const uint32_t to = ptx::cluster_addr(&sh.meet[buf][rank], lane);
-                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(all), "f"(sum) : "memory");
-                    ptx::mbar_arrive_cluster(ptx::cluster_addr(&sh.met[buf], lane));
-                }
-                wait_bar(&sh.met[buf], (meeting >> 1) & 1, a.health, abort_flag, true);
-                const float2 x = sh.meet[buf][lane & (size - 1)];
-                all = warp_max(x.x);
-                sum = warp_sum(lane < size ? x.y * relative(x.x, all) : 0.0f);
-            }
-            ++meeting;
-            return make_float2(all, sum);
-        };
-        // the next row's weight and edge, loaded while this row is worked on
-        struct Ahead {
-            float weight, edge;
-        };
-        auto load_ahead = [&](long long row) {
-            Ahead x{0.0f, -INFINITY};
-            if (row < a.rows) {
-                const Slice<L> in(a, row, rank, size);
-                x.weight = a.row_weight ? a.row_weight[row] : 1.0f;
-                if (rank == 0 && tid < in.head + (a.vocab - in.tail)) x.edge = to_float(in.s[tid < in.head ? tid : in.tail + tid - in.head]);
-            }
-            return x;
-        };
-        Ahead ahead = load_ahead(first_row);
-        for (long long row = first_row; row < a.rows; row += step) {
-            const Slice<L> in(a, row, rank, size);
-            G* ds = a.dlogits ? static_cast<G*>(a.dlogits) + row * a.ld_dlogits : nullptr;
-            const float weight = ahead.weight, edge_now = ahead.edge;
-            ahead = load_ahead(row + step);
-            if (weight == 0.0f) {
-                if (ds) {
-                    const int lo = rank == 0 ? 0 : in.head + in.from * kN, hi = static_cast<int>(rank) == size - 1 ? a.vocab : in.head + (in.from + in.count) * kN;
-                    for (int j = lo + tid; j < hi; j += kConsumers) ds[j] = narrow<G>(0.0f);
-                }
-                if (tid == 0 && rank == 0) a.row_loss[row] = 0.0f;
-                continue;
-            }
-            // elements outside the vectors: one a thread, on the first CTA
-            const int outside = in.head + (a.vocab - in.tail);
-            const bool has_edge = rank == 0 && tid < outside;
-            const int edge_at = tid < in.head ? tid : in.tail + tid - in.head;
-            const float edge = has_edge ? edge_now : -INFINITY;
-            // f(vector of the slice, its elements) for this thread's vectors of chunk c in ring slot `at`
-            auto chunk = [&](int c, int at, auto&& f) {
-                const uint4* data = reinterpret_cast<const uint4*>(ring + at * kChunk);
-                const int left = in.count - c * (kChunk / 16);
+    // this thread's vectors, and its element outside them
+    constexpr int kHeld = VPT > 0 ? VPT : 4;  // VPT 0: four at a time, read again by the second pass
+    uint4 x[kHeld];
+    const uint4* data = reinterpret_cast<const uint4*>(in.s + in.head) + in.from + tid;
+    auto load = [&](int first) {
 #pragma unroll
-                for (int k = 0; k < kChunk / 16 / kConsumers; ++k) {
-                    const int i = k * kConsumers + tid;
-                    if (i < left) f(c * (kChunk / 16) + i, data[i]);
-                }
-            };
-            auto next = [&](int& at, uint32_t& ph) {
-                if (++at == slots) {
-                    at = 0;
-                    ph ^= 1;
-                }
-            };
-            // ---- first pass ----
-            float o = -kTame, sum = 0.0f;
-            int at = slot;
-            uint32_t ph = phase;
-            if (has_edge && edge * scale > o) {
-                o = edge * scale;
-                sum = exp2_fast(fmaf(edge, scale, -o));
-            } else if (edge != edge) {
-                sum = edge;
+        for (int k = 0; k < kHeld; ++k)
+            x[k] = first + k * kLong + tid < in.count ? __ldg(data + first + k * kLong) : nothing(L(0.0f));
+    };
+    load(0);
+    const bool has_edge = rank == 0 && tid < in.head + (a.vocab - in.tail);
+    const int edge_at = tid < in.head ? tid : in.tail + tid - in.head;
+    const float edge = has_edge ? to_float(in.s[edge_at]) : -INFINITY;
+    // the teacher: its softmax as a running one
+    Running teacher{-INFINITY, 0.0f};
+    for (int k = tid; k < padded; k += kLong) {
+        const long long i = k < K ? teacher_index(a, row, k) : -1;
+        if (i >= a.vocab && a.health) atomicOr(a.health, kHealthIndex);
+        const bool here = i >= 0 && i < a.vocab;
+        const float v = here ? teacher_value(a, row, k) : -INFINITY;
+        token[k] = here ? static_cast<int>(i) : -1;
+        given[k] = v;
+        own[k] = here ? to_float(in.s[i]) : 0.0f;
+        teacher = merge(teacher, Running{v, v == -INFINITY ? 0.0f : (v == v ? 1.0f : v)}, scale);
+    }
+    if (warp * 32 < K) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            teacher = merge(teacher, Running{__shfl_xor_sync(0xffffffffu, teacher.max, o), __shfl_xor_sync(0xffffffffu, teacher.sum, o)}, scale);
+    }
+    if (lane == 0) sh.teacher[warp] = teacher;
+    if (size > 1) ptx::cluster_sync();  // the peers' barriers exist
+    const float factor = weight * a.loss_weight * a.temperature * (a.grad_scale ? *a.grad_scale : 1.0f);
+    int meeting = 0;
+    // over the CTA, then the cluster: a maximum and the sum (unless `plain`, relative to it as powers of two)
+    auto meet = [&](float top, float sum, bool plain) {
+        auto relative = [&](float t, float all) { return plain ? 1.0f : exp2_fast(t - all); };
+        float all = warp_max(top);
+        sum = warp_sum(sum * relative(top, all));
+        const int buf = meeting & 1;
+        if (lane == 0) {
+            sh.top[buf][warp] = all;
+            sh.sum[buf][warp] = sum;
+        }
+        __syncthreads();
+        top = sh.top[buf][lane % kLongWarps];
+        all = warp_max(top);
+        sum = warp_sum(lane < kLongWarps ? sh.sum[buf][lane % kLongWarps] * relative(top, all) : 0.0f);
+        if (size > 1) {
+            if (warp == 0 && lane < size) {
+                const uint32_t to = ptx::cluster_addr(&sh.meet[buf][rank], lane);
+                asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(all), "f"(sum) : "memory");
+                ptx::mbar_arrive_cluster(ptx::cluster_addr(&sh.met[buf], lane));
             }
-            for (int c = 0; c < in.chunks; ++c) {
-                wait_bar(&sh.full[at], ph, a.health, abort_flag);
-                chunk(c, at, [&](int, uint4 x) {
+            wait_bar(&sh.met[buf], (meeting >> 1) & 1, a.health);
+            const float2 y = sh.meet[buf][lane & (size - 1)];
+            all = warp_max(y.x);
+            sum = warp_sum(lane < size ? y.y * relative(y.x, all) : 0.0f);
+        }
+        ++meeting;
+        return make_float2(all, sum);
+    };
+    // ---- first pass ----
+    float o = fmaxf(edge * scale, -kTame);
+    float sum = exp2_fast(fmaf(edge, scale, -o));  // 0 without one (-inf)
+    for (int first = 0;;) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            float v[kN];
+            unpack<L>(x[k], v);
+            m = fmaxf(m, most_as(x[k], v, L(0.0f)));
+        }
+        const float up = fmaxf(o, m * scale);
+        sum *= exp2_fast(o - up);
+        o = up;
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            float v[kN], part = 0.0f;
+            unpack<L>(x[k], v);
+#pragma unroll
+            for (int e = 0; e < kN; e += 2) {
+                sum += exp2_fast(fmaf(v[e], scale, -o));
+                part += exp2_fast(fmaf(v[e + 1], scale, -o));
+            }
+            sum += part;
+        }
+        first += kHeld * kLong;
+        if (VPT > 0 || first >= in.count) break;
+        load(first);
+    }
+    const float2 whole = meet(o, sum, false);
+    o = whole.x;
+    sum = whole.y;
+    teacher = sh.teacher[lane % kLongWarps];
+#pragma unroll
+    for (int w = kLongWarps / 2; w; w >>= 1)
+        teacher = merge(teacher, Running{__shfl_xor_sync(0xffffffffu, teacher.max, w), __shfl_xor_sync(0xffffffffu, teacher.sum, w)}, scale);
+    float base = 0.0f;
+    const bool tame = o < kTame && sum > 0.0f;
+    if (!tame) {  // from (s - max) c
+        auto each = [&](auto&& f) {
+            if (has_edge) f(edge);
+            for (int first = 0; first < in.count; first += kHeld * kLong) {
+                if (VPT == 0) load(first);
+#pragma unroll
+                for (int k = 0; k < kHeld; ++k) {
+                    if (first + k * kLong + tid >= in.count) continue;
                     float v[kN];
-                    unpack<L>(x, v);
-                    const float up = fmaxf(o, most_as(x, v, L(0.0f)) * scale);
-                    sum *= exp2_fast(o - up);
-                    float part = 0.0f;
+                    unpack<L>(x[k], v);
 #pragma unroll
-                    for (int e = 0; e < kN; e += 2) {
-                        sum += exp2_fast(fmaf(v[e], scale, -up));
-                        part += exp2_fast(fmaf(v[e + 1], scale, -up));
-                    }
-                    sum += part;
-                    o = up;
-                });
-                next(at, ph);
-            }
-            const float2 whole = meet(o, sum, false);
-            o = whole.x;
-            sum = whole.y;
-            float base = 0.0f;
-            const bool tame = o < kTame && sum > 0.0f;
-            if (!tame) {  // from (s - max) c
-                float m = edge;
-                auto again = [&](auto&& f) {
-                    int s2 = slot;
-                    uint32_t p2 = phase;
-                    for (int c = 0; c < in.chunks; ++c) {
-                        chunk(c, s2, [&](int, uint4 x) {
-                            float v[kN];
-                            unpack<L>(x, v);
-#pragma unroll
-                            for (int e = 0; e < kN; ++e) f(v[e]);
-                        });
-                        next(s2, p2);
-                    }
-                };
-                again([&](float v) { m = fmaxf(m, v); });
-                base = meet(m, 0.0f, true).x;
-                if (base == -INFINITY) base = 0.0f;
-                sum = has_edge ? exp2_fast((edge - base) * scale) : 0.0f;
-                again([&](float v) { sum += exp2_fast((v - base) * scale); });
-                sum = meet(0.0f, sum, true).y;
-            }
-            const int buf = n & 1;
-            // the teacher warp arrives here for a row once it is done with the row before the last, so the
-            // slots of that one are free
-            wait_bar(&sh.teacher_full[buf], (n >> 1) & 1, a.health, abort_flag);
-            if (tid == 0) {
-                sh.softmax[buf] = Softmax{o, base, sum, tame};
-                ptx::mbar_arrive(&sh.passed[buf]);
-            }
-            // ---- gradient ----
-            const bool some = sh.some[buf] != 0.0f && sum != 0.0f;
-            const float f = weight * grad_factor / sum;
-            auto grad = [&](float v) {
-                if (tame) return exp2_fast(fmaf(v, scale, -o)) * f;
-                return exp2_fast((v - base) * scale) * f;
-            };
-            if (has_edge && ds) ds[edge_at] = narrow<G>(some ? grad(edge) : 0.0f);
-            G* out = ds ? ds + in.head + static_cast<long long>(in.from) * kN : nullptr;
-            const bool vec = reinterpret_cast<uintptr_t>(out) % (sizeof(G) * kN <= 16 ? sizeof(G) * kN : 16) == 0;
-            auto write = [&](auto is_tame) {
-                for (int c = 0; c < in.chunks; ++c) {
-                    if (out)
-                        chunk(c, slot, [&](int i, uint4 x) {
-                            float v[kN];
-                            unpack<L>(x, v);
-#pragma unroll
-                            for (int e = 0; e < kN; ++e)
-                                v[e] = decltype(is_tame)::value ? exp2_fast(fmaf(v[e], scale, -o)) * f : (some ? grad(v[e]) : 0.0f);
-                            G* to = out + static_cast<long long>(i) * kN;
-                            if (vec) {
-                                store_vector<G, kN>(to, v);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < kN; ++e) to[e] = narrow<G>(v[e]);
-                            }
-                        });
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(&sh.empty[slot]);
-                    next(slot, phase);
+                    for (int e = 0; e < kN; ++e) f(v[e]);
                 }
-            };
-            if (tame && some)
-                write(std::true_type{});
-            else
-                write(std::false_type{});
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&sh.written[buf]);
-            ++n;
-        }
+            }
+        };
+        float m = -INFINITY;
+        each([&](float v) { m = fmaxf(m, v); });
+        base = meet(m, 0.0f, true).x;
+        if (base == -INFINITY) base = 0.0f;
+        sum = 0.0f;
+        each([&](float v) { sum += exp2_fast((v - base) * scale); });
+        sum = meet(0.0f, sum, true).y;
+    }
+    const bool some = teacher.sum != 0.0f && sum != 0.0f;  // a teacher entry and a logit that are not -inf (NaN passes)
+    const float f = factor / sum;
+    auto grad = [&](float v) {
+        if (tame) return exp2_fast(fmaf(v, scale, -o)) * f;
+        return exp2_fast((v - base) * scale) * f;
+    };
+    // ---- second pass ----
+    if (ds) {
+        if (has_edge) ds[edge_at] = narrow<G>(some ? grad(edge) : 0.0f);
+        G* out = ds + in.head + (static_cast<long long>(in.from) + tid) * kN;
+        const bool vec = reinterpret_cast<uintptr_t>(out) % (sizeof(G) * kN <= 16 ? sizeof(G) * kN : 16) == 0;
+        auto write = [&](auto is_plain) {
+            for (int first = 0; first < in.count; first += kHeld * kLong) {
+                if (VPT == 0) load(first);
+#pragma unroll
+                for (int k = 0; k < kHeld; ++k) {
+                    float v[kN];
+                    unpack<L>(x[k], v);
+#pragma unroll
+                    for (int e = 0; e < kN; ++e)
+                        v[e] = decltype(is_plain)::value ? exp2_fast(fmaf(v[e], scale, -o)) * f : (some ? grad(v[e]) : 0.0f);
+                    if (first + k * kLong + tid >= in.count) break;
+                    G* to = out + (first + k * kLong) * static_cast<long long>(kN);
+                    if (vec) {
+                        store_vector<G, kN>(to, v);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < kN; ++e) to[e] = narrow<G>(v[e]);
+                    }
+                }
+            }
+        };
+        if (tame && some)
+            write(std::true_type{});
+        else
+            write(std::false_type{});
     }
     __syncthreads();
-    if (size > 1) ptx::cluster_sync();  // no CTA leaves while another may write into its shared memory
+    // ---- the teacher's entries: loss, and the gradient of the tokens of this CTA's part of the row ----
+    const float inverse = 1.0f / teacher.sum, log_total = logf(teacher.sum), log_sum = logf(sum);
+    auto share = [&](int k) { return given[k] == -INFINITY ? 0.0f : exp2_fast((given[k] - teacher.max) * scale) * inverse; };
+    const int lo = rank == 0 ? 0 : in.head + in.from * kN, hi = in.head + (in.from + in.count) * kN;
+    float loss = 0.0f;
+    if (some) {
+        for (int k = tid; k < K; k += kLong) {
+            const int i = token[k];
+            float q = share(k);
+            if (rank == 0 && q != 0.0f)
+                loss += q * (((given[k] - teacher.max) * scale * kLn2 - log_total) -
+                             ((tame ? fmaf(own[k], scale, -o) : (own[k] - base) * scale) * kLn2 - log_sum));
+            if (!ds || i < 0 || !((i >= lo && i < hi) || (rank == 0 && i >= in.tail))) continue;
+            int same = 0;
+#pragma unroll 4
+            for (int j = 0; j < padded; j += 4) {
+                const int4 t = *reinterpret_cast<const int4*>(token + j);
+                same += (t.x == i) + (t.y == i) + (t.z == i) + (t.w == i);
+            }
+            bool first = true;
+            if (same > 1) {
+                q = 0.0f;
+                for (int j = 0; j < K; ++j)
+                    if (token[j] == i) {
+                        first &= j >= k;
+                        q += share(j);
+                    }
+            }
+            if (first) ds[i] = narrow<G>(grad(own[k]) - factor * q);
+        }
+    }
+    if (rank == 0) {
+        loss = warp_sum(loss);
+        if (lane == 0) sh.loss[warp] = loss;
+        __syncthreads();
+        if (warp == 0) {
+            loss = warp_sum(lane < kLongWarps ? sh.loss[lane] : 0.0f);
+            if (lane == 0) a.row_loss[row] = some ? a.temperature * a.temperature * loss : 0.0f;
+        }
+    }
     finish(a);
+}
+
+template <typename L, typename G, int VPT>
+int launch_long(const rl2_distill_args& a, int size, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(static_cast<long long>(a.rows) * size));
+    cfg.blockDim = dim3(kLong);
+    cfg.dynamicSmemBytes = (a.top + 3) / 4 * 4 * 12;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, long_kernel<L, G, VPT>, a, size);
+    if (e != cudaSuccess) {
+        set_error("distillation: %s", cudaGetErrorString(e));
+        return -1;
+    }
+    return launch_status("distillation");
 }
 
 template <typename L, typename G>
@@ -870,56 +703,7 @@ int launch(const rl2_distill_args& a, cudaStream_t stream) {
         row_kernel<L, G, 128><<<std::min(a.rows, 148 * 16), 128, 0, stream>>>(a);
         return launch_status("distillation");
     }
-    // two CTAs an SM; the smallest cluster whose slices leave two chunks of the ring to the next row
-    constexpr int kBudget = 113 * 1024 - static_cast<int>(sizeof(Stream)) - 1024;
-    const int slots = std::min(kMaxSlots, (kBudget - 2 * Entries::bytes(a.top)) / kChunk);
-    auto chunks = [&](int size) {
-        return static_cast<int>(((a.vocab / Slice<L>::kN + size - 1) / size * 16ll + kChunk - 1) / kChunk);
-    };
-    int size = 1;
-    while (size < kMaxCluster && chunks(size) > slots - 2) size *= 2;
-    if (a.vocab <= 8192 || chunks(size) > slots) {
-        // short rows (a CTA each, several an SM), or a row that no cluster holds
-        if (a.vocab <= 8192)
-            row_kernel<L, G, 256><<<std::min(a.rows, 148 * 8), 256, 0, stream>>>(a);
-        else
-            row_kernel<L, G, 512><<<std::min(a.rows, 148 * 4), 512, 0, stream>>>(a);
-        return launch_status("distillation");
-    }
-    const int smem = slots * kChunk + 2 * Entries::bytes(a.top);
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = size;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(size);
-    cfg.blockDim = dim3(kConsumers + 64);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    // clusters resident at once (each walks over its rows, so one that started later would end as much later):
-    // asked once a device, cluster size and type, at the largest shared memory
-    static std::atomic<int> resident[64][4];
-    int device = 0, log_size = 0;
-    while ((1 << log_size) < size) ++log_size;
-    cudaError_t e = cudaGetDevice(&device);
-    int most = device < 64 ? resident[device][log_size].load() : 0;
-    if (e == cudaSuccess && most == 0) {
-        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(stream_kernel<L, G>), cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget);
-        cudaLaunchConfig_t full = cfg;
-        full.dynamicSmemBytes = kBudget;
-        if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&most, stream_kernel<L, G>, &full);
-        most = std::max(most, 1);
-        if (e == cudaSuccess && device < 64) resident[device][log_size].store(most);
-    }
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min(a.rows, most)) * size);
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, stream_kernel<L, G>, a, size, slots);
-    if (e != cudaSuccess) {
-        set_error("distillation: %s", cudaGetErrorString(e));
-        return -1;
-    }
-    return launch_status("distillation");
+    return launch_long<L, G, 0>(a, 1, stream);
 }
 
 template <typename L>
