@@ -927,8 +927,8 @@ int rl2_gated_backward(void* plan, const rl2_gated_backward_args* args, void* st
  *   dlogits_j = loss_weight w_n T (p_j - sum_{k: i_k = j} q_k) * *grad_scale, assigned.
  * teacher_values / teacher_indices [rows][top], 1 <= top <= 1024, any order; an index < 0
  * marks an absent entry, one >= vocab is left out and sets bit 8 of *health; a token may
- * appear more than once (its q add up). row_weight null: 1. A row of weight 0 (its logits
- * are not read), without a teacher entry above -inf or without a logit above -inf has loss 0
+ * appear more than once (its q add up). row_weight null: 1. A row of weight 0
+ * (whatever its logits), without a teacher entry above -inf or without a logit above -inf has loss 0
  * and gradient 0; otherwise NaN and +inf give NaN. A token at -inf has p = 0: a teacher entry
  * on it makes the loss +inf, its gradient stays finite.
  * Types: 0 = fp32, 1 = fp16, 2 = bf16, each matrix its own; rows contiguous, any row stride

@@ -8,7 +8,7 @@
 //
 // A row is read from memory once and stays on the chip between its two passes (running maximum and
 // sum of the softmax; gradient): in L1 behind a warp (up to 1024 tokens) or a CTA (up to
-// 2048), and above that in the registers of a CTA or of a cluster of CTAs (long_kernel). All sums
+// 2048), and above that in shared memory and L2 (long_kernel). All sums
 // are fp32; exponentials are the hardware's exp2 of s log2(e) / T less the same of the maximum, so every
 // value is within a few units in the last place of fp32 times 1 + its argument.
 
@@ -18,6 +18,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace rl2 {
@@ -320,13 +321,20 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const rl2_distill_args a) 
     finish(a);
 }
 
-// ---- long rows: in the registers of a CTA or a cluster ----------------------------------
+// ---- long rows: a CTA each, or with few rows a cluster of CTAs ---------------------------
 //
-// A cluster of CTAs holds a row, VPT 16-byte vectors a thread, all of them loaded at once: one read of the row,
-// no staging, and two (VPT 8) or three CTAs an SM, so that one loads while another computes. The CTAs of a
-// cluster exchange their maxima and sums through shared memory. The teacher's entries are a thread's each: their
-// loads and their softmax go along with the row's. The first entry of each token writes the token's gradient
-// over what the second pass wrote. The few elements of a row outside its 16-byte vectors are one thread's each.
+// 512 threads read the row (of a cluster: each CTA its part) 32 KB at a time, the next 32 KB on their way, and
+// keep the first 64 KB in shared memory; the second pass takes those from there and the rest from L2, the last
+// read first. Two CTAs an SM: one row's reading goes along with the other's writing. What bounds it is DRAM:
+// 1.05 GB in 217 us at 2047 x 128257 bf16 (4.8 TB/s of algorithmic bytes; 84% of the DRAM time was busy when the
+// second pass read forward and kept nothing, because two thirds of the rows had left L2 by then: 246 us).
+// Slower there: rows held in registers by clusters of four CTAs (389 us), rows streamed through a ring in
+// shared memory by bulk copies (308 us), both waiting for one another at each row.
+//
+// The CTAs of a cluster exchange their maxima and sums through shared memory. The teacher's entries are a
+// thread's each: their loads and their softmax go along with the row's. The first entry of each token writes the
+// token's gradient over what the second pass wrote. The few elements of a row outside its 16-byte vectors are
+// one thread's each.
 //
 // The passes use the offset o = max log2(e) / T: p = 2^(s c - o) / sum needs one multiply-add and one exp2 an
 // element, and the rounding of o cancels. Rows where that does not hold (no logit above -1e30, or one above
@@ -335,6 +343,8 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const rl2_distill_args a) 
 constexpr int kLong = 512;  // threads of a CTA
 constexpr int kLongWarps = kLong / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kHeld = 4;                      // vectors a thread has in registers
+constexpr int kKept = 2 * kHeld * kLong;      // vectors kept in shared memory
 constexpr float kTame = 1e30f;
 
 struct Meeting {
@@ -431,52 +441,53 @@ template <typename G, int N>
 __device__ __forceinline__ void store_vector(G* to, const float (&y)[N]) {
     if constexpr (sizeof(G) == 4) {
 #pragma unroll
-        for (int e = 0; e < N; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+        for (int e = 0; e < N; e += 4) __stcs(reinterpret_cast<float4*>(to + e), make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]));
     } else if constexpr (N == 8) {
-        *reinterpret_cast<uint4*>(to) = make_uint4(narrow2<G>(y[0], y[1]), narrow2<G>(y[2], y[3]), narrow2<G>(y[4], y[5]), narrow2<G>(y[6], y[7]));
+        __stcs(reinterpret_cast<uint4*>(to), make_uint4(narrow2<G>(y[0], y[1]), narrow2<G>(y[2], y[3]), narrow2<G>(y[4], y[5]), narrow2<G>(y[6], y[7])));
     } else {
-        *reinterpret_cast<uint2*>(to) = make_uint2(narrow2<G>(y[0], y[1]), narrow2<G>(y[2], y[3]));
+        __stcs(reinterpret_cast<uint2*>(to), make_uint2(narrow2<G>(y[0], y[1]), narrow2<G>(y[2], y[3])));
     }
 }
 
-template <typename L, typename G, int VPT>
-__global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kernel(const rl2_distill_args a, const int size) {
-    extern __shared__ __align__(16) uint8_t raw[];  // the teacher's entries
+template <typename L, typename G>
+__global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a, const int size) {
+    extern __shared__ __align__(16) uint8_t raw[];  // the row's first vectors; the teacher's entries
     __shared__ Meeting sh;
     constexpr int kN = Slice<L>::kN;
+    uint4* kept = reinterpret_cast<uint4*>(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = size > 1 ? ptx::cluster_rank() : 0u;
     const long long row = blockIdx.x / size;
     const Slice<L> in(a, row, rank, size);
     const int K = a.top, padded = (K + 3) / 4 * 4;
-    int* token = reinterpret_cast<int*>(raw);                  // -1: absent
+    int* token = reinterpret_cast<int*>(kept + kKept);         // -1: absent
     float* given = reinterpret_cast<float*>(token + padded);   // the teacher's value
-    float* own = given + padded;                               // the student's
     const float scale = kLog2e / a.temperature;
     const float weight = a.row_weight ? a.row_weight[row] : 1.0f;
     G* ds = a.dlogits ? static_cast<G*>(a.dlogits) + row * a.ld_dlogits : nullptr;
-    if (weight == 0.0f) {
-        const int lo = rank == 0 ? 0 : in.head + in.from * kN, hi = static_cast<int>(rank) == size - 1 ? a.vocab : in.head + (in.from + in.count) * kN;
-        if (ds)
-            for (int j = lo + tid; j < hi; j += kLong) ds[j] = narrow<G>(0.0f);
-        if (tid == 0 && rank == 0) a.row_loss[row] = 0.0f;
-        finish(a);
-        return;
-    }
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) ptx::mbar_init(&sh.met[i], size);
         ptx::fence_barrier_init();
     }
     // this thread's vectors, and its element outside them
-    constexpr int kHeld = VPT > 0 ? VPT : 4;  // VPT 0: four at a time, read again by the second pass
     uint4 x[kHeld];
     const uint4* data = reinterpret_cast<const uint4*>(in.s + in.head) + in.from + tid;
-    auto load = [&](int first) {
+    auto load = [&](uint4 (&to)[kHeld], int first) {
 #pragma unroll
         for (int k = 0; k < kHeld; ++k)
-            x[k] = first + k * kLong + tid < in.count ? __ldg(data + first + k * kLong) : nothing(L(0.0f));
+            to[k] = first + k * kLong + tid < in.count ? __ldg(data + first + k * kLong) : nothing(L(0.0f));
     };
-    load(0);
+    // the second pass's: from shared memory where the first kept them
+    auto load_again = [&](uint4 (&to)[kHeld], int first) {
+        if (first < 0) return;
+        if (first < kKept) {
+#pragma unroll
+            for (int k = 0; k < kHeld; ++k) to[k] = kept[first + k * kLong + tid];
+        } else {
+            load(to, first);
+        }
+    };
+    load(x, 0);
     const bool has_edge = rank == 0 && tid < in.head + (a.vocab - in.tail);
     const int edge_at = tid < in.head ? tid : in.tail + tid - in.head;
     const float edge = has_edge ? to_float(in.s[edge_at]) : -INFINITY;
@@ -484,12 +495,11 @@ __global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kern
     Running teacher{-INFINITY, 0.0f};
     for (int k = tid; k < padded; k += kLong) {
         const long long i = k < K ? teacher_index(a, row, k) : -1;
-        if (i >= a.vocab && a.health) atomicOr(a.health, kHealthIndex);
+        if (i >= a.vocab && weight != 0.0f && a.health) atomicOr(a.health, kHealthIndex);
         const bool here = i >= 0 && i < a.vocab;
         const float v = here ? teacher_value(a, row, k) : -INFINITY;
         token[k] = here ? static_cast<int>(i) : -1;
         given[k] = v;
-        own[k] = here ? to_float(in.s[i]) : 0.0f;
         teacher = merge(teacher, Running{v, v == -INFINITY ? 0.0f : (v == v ? 1.0f : v)}, scale);
     }
     if (warp * 32 < K) {
@@ -498,6 +508,13 @@ __global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kern
             teacher = merge(teacher, Running{__shfl_xor_sync(0xffffffffu, teacher.max, o), __shfl_xor_sync(0xffffffffu, teacher.sum, o)}, scale);
     }
     if (lane == 0) sh.teacher[warp] = teacher;
+    if (weight == 0.0f) {
+        const int lo = rank == 0 ? 0 : in.head + in.from * kN, hi = static_cast<int>(rank) == size - 1 ? a.vocab : in.head + (in.from + in.count) * kN;
+        if (ds)
+            for (int j = lo + tid; j < hi; j += kLong) ds[j] = narrow<G>(0.0f);
+        if (tid == 0 && rank == 0) a.row_loss[row] = 0.0f;
+        return;
+    }
     if (size > 1) ptx::cluster_sync();  // the peers' barriers exist
     const float factor = weight * a.loss_weight * a.temperature * (a.grad_scale ? *a.grad_scale : 1.0f);
     int meeting = 0;
@@ -533,6 +550,9 @@ __global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kern
     float o = fmaxf(edge * scale, -kTame);
     float sum = exp2_fast(fmaf(edge, scale, -o));  // 0 without one (-inf)
     for (int first = 0;;) {
+        const int after = first + kHeld * kLong;
+        uint4 next[kHeld];
+        load(next, after);  // on its way while this is worked on
         float m = -INFINITY;
 #pragma unroll
         for (int k = 0; k < kHeld; ++k) {
@@ -554,10 +574,18 @@ __global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kern
             }
             sum += part;
         }
-        first += kHeld * kLong;
-        if (VPT > 0 || first >= in.count) break;
-        load(first);
+        if (first < kKept) {
+#pragma unroll
+            for (int k = 0; k < kHeld; ++k) kept[first + k * kLong + tid] = x[k];
+        }
+        first = after;
+        if (first >= in.count) break;
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) x[k] = next[k];
     }
+    // the student's logit of this thread's teacher entry
+    const int own_token = tid < K ? token[tid] : -1;
+    const float own = own_token >= 0 ? to_float(in.s[own_token]) : 0.0f;
     const float2 whole = meet(o, sum, false);
     o = whole.x;
     sum = whole.y;
@@ -571,7 +599,7 @@ __global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kern
         auto each = [&](auto&& f) {
             if (has_edge) f(edge);
             for (int first = 0; first < in.count; first += kHeld * kLong) {
-                if (VPT == 0) load(first);
+                load_again(x, first);
 #pragma unroll
                 for (int k = 0; k < kHeld; ++k) {
                     if (first + k * kLong + tid >= in.count) continue;
@@ -602,8 +630,12 @@ __global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kern
         G* out = ds + in.head + (static_cast<long long>(in.from) + tid) * kN;
         const bool vec = reinterpret_cast<uintptr_t>(out) % (sizeof(G) * kN <= 16 ? sizeof(G) * kN : 16) == 0;
         auto write = [&](auto is_plain) {
-            for (int first = 0; first < in.count; first += kHeld * kLong) {
-                if (VPT == 0) load(first);
+            // the last read first: they are the likeliest still in L2
+            const int last = in.count > 0 ? (in.count - 1) / (kHeld * kLong) * (kHeld * kLong) : -1;
+            load_again(x, last);
+            for (int first = last; first >= 0; first -= kHeld * kLong) {
+                uint4 next[kHeld];
+                load_again(next, first - kHeld * kLong);
 #pragma unroll
                 for (int k = 0; k < kHeld; ++k) {
                     float v[kN];
@@ -620,6 +652,8 @@ __global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kern
                         for (int e = 0; e < kN; ++e) to[e] = narrow<G>(v[e]);
                     }
                 }
+#pragma unroll
+                for (int k = 0; k < kHeld; ++k) x[k] = next[k];
             }
         };
         if (tame && some)
@@ -636,10 +670,11 @@ __global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kern
     if (some) {
         for (int k = tid; k < K; k += kLong) {
             const int i = token[k];
+            const float s = k == tid || i < 0 ? own : to_float(in.s[i]);
             float q = share(k);
             if (rank == 0 && q != 0.0f)
                 loss += q * (((given[k] - teacher.max) * scale * kLn2 - log_total) -
-                             ((tame ? fmaf(own[k], scale, -o) : (own[k] - base) * scale) * kLn2 - log_sum));
+                             ((tame ? fmaf(s, scale, -o) : (s - base) * scale) * kLn2 - log_sum));
             if (!ds || i < 0 || !((i >= lo && i < hi) || (rank == 0 && i >= in.tail))) continue;
             int same = 0;
 #pragma unroll 4
@@ -656,7 +691,7 @@ __global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kern
                         q += share(j);
                     }
             }
-            if (first) ds[i] = narrow<G>(grad(own[k]) - factor * q);
+            if (first) ds[i] = narrow<G>(grad(s) - factor * q);
         }
     }
     if (rank == 0) {
@@ -668,11 +703,35 @@ __global__ void __launch_bounds__(kLong, VPT == 8 || VPT == 0 ? 2 : 3) long_kern
             if (lane == 0) a.row_loss[row] = some ? a.temperature * a.temperature * loss : 0.0f;
         }
     }
-    finish(a);
 }
 
-template <typename L, typename G, int VPT>
-int launch_long(const rl2_distill_args& a, int size, cudaStream_t stream) {
+// The total of long rows, in a fixed order, by one CTA of a launch of its own: a ticket and a fence at the end of
+// every CTA of long_kernel cost 14 us at 2047 rows of 128257, this 3 us.
+__global__ void __launch_bounds__(1024) total_kernel(const rl2_distill_args a) {
+    __shared__ float part[32];
+    const int tid = threadIdx.x;
+    float sum = 0.0f;
+    for (int n = tid; n < a.rows; n += 1024) {
+        const float w = a.row_weight ? a.row_weight[n] : 1.0f;
+        if (w != 0.0f) sum += w * a.row_loss[n];
+    }
+    sum = warp_sum(sum);
+    if ((tid & 31) == 0) part[tid >> 5] = sum;
+    __syncthreads();
+    if (tid < 32) {
+        sum = warp_sum(part[tid]);
+        if (tid == 0) *a.loss_out = a.loss_weight * sum;
+    }
+}
+
+template <typename L, typename G>
+int launch_long(const rl2_distill_args& a, cudaStream_t stream) {
+    // few rows: more CTAs a row, while each has four vectors a thread
+    int size = 1;
+    while (size < kMaxCluster && static_cast<long long>(a.rows) * size * 2 <= 148 * 2 &&
+           a.vocab / Slice<L>::kN / (size * 2) >= kHeld * kLong)
+        size *= 2;
+    constexpr int kMost = kKept * 16 + kMaxTop * 8;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -680,15 +739,23 @@ int launch_long(const rl2_distill_args& a, int size, cudaStream_t stream) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(static_cast<long long>(a.rows) * size));
     cfg.blockDim = dim3(kLong);
-    cfg.dynamicSmemBytes = (a.top + 3) / 4 * 4 * 12;
+    cfg.dynamicSmemBytes = kMost - (kMaxTop - (a.top + 3) / 4 * 4) * 8;
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, long_kernel<L, G, VPT>, a, size);
+    static std::atomic<unsigned long long> allowed{0};  // devices (up to 64) whose limit is raised
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && (device > 63 || !(allowed.load() >> device & 1))) {
+        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(long_kernel<L, G>), cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+        if (e == cudaSuccess && device <= 63) allowed.fetch_or(1ull << device);
+    }
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, long_kernel<L, G>, a, size);
     if (e != cudaSuccess) {
         set_error("distillation: %s", cudaGetErrorString(e));
         return -1;
     }
+    if (a.loss_out) total_kernel<<<1, 1024, 0, stream>>>(a);
     return launch_status("distillation");
 }
 
@@ -703,7 +770,7 @@ int launch(const rl2_distill_args& a, cudaStream_t stream) {
         row_kernel<L, G, 128><<<std::min(a.rows, 148 * 16), 128, 0, stream>>>(a);
         return launch_status("distillation");
     }
-    return launch_long<L, G, 0>(a, 1, stream);
+    return launch_long<L, G>(a, stream);
 }
 
 template <typename L>
