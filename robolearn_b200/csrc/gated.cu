@@ -40,16 +40,24 @@ namespace gated {
 
 constexpr int kBM = 128;  // rows of A per CTA (256 per pair)
 constexpr int kBK = 64;   // 128 bytes of 16-bit operands
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr int kBoxBytes = 4096;  // 32 rows x 128 bytes
+constexpr int kMaxEpiWarps = 16;
 constexpr int kMaxSmem = 232448;
 constexpr int kMaxStages = 8;
 
 enum Mode { kForward = 0, kGate = 1, kInput = 2, kWeight = 3 };
 enum Act { kSilu = 0, kGelu = 1, kRelu = 2 };
 
+// Epilogue warps: four per TMEM lane quarter where the epilogue computes (the activation's two special-function
+// steps an element need the warps to hide them), two where it only rounds and stores.
+__host__ __device__ constexpr int epi_warps(int mode) { return mode == kForward || mode == kGate ? 16 : 8; }
+__host__ __device__ constexpr int threads_of(int mode) { return 64 + 32 * epi_warps(mode); }
+// Store boxes: 32 rows of 32 (or 16) hidden units, one a warp (kForward) or two (kGate: dh and dg, du); or of 128
+// bytes, one a warp.
+__host__ __device__ constexpr int box_bytes(int mode) { return mode == kForward || mode == kGate ? 2048 : 4096; }
+__host__ __device__ constexpr int boxes_of(int mode) { return mode == kGate ? 2 : 1; }
+
 struct Params {
+    int a_merged, b_merged;  // M- or N-contiguous operand: one copy brings all its 64-wide chunks
     int kblocks;        // k-blocks of the whole contraction
     int kb_segment;     // kInput: k-blocks of one half (F / 64, rounded up)
     int splits, kb_per_split;
@@ -156,6 +164,17 @@ __device__ __forceinline__ Tile decode(const Params& p, int t) {
 
 // ---- roles --------------------------------------------------------------------
 
+// `chunks` 64-wide pieces (from column n0 on) of 64 k-rows of an M- or N-contiguous operand: one behind the other
+// in shared memory. Merged maps see the row as {64, rows, columns / 64, planes}.
+__device__ __forceinline__ void load_chunks(uint8_t* to, const CUtensorMap* map, uint32_t bar, int n0, int k0, int z, int chunks,
+                                            int merged) {
+    if (merged) {
+        ptx::tma_load_4d_pair(to, map, bar, 0, k0, n0 / 64, z);
+    } else {
+        for (int c = 0; c < chunks; ++c) ptx::tma_load_4d_pair(to + c * (kBK * 128), map, bar, n0 + c * 64, k0, 0, z);
+    }
+}
+
 template <int MODE>
 __device__ __forceinline__ void produce(const Maps& maps, const Params& p, uint8_t* smem, uint32_t stage_bytes,
                                         uint64_t* full, uint64_t* empty, volatile int* abort_flag) {
@@ -187,14 +206,11 @@ __device__ __forceinline__ void produce(const Maps& maps, const Params& p, uint8
                 const int f0 = (kb - seg * p.kb_segment) * kBK;
                 const int n0 = w.n * p.tile_cols + rank * p.bnc;
                 ptx::tma_load_3d_pair(sa, &maps.a, bar, f0, row0, seg);
-                for (int c = 0; c < p.bnc / 64; ++c)
-                    ptx::tma_load_3d_pair(sb + c * (kBK * 128), seg ? &maps.b1 : &maps.b0, bar, n0 + c * 64, f0, 0);
+                load_chunks(sb, seg ? &maps.b1 : &maps.b0, bar, n0, f0, 0, p.bnc / 64, p.b_merged);
             } else {
                 const int n0 = w.n * p.tile_cols + rank * p.bnc;
-                for (int c = 0; c < kBM / 64; ++c)
-                    ptx::tma_load_3d_pair(sa + c * (kBK * 128), &maps.a, bar, row0 + c * 64, kb * kBK, w.z);
-                for (int c = 0; c < p.bnc / 64; ++c)
-                    ptx::tma_load_3d_pair(sb + c * (kBK * 128), &maps.b0, bar, n0 + c * 64, kb * kBK, 0);
+                load_chunks(sa, &maps.a, bar, row0, kb * kBK, w.z, kBM / 64, p.a_merged);
+                load_chunks(sb, &maps.b0, bar, n0, kb * kBK, 0, p.bnc / 64, p.b_merged);
             }
             if (++s == p.stages) {
                 s = 0;
@@ -256,23 +272,23 @@ __device__ __forceinline__ void issue(const Params& p, uint8_t* smem, uint32_t s
     }
 }
 
-// Byte offset of 16-byte chunk j of row r in a store box whose rows are 128 bytes (128-byte
-// swizzle) or 64 bytes (64-byte swizzle): lane = row writes without bank conflicts.
-__device__ __forceinline__ uint32_t box_at(int r, int j, bool wide) {
-    return wide ? static_cast<uint32_t>(r * 128 + ((j ^ (r & 7)) << 4))
-                : static_cast<uint32_t>(r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
+// Byte offset of 16-byte chunk j of row r in a store box whose rows are 128, 64 or 32 bytes (the swizzle of that
+// width): lane = row writes without bank conflicts.
+__device__ __forceinline__ uint32_t box_at(int r, int j, int row_bytes) {
+    const int swizzled = row_bytes == 128 ? j ^ (r & 7) : row_bytes == 64 ? j ^ ((r >> 1) & 3) : j ^ ((r >> 2) & 1);
+    return static_cast<uint32_t>(r * row_bytes + (swizzled << 4));
 }
 
 // Columns [store_cols, out_cols) of this lane's row, if its box (columns col0 .. col0 + box_cols - 1)
 // holds them: the store engine clips a row at 16-byte granules, so it would also write the columns
 // beside a row that ends inside one.
 template <int ELEM>
-__device__ __forceinline__ void store_tail(const Params& p, const uint8_t* box, bool wide, void* base, long long ld,
+__device__ __forceinline__ void store_tail(const Params& p, const uint8_t* box, int row_bytes, void* base, long long ld,
                                            int col0, int row0, int lane) {
     constexpr int kPer = 16 / ELEM;
     if (p.store_cols >= p.out_cols || p.store_cols < col0 || p.store_cols >= col0 + p.box_cols || row0 + lane >= p.out_rows)
         return;
-    const uint4 v = *reinterpret_cast<const uint4*>(box + box_at(lane, (p.store_cols - col0) / kPer, wide));
+    const uint4 v = *reinterpret_cast<const uint4*>(box + box_at(lane, (p.store_cols - col0) / kPer, row_bytes));
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int e = 0; e < kPer - 1; ++e) {
@@ -285,28 +301,29 @@ __device__ __forceinline__ void store_tail(const Params& p, const uint8_t* box, 
     }
 }
 
-// Epilogue warps: warp w reads TMEM lanes 32 (w % 4) .. + 31 (rows of the tile), the two warps of
-// a lane quarter take half of the tile's output columns each.
+// Epilogue warps: warp w reads TMEM lanes 32 (w % 4) .. + 31 (rows of the tile), the warps of a lane quarter
+// share the tile's output columns.
 template <int MODE, bool BF16, int ACT, bool OUT32>
 __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t* boxes, uint64_t* in_full,
                                       uint64_t* acc_full, uint64_t* acc_empty, uint32_t tmem,
                                       volatile int* abort_flag) {
+    constexpr bool kGated = MODE == kForward || MODE == kGate;
+    constexpr int kSlots = epi_warps(MODE) / 4;  // warps of a lane quarter
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int q = warp & 3, half = (warp - 2) >> 2;
+    const int q = warp & 3, slot = (warp - 2) >> 2;
     const int rank = static_cast<int>(blockIdx.x & 1u);
-    uint8_t* box = boxes + (warp - 2) * 2 * kBoxBytes;  // two boxes per warp
-    uint8_t* box1 = box + kBoxBytes;
+    uint8_t* box = boxes + (warp - 2) * boxes_of(MODE) * box_bytes(MODE);
+    uint8_t* box1 = box + box_bytes(MODE);
     uint64_t* in_bar = in_full + (warp - 2);
     const uint32_t n = 2u * p.bnc;
-    const bool wide = OUT32 || p.box_cols == 64;
+    const int row_bytes = OUT32 ? 128 : p.box_cols * 2;
     int i = 0;
-    uint32_t used = 0;  // boxes handed to the store engine (kForward, kInput, kWeight)
     for (int t = blockIdx.x >> 1; t < p.tiles_total; t += gridDim.x >> 1, ++i) {
         const Tile w = decode(p, t);
         const int buf = i & 1;
         const int row0 = w.m * 2 * kBM + rank * kBM + q * 32;
-        const int mine = MODE == kForward || MODE == kGate ? p.bnc / 2 : p.bnc;  // this warp's output columns
-        const int col0 = w.n * p.tile_cols + half * mine;
+        const int mine = kGated ? p.bnc / kSlots : 2 * p.bnc / kSlots;  // this warp's output columns
+        const int col0 = w.n * p.tile_cols + slot * mine;
         if (MODE == kGate) {  // this tile's dh, while the products run
             if (lane == 0) {
                 ptx::bulk_wait_read0();
@@ -324,22 +341,20 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
         }
         ptx::tc_fence_after();
         const uint32_t base = tmem + static_cast<uint32_t>(buf) * n + (static_cast<uint32_t>(q * 32) << 16);
-        if (MODE == kForward || MODE == kGate) {
-            uint8_t* out0 = box;
+        if (kGated) {
             if (MODE == kForward) {
-                out0 = used & 1 ? box1 : box;
-                if (lane == 0) ptx::bulk_wait_read1();
+                if (lane == 0) ptx::bulk_wait_read0();
                 __syncwarp();
             }
             for (int c = 0; c < mine; c += 16) {
                 uint32_t gr[16], ur[16];
-                ptx::tmem_ld16_issue(base + half * mine + c, gr);
-                ptx::tmem_ld16_issue(base + p.bnc + half * mine + c, ur);
+                ptx::tmem_ld16_issue(base + slot * mine + c, gr);
+                ptx::tmem_ld16_issue(base + p.bnc + slot * mine + c, ur);
                 ptx::tmem_ld_wait(gr);
                 ptx::tmem_ld_wait(ur);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const uint32_t at = box_at(lane, c / 8 + e, wide);
+                    const uint32_t at = box_at(lane, c / 8 + e, row_bytes);
                     uint32_t o0[4], o1[4];
                     uint4 in4 = make_uint4(0, 0, 0, 0);
                     if (MODE == kGate) in4 = *reinterpret_cast<const uint4*>(box + at);
@@ -359,60 +374,53 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
                             o1[k] = pack2<BF16>(dh.x * a0, dh.y * a1);
                         }
                     }
-                    *reinterpret_cast<uint4*>(out0 + at) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+                    *reinterpret_cast<uint4*>(box + at) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
                     if (MODE == kGate) *reinterpret_cast<uint4*>(box1 + at) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
                 }
             }
             ptx::tc_fence_before();
-            if (MODE == kForward) store_tail<2>(p, out0, wide, p.out[0], p.ld_out[0], col0, row0, lane);
+            if (MODE == kForward) store_tail<2>(p, box, row_bytes, p.out[0], p.ld_out[0], col0, row0, lane);
             ptx::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
                 ptx::mbar_arrive_cluster(ptx::cluster_addr(&acc_empty[buf], 0));
                 if (col0 < p.store_cols && row0 < p.out_rows) {  // the store engine clips a box, it needs one to start inside
-                    ptx::tma_store_3d(&maps.d0, out0, col0, row0, 0);
+                    ptx::tma_store_3d(&maps.d0, box, col0, row0, 0);
                     if (MODE == kGate) ptx::tma_store_3d(&maps.d0, box1, col0, row0, 1);
                 }
                 ptx::bulk_commit();
             }
-            ++used;
         } else {
             const int z = MODE == kWeight ? (p.splits > 1 ? w.split * 2 + w.z : 0) : 0;
             const CUtensorMap* dst = MODE == kWeight && p.splits == 1 && w.z ? &maps.d1 : &maps.d0;
             for (int c = 0; c < mine; c += p.box_cols) {
-                uint8_t* out = used & 1 ? box1 : box;
-                if (lane == 0) ptx::bulk_wait_read1();
+                if (lane == 0) ptx::bulk_wait_read0();
                 __syncwarp();
-                for (int e = 0; e < p.box_cols; e += 16) {
-                    uint32_t r[16];
-                    ptx::tmem_ld16_issue(base + half * mine + c + e, r);
-                    ptx::tmem_ld_wait(r);
+                for (int e = 0; e < p.box_cols; e += 32) {
+                    float r[32];
+                    ptx::tmem_ld32(base + slot * mine + c + e, r);
                     if (OUT32) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            *reinterpret_cast<uint4*>(out + box_at(lane, e / 4 + k, true)) =
-                                make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+                        for (int k = 0; k < 8; ++k)
+                            *reinterpret_cast<float4*>(box + box_at(lane, e / 4 + k, 128)) =
+                                make_float4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
                     } else {
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            uint32_t o[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                o[j] = pack2<BF16>(__uint_as_float(r[8 * k + 2 * j]), __uint_as_float(r[8 * k + 2 * j + 1]));
-                            *reinterpret_cast<uint4*>(out + box_at(lane, e / 8 + k, wide)) = make_uint4(o[0], o[1], o[2], o[3]);
-                        }
+                        for (int k = 0; k < 4; ++k)
+                            *reinterpret_cast<uint4*>(box + box_at(lane, e / 8 + k, row_bytes)) =
+                                make_uint4(pack2<BF16>(r[8 * k], r[8 * k + 1]), pack2<BF16>(r[8 * k + 2], r[8 * k + 3]),
+                                           pack2<BF16>(r[8 * k + 4], r[8 * k + 5]), pack2<BF16>(r[8 * k + 6], r[8 * k + 7]));
                     }
                 }
                 if (c + p.box_cols >= mine) ptx::tc_fence_before();
-                store_tail<OUT32 ? 4 : 2>(p, out, wide, p.out[w.z], p.ld_out[w.z], col0 + c, row0, lane);
+                store_tail<OUT32 ? 4 : 2>(p, box, row_bytes, w.z ? p.out[1] : p.out[0], w.z ? p.ld_out[1] : p.ld_out[0], col0 + c, row0, lane);
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
                     if (c + p.box_cols >= mine) ptx::mbar_arrive_cluster(ptx::cluster_addr(&acc_empty[buf], 0));
-                    if (col0 + c < p.store_cols && row0 < p.out_rows) ptx::tma_store_3d(dst, out, col0 + c, row0, z);
+                    if (col0 + c < p.store_cols && row0 < p.out_rows) ptx::tma_store_3d(dst, box, col0 + c, row0, z);
                     ptx::bulk_commit();
                 }
-                ++used;
             }
         }
     }
@@ -420,10 +428,10 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
 }
 
 template <int MODE, bool BF16, int ACT, bool OUT32>
-__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+__global__ void __launch_bounds__(threads_of(MODE), 1) __cluster_dims__(2, 1, 1)
     product_kernel(const __grid_constant__ Maps maps, const Params p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], mma_done, in_full[kEpiWarps];
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], mma_done, in_full[kMaxEpiWarps];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -440,9 +448,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         }
         for (int b = 0; b < 2; ++b) {
             ptx::mbar_init(&acc_full[b], 1);
-            ptx::mbar_init(&acc_empty[b], 2 * kEpiWarps);
+            ptx::mbar_init(&acc_empty[b], 2 * epi_warps(MODE));
         }
-        for (int e = 0; e < kEpiWarps; ++e) ptx::mbar_init(&in_full[e], 1);
+        for (int e = 0; e < kMaxEpiWarps; ++e) ptx::mbar_init(&in_full[e], 1);
         ptx::mbar_init(&mma_done, 1);
         abort_flag = 0;
         ptx::fence_barrier_init();
@@ -554,12 +562,33 @@ bool make_map(CUtensorMap* map, const char* what, CUtensorMapDataType type, cons
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * elem), static_cast<cuuint64_t>(depth_stride * elem)};
     const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer), 1};
     const cuuint32_t ones[3] = {1, 1, 1};
-    const CUtensorMapSwizzle swizzle = box_inner * elem == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    const CUtensorMapSwizzle swizzle = box_inner * elem == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                       : box_inner * elem == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                                : CU_TENSOR_MAP_SWIZZLE_32B;
     const CUresult r = encoder()(map, type, 3, const_cast<void*>(base), dims, strides, box, ones,
                                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r == CUDA_SUCCESS) return true;
     set_error("gated MLP: tensor map of %s failed (%d) for %lld x %lld", what, static_cast<int>(r), inner, outer);
+    return false;
+}
+
+// An M- or N-contiguous 16-bit operand (`cols` contiguous, contraction over `rows`) for load_chunks: with whole
+// 64-wide chunks the row is seen as {64, rows, cols / 64, planes} and one box takes `chunks` of them; otherwise
+// (the last chunk would read past the last row) as it is, a box a chunk.
+bool make_chunk_map(CUtensorMap* map, int* merged, const char* what, CUtensorMapDataType type, const void* base, long long cols,
+                    long long rows, long long planes, long long ld, int chunks) {
+    *merged = cols % 64 == 0;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(*merged ? 64 : cols), static_cast<cuuint64_t>(rows),
+                                static_cast<cuuint64_t>(*merged ? cols / 64 : 1), static_cast<cuuint64_t>(planes)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(ld * 2), *merged ? 128u : static_cast<cuuint64_t>(ld * 2),
+                                   static_cast<cuuint64_t>(ld * rows * 2)};
+    const cuuint32_t box[4] = {64, kBK, static_cast<cuuint32_t>(*merged ? chunks : 1), 1};
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    const CUresult r = encoder()(map, type, 4, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return true;
+    set_error("gated MLP: tensor map of %s failed (%d) for %lld x %lld", what, static_cast<int>(r), cols, rows);
     return false;
 }
 
@@ -595,7 +624,7 @@ constexpr int kStaticSmem = 1024;  // room left for the barriers, the TMEM slot 
 
 int launch(const Plan* plan, int mode, bool out32, Params& p, const Maps& maps, cudaStream_t stream) {
     const int stage = (kBM + p.bnc) * 128;
-    const int fixed = 1024 + kEpiWarps * 2 * kBoxBytes;
+    const int fixed = 1024 + epi_warps(mode) * boxes_of(mode) * box_bytes(mode);
     p.stages = std::min(kMaxStages, (kMaxSmem - kStaticSmem - fixed) / stage);
     const long long total = static_cast<long long>(p.tiles_n) * p.tiles_m * p.tiles_z * p.splits;
     if (total > 0x3FFFFFFF) {
@@ -604,7 +633,7 @@ int launch(const Plan* plan, int mode, bool out32, Params& p, const Maps& maps, 
     }
     p.tiles_total = static_cast<int>(total);
     const int pairs = static_cast<int>(std::min<long long>(total, plan->pairs));
-    kernel_of(plan, mode, out32)<<<2 * pairs, kThreads, p.stages * stage + fixed, stream>>>(maps, p);
+    kernel_of(plan, mode, out32)<<<2 * pairs, threads_of(mode), p.stages * stage + fixed, stream>>>(maps, p);
     return launch_status("gated MLP product");
 }
 
@@ -666,7 +695,7 @@ int project(const Plan* plan, int rows, const void* x, long long ldx, const void
     p.tiles_n = (F + p.bnc - 1) / p.bnc;
     p.tiles_z = p.splits = 1;
     p.kblocks = p.kb_per_split = (K + kBK - 1) / kBK;
-    p.box_cols = p.bnc / 2;
+    p.box_cols = p.bnc / (epi_warps(mode) / 4);
     p.out_rows = rows;
     p.out_cols = F;
     p.store_cols = grad_out ? F : F / 8 * 8;  // the workspace's rows are padded: nothing beside them
@@ -707,8 +736,8 @@ int input_gradient(const Plan* plan, const rl2_gated_backward_args* g, cudaStrea
     p.health = g->health;
     Maps maps;
     if (!make_map(&maps.a, "hidden gradients", type, g->workspace, F, rows, 2, ldw, ldw * rows, kBK, kBM) ||
-        !make_map(&maps.b0, "gate weight", type, g->gate_weight, K, F, 1, g->ld_gate, g->ld_gate * F, 64, kBK) ||
-        !make_map(&maps.b1, "up weight", type, g->up_weight, K, F, 1, g->ld_up, g->ld_up * F, 64, kBK) ||
+        !make_chunk_map(&maps.b0, &p.b_merged, "gate weight", type, g->gate_weight, K, F, 1, g->ld_gate, p.bnc / 64) ||
+        !make_chunk_map(&maps.b1, &p.b_merged, "up weight", type, g->up_weight, K, F, 1, g->ld_up, p.bnc / 64) ||
         !make_map(&maps.d0, "input gradient", type, g->grad_x, stored(K, 8), rows, 1, g->ld_grad_x, g->ld_grad_x * rows, 64, 32))
         return -1;
     maps.d1 = maps.in = maps.d0;
@@ -751,8 +780,8 @@ int weight_gradients(const Plan* plan, const rl2_gated_backward_args* g, cudaStr
     p.ld_out[0] = g->ld_grad_gate;
     p.ld_out[1] = g->ld_grad_up;
     Maps maps;
-    if (!make_map(&maps.a, "hidden gradients", type, g->workspace, F, rows, 2, ldw, ldw * rows, 64, kBK) ||
-        !make_map(&maps.b0, "x", type, g->x, K, rows, 1, g->ldx, g->ldx * rows, 64, kBK))
+    if (!make_chunk_map(&maps.a, &p.a_merged, "hidden gradients", type, g->workspace, F, rows, 2, ldw, kBM / 64) ||
+        !make_chunk_map(&maps.b0, &p.b_merged, "x", type, g->x, K, rows, 1, g->ldx, p.bnc / 64))
         return -1;
     maps.b1 = maps.b0;
     if (p.splits > 1) {
@@ -813,7 +842,7 @@ extern "C" void* rl2_gated_create(const rl2_gated_desc* d) {
         attr[0].val.clusterDim.x = 2;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.gridDim = dim3(static_cast<unsigned>(2 * std::max(1, sms / 2)));
-        cfg.blockDim = dim3(kThreads);
+        cfg.blockDim = dim3(threads_of(std::min(i, 3)));
         cfg.dynamicSmemBytes = kMaxSmem - kStaticSmem;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
