@@ -22,6 +22,10 @@
 //                     (K-major), B = [Wg ; Wu] read N-contiguous, no transposed copies.
 //   kWeight           contraction over the M rows: A = dg or du read M-contiguous, B = x read
 //                     N-contiguous; split over rows when the tiles do not fill the GPU.
+// dg and du live in the workspace in blocks of 128 rows by 64 hidden units, 16 KB each in one piece, because the
+// last two products read them so: as rows of the matrix, a block is 128 pieces of 128 bytes in as many DRAM pages,
+// and dx at 8192 x 512 x 2048 took 0.53 us a k-block for the 0.38 that the tensor cores take. Rows and hidden units
+// past the matrix are zeros there (the projections of zero-filled operands).
 // Warp roles as in the dense products: TMA producer, MMA issuer, eight epilogue warps on a
 // double-buffered accumulator. Outputs leave through shared-memory boxes and TMA stores, which
 // clip at the output's extents. Every wait is bounded by wall-clock time.
@@ -32,7 +36,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
-#include <cstring>
+#include <initializer_list>
 #include <new>
 
 namespace rl2 {
@@ -57,7 +61,8 @@ __host__ __device__ constexpr int box_bytes(int mode) { return mode == kForward 
 __host__ __device__ constexpr int boxes_of(int mode) { return mode == kGate ? 2 : 1; }
 
 struct Params {
-    int a_merged, b_merged;  // M- or N-contiguous operand: one copy brings all its 64-wide chunks
+    int b_merged;       // N-contiguous operand: one copy brings all its 64-wide chunks
+    int row_blocks;     // 128-row blocks of dg (of du) in the workspace
     int kblocks;        // k-blocks of the whole contraction
     int kb_segment;     // kInput: k-blocks of one half (F / 64, rounded up)
     int splits, kb_per_split;
@@ -164,14 +169,14 @@ __device__ __forceinline__ Tile decode(const Params& p, int t) {
 
 // ---- roles --------------------------------------------------------------------
 
-// `chunks` 64-wide pieces (from column n0 on) of 64 k-rows of an M- or N-contiguous operand: one behind the other
-// in shared memory. Merged maps see the row as {64, rows, columns / 64, planes}.
-__device__ __forceinline__ void load_chunks(uint8_t* to, const CUtensorMap* map, uint32_t bar, int n0, int k0, int z, int chunks,
+// `chunks` 64-wide pieces (from column n0 on) of 64 k-rows of an N-contiguous operand: one behind the other in
+// shared memory. Merged maps see the matrix as {64, rows, columns / 64}.
+__device__ __forceinline__ void load_chunks(uint8_t* to, const CUtensorMap* map, uint32_t bar, int n0, int k0, int chunks,
                                             int merged) {
     if (merged) {
-        ptx::tma_load_4d_pair(to, map, bar, 0, k0, n0 / 64, z);
+        ptx::tma_load_3d_pair(to, map, bar, 0, k0, n0 / 64);
     } else {
-        for (int c = 0; c < chunks; ++c) ptx::tma_load_4d_pair(to + c * (kBK * 128), map, bar, n0 + c * 64, k0, 0, z);
+        for (int c = 0; c < chunks; ++c) ptx::tma_load_3d_pair(to + c * (kBK * 128), map, bar, n0 + c * 64, k0, 0);
     }
 }
 
@@ -205,12 +210,12 @@ __device__ __forceinline__ void produce(const Maps& maps, const Params& p, uint8
                 const int seg = kb >= p.kb_segment ? 1 : 0;
                 const int f0 = (kb - seg * p.kb_segment) * kBK;
                 const int n0 = w.n * p.tile_cols + rank * p.bnc;
-                ptx::tma_load_3d_pair(sa, &maps.a, bar, f0, row0, seg);
-                load_chunks(sb, seg ? &maps.b1 : &maps.b0, bar, n0, f0, 0, p.bnc / 64, p.b_merged);
+                ptx::tma_load_4d_pair(sa, &maps.a, bar, 0, 0, f0 / 64, row0 / kBM + seg * p.row_blocks);
+                load_chunks(sb, seg ? &maps.b1 : &maps.b0, bar, n0, f0, p.bnc / 64, p.b_merged);
             } else {
                 const int n0 = w.n * p.tile_cols + rank * p.bnc;
-                load_chunks(sa, &maps.a, bar, row0, kb * kBK, w.z, kBM / 64, p.a_merged);
-                load_chunks(sb, &maps.b0, bar, n0, kb * kBK, 0, p.bnc / 64, p.b_merged);
+                ptx::tma_load_4d_pair(sa, &maps.a, bar, 0, kb % 2 * kBK, row0 / 64, kb / 2 + w.z * p.row_blocks);
+                load_chunks(sb, &maps.b0, bar, n0, kb * kBK, p.bnc / 64, p.b_merged);
             }
             if (++s == p.stages) {
                 s = 0;
@@ -384,9 +389,11 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
             __syncwarp();
             if (lane == 0) {
                 ptx::mbar_arrive_cluster(ptx::cluster_addr(&acc_empty[buf], 0));
-                if (col0 < p.store_cols && row0 < p.out_rows) {  // the store engine clips a box, it needs one to start inside
+                if (MODE == kGate) {
+                    ptx::tma_store_4d(&maps.d0, box, col0 % 64, row0 % kBM, col0 / 64, row0 / kBM);
+                    ptx::tma_store_4d(&maps.d0, box1, col0 % 64, row0 % kBM, col0 / 64, row0 / kBM + p.row_blocks);
+                } else if (col0 < p.store_cols && row0 < p.out_rows) {  // the store engine clips a box, it needs one to start inside
                     ptx::tma_store_3d(&maps.d0, box, col0, row0, 0);
-                    if (MODE == kGate) ptx::tma_store_3d(&maps.d0, box1, col0, row0, 1);
                 }
                 ptx::bulk_commit();
             }
@@ -553,43 +560,50 @@ struct Plan {
     int device, pairs;  // CTA pairs resident at once
 };
 
+// Tensor map of `rank` dimensions (extents and box in elements, strides in bytes from the second dimension on), the
+// box's rows swizzled over their width.
+bool encode(CUtensorMap* map, const char* what, CUtensorMapDataType type, const void* base, int rank,
+            std::initializer_list<long long> extents, std::initializer_list<long long> strides, std::initializer_list<int> box) {
+    cuuint64_t dims[4], steps[3];
+    cuuint32_t boxes[4];
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    std::copy(extents.begin(), extents.end(), dims);
+    std::copy(strides.begin(), strides.end(), steps);
+    std::copy(box.begin(), box.end(), boxes);
+    const int row_bytes = *box.begin() * (type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2);
+    const CUtensorMapSwizzle swizzle = row_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                       : row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                         : CU_TENSOR_MAP_SWIZZLE_32B;
+    const CUresult r = encoder()(map, type, rank, const_cast<void*>(base), dims, steps, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return true;
+    set_error("gated MLP: tensor map of %s failed (%d) for %lld x %lld", what, static_cast<int>(r), *extents.begin(),
+              *(extents.begin() + 1));
+    return false;
+}
+
 // {inner, outer, depth} elements at base; boxes of box_inner x box_outer
 bool make_map(CUtensorMap* map, const char* what, CUtensorMapDataType type, const void* base, long long inner,
               long long outer, long long depth, long long ld, long long depth_stride, int box_inner, int box_outer) {
     const int elem = type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
-    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer),
-                                static_cast<cuuint64_t>(depth)};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * elem), static_cast<cuuint64_t>(depth_stride * elem)};
-    const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer), 1};
-    const cuuint32_t ones[3] = {1, 1, 1};
-    const CUtensorMapSwizzle swizzle = box_inner * elem == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                                       : box_inner * elem == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                                : CU_TENSOR_MAP_SWIZZLE_32B;
-    const CUresult r = encoder()(map, type, 3, const_cast<void*>(base), dims, strides, box, ones,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r == CUDA_SUCCESS) return true;
-    set_error("gated MLP: tensor map of %s failed (%d) for %lld x %lld", what, static_cast<int>(r), inner, outer);
-    return false;
+    return encode(map, what, type, base, 3, {inner, outer, depth}, {ld * elem, depth_stride * elem}, {box_inner, box_outer, 1});
 }
 
-// An M- or N-contiguous 16-bit operand (`cols` contiguous, contraction over `rows`) for load_chunks: with whole
-// 64-wide chunks the row is seen as {64, rows, cols / 64, planes} and one box takes `chunks` of them; otherwise
-// (the last chunk would read past the last row) as it is, a box a chunk.
+// An N-contiguous 16-bit operand (`cols` contiguous, contraction over `rows`) for load_chunks: with whole 64-wide
+// chunks the matrix is seen as {64, rows, cols / 64} and one box takes `chunks` of them; otherwise (the last chunk
+// would read past the last row) as it is, a box a chunk.
 bool make_chunk_map(CUtensorMap* map, int* merged, const char* what, CUtensorMapDataType type, const void* base, long long cols,
-                    long long rows, long long planes, long long ld, int chunks) {
+                    long long rows, long long ld, int chunks) {
     *merged = cols % 64 == 0;
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(*merged ? 64 : cols), static_cast<cuuint64_t>(rows),
-                                static_cast<cuuint64_t>(*merged ? cols / 64 : 1), static_cast<cuuint64_t>(planes)};
-    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(ld * 2), *merged ? 128u : static_cast<cuuint64_t>(ld * 2),
-                                   static_cast<cuuint64_t>(ld * rows * 2)};
-    const cuuint32_t box[4] = {64, kBK, static_cast<cuuint32_t>(*merged ? chunks : 1), 1};
-    const cuuint32_t ones[4] = {1, 1, 1, 1};
-    const CUresult r = encoder()(map, type, 4, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r == CUDA_SUCCESS) return true;
-    set_error("gated MLP: tensor map of %s failed (%d) for %lld x %lld", what, static_cast<int>(r), cols, rows);
-    return false;
+    return encode(map, what, type, base, 3, {*merged ? 64 : cols, rows, *merged ? cols / 64 : 1},
+                  {ld * 2, *merged ? 128 : ld * rows * 2}, {64, kBK, *merged ? chunks : 1});
+}
+
+// The workspace's blocks of dg and du: {64 hidden units, 128 rows, blocks of hidden units, blocks of rows of both}.
+bool make_block_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long hidden_blocks, long long row_blocks,
+                    int box_units, int box_rows, int box_blocks) {
+    return encode(map, "hidden gradients", type, base, 4, {64, kBM, hidden_blocks, 2 * row_blocks},
+                  {128, kBM * 128, hidden_blocks * kBM * 128}, {box_units, box_rows, box_blocks, 1});
 }
 
 bool matrix_ok(const char* what, const void* base, long long ld, long long cols, int elem) {
@@ -642,14 +656,17 @@ int width_for(const Plan* plan, long long row_tiles, long long cols, int per_row
     return row_tiles * ((cols + 128 * per_row - 1) / (128 * per_row)) < plan->pairs ? 64 : 128;
 }
 
-// Splits of the weight gradients' contraction over `rows`: one tile per pair where the splits stay
-// at least 16 k-blocks long; and chains of at most 8192 rows, because the tensor cores' fp32
-// accumulation error grows with the chain (about 7e-9 per product, measured).
+// Splits of the weight gradients' contraction over `rows`: one tile per pair where the splits stay at least 16
+// k-blocks long; and chains that keep the tensor cores' fp32 accumulation error (about 7e-9 a product, measured)
+// below a quarter of the operands' rounding: 16384 rows for fp16, 65536 for bf16.
 int splits_for(const Plan* plan, int rows) {
-    const long long tiles = 2LL * ((plan->hidden + 255) / 256) * ((plan->features + 255) / 256);
+    const long long row_tiles = 2LL * ((plan->hidden + 255) / 256);
+    const int width = 2 * width_for(plan, row_tiles, plan->features, 2);
+    const long long tiles = row_tiles * ((plan->features + width - 1) / width);
     const int kblocks = (rows + kBK - 1) / kBK;
     const long long fill = std::max<long long>(1, std::min<long long>(plan->pairs / tiles, kblocks / 16));
-    return static_cast<int>(std::max<long long>(fill, (kblocks + 127) / 128));
+    const int chain = plan->bf16 ? 1024 : 256;
+    return static_cast<int>(std::max<long long>(fill, (kblocks + chain - 1) / chain));
 }
 
 long long pad(long long cols, long long to) { return (cols + to - 1) / to * to; }
@@ -657,8 +674,17 @@ long long pad(long long cols, long long to) { return (cols + to - 1) / to * to; 
 // inner extent of an output's tensor map: whole granules (rows shorter than one are not stored by it)
 long long stored(long long cols, long long granule) { return std::max(granule, cols / granule * granule); }
 
+// blocks of dg (of du) for so many rows: of 128 rows (whole pair tiles), and of 64 hidden units (whole tiles)
+int row_blocks(int rows) { return (rows + 2 * kBM - 1) / (2 * kBM) * 2; }
+int hidden_blocks(const Plan* plan, int rows) {
+    const int width = width_for(plan, row_blocks(rows) / 2, plan->hidden, 1);
+    return (plan->hidden + width - 1) / width * (width / 64);
+}
+
 // workspace: dg and du, then (when split) the fp32 partial weight gradients
-long long gate_bytes(const Plan* plan) { return pad(4LL * plan->rows * pad(plan->hidden, 8), 256); }
+long long gate_bytes(const Plan* plan) {
+    return 2LL * row_blocks(plan->rows) * ((plan->hidden + 127) / 128 * 2) * kBM * 128;
+}
 long long part_bytes(const Plan* plan) {  // splits grow with the rows
     const long long s = splits_for(plan, plan->rows);
     return s > 1 ? s * 2 * plan->hidden * pad(plan->features, 4) * 4 : 0;
@@ -683,8 +709,8 @@ bool ready(const Plan* plan, int rows) {
 
 // The two projections: forward (out = h) or backward (grad_out in, dg and du out).
 int project(const Plan* plan, int rows, const void* x, long long ldx, const void* wg, long long ldg, const void* wu,
-            long long ldu, const void* grad_out, long long ld_grad, void* out, long long ld_out, long long out_plane,
-            int* health, cudaStream_t stream) {
+            long long ldu, const void* grad_out, long long ld_grad, void* out, long long ld_out, int* health,
+            cudaStream_t stream) {
     const int K = plan->features, F = plan->hidden;
     const CUtensorMapDataType type = plan->bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const int mode = grad_out ? kGate : kForward;
@@ -698,16 +724,17 @@ int project(const Plan* plan, int rows, const void* x, long long ldx, const void
     p.box_cols = p.bnc / (epi_warps(mode) / 4);
     p.out_rows = rows;
     p.out_cols = F;
-    p.store_cols = grad_out ? F : F / 8 * 8;  // the workspace's rows are padded: nothing beside them
+    p.store_cols = F / 8 * 8;
+    p.row_blocks = row_blocks(rows);
     p.out[0] = out;
     p.ld_out[0] = ld_out;
     p.health = health;
     Maps maps;
-    const long long planes = grad_out ? 2 : 1;
     if (!make_map(&maps.a, "x", type, x, K, rows, 1, ldx, ldx * rows, kBK, kBM) ||
         !make_map(&maps.b0, "gate weight", type, wg, K, F, 1, ldg, ldg * F, kBK, p.bnc) ||
         !make_map(&maps.b1, "up weight", type, wu, K, F, 1, ldu, ldu * F, kBK, p.bnc) ||
-        !make_map(&maps.d0, "output", type, out, grad_out ? F : stored(F, 8), rows, planes, ld_out, out_plane, p.box_cols, 32))
+        !(grad_out ? make_block_map(&maps.d0, type, out, hidden_blocks(plan, rows), p.row_blocks, p.box_cols, 32, 1)
+                   : make_map(&maps.d0, "output", type, out, stored(F, 8), rows, 1, ld_out, ld_out * rows, p.box_cols, 32)))
         return -1;
     maps.d1 = maps.in = maps.d0;
     if (grad_out && !make_map(&maps.in, "output gradient", type, grad_out, F, rows, 1, ld_grad, ld_grad * rows, p.box_cols, 32))
@@ -718,8 +745,8 @@ int project(const Plan* plan, int rows, const void* x, long long ldx, const void
 int input_gradient(const Plan* plan, const rl2_gated_backward_args* g, cudaStream_t stream) {
     const int K = plan->features, F = plan->hidden, rows = g->rows;
     const CUtensorMapDataType type = plan->bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const long long ldw = pad(F, 8);
     Params p{};
+    p.row_blocks = row_blocks(rows);
     p.tiles_m = (rows + 2 * kBM - 1) / (2 * kBM);
     p.bnc = width_for(plan, p.tiles_m, K, 2);
     p.tile_cols = 2 * p.bnc;
@@ -735,9 +762,9 @@ int input_gradient(const Plan* plan, const rl2_gated_backward_args* g, cudaStrea
     p.ld_out[0] = g->ld_grad_x;
     p.health = g->health;
     Maps maps;
-    if (!make_map(&maps.a, "hidden gradients", type, g->workspace, F, rows, 2, ldw, ldw * rows, kBK, kBM) ||
-        !make_chunk_map(&maps.b0, &p.b_merged, "gate weight", type, g->gate_weight, K, F, 1, g->ld_gate, p.bnc / 64) ||
-        !make_chunk_map(&maps.b1, &p.b_merged, "up weight", type, g->up_weight, K, F, 1, g->ld_up, p.bnc / 64) ||
+    if (!make_block_map(&maps.a, type, g->workspace, hidden_blocks(plan, rows), p.row_blocks, 64, kBM, 1) ||
+        !make_chunk_map(&maps.b0, &p.b_merged, "gate weight", type, g->gate_weight, K, F, g->ld_gate, p.bnc / 64) ||
+        !make_chunk_map(&maps.b1, &p.b_merged, "up weight", type, g->up_weight, K, F, g->ld_up, p.bnc / 64) ||
         !make_map(&maps.d0, "input gradient", type, g->grad_x, stored(K, 8), rows, 1, g->ld_grad_x, g->ld_grad_x * rows, 64, 32))
         return -1;
     maps.d1 = maps.in = maps.d0;
@@ -755,15 +782,16 @@ void reduce(const float* part, int splits, int rows, int cols, int ld, const rl2
 int weight_gradients(const Plan* plan, const rl2_gated_backward_args* g, cudaStream_t stream) {
     const int K = plan->features, F = plan->hidden, rows = g->rows;
     const CUtensorMapDataType type = plan->bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const long long ldw = pad(F, 8), ldp = pad(K, 4);
+    const long long ldp = pad(K, 4);
     Params p{};
+    p.row_blocks = row_blocks(rows);
     p.tiles_m = (F + 2 * kBM - 1) / (2 * kBM);
     p.tiles_z = 2;
     p.kblocks = (rows + kBK - 1) / kBK;
     p.splits = splits_for(plan, rows);
     p.kb_per_split = (p.kblocks + p.splits - 1) / p.splits;
     p.splits = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;  // every split non-empty
-    p.bnc = width_for(plan, 2LL * p.tiles_m * p.splits, K, 2);
+    p.bnc = width_for(plan, 2LL * p.tiles_m, K, 2);
     p.tile_cols = 2 * p.bnc;
     p.tiles_n = (K + p.tile_cols - 1) / p.tile_cols;
     p.out_rows = F;
@@ -780,8 +808,8 @@ int weight_gradients(const Plan* plan, const rl2_gated_backward_args* g, cudaStr
     p.ld_out[0] = g->ld_grad_gate;
     p.ld_out[1] = g->ld_grad_up;
     Maps maps;
-    if (!make_chunk_map(&maps.a, &p.a_merged, "hidden gradients", type, g->workspace, F, rows, 2, ldw, kBM / 64) ||
-        !make_chunk_map(&maps.b0, &p.b_merged, "x", type, g->x, K, rows, 1, g->ldx, p.bnc / 64))
+    if (!make_block_map(&maps.a, type, g->workspace, hidden_blocks(plan, rows), p.row_blocks, 64, kBK, kBM / 64) ||
+        !make_chunk_map(&maps.b0, &p.b_merged, "x", type, g->x, K, rows, g->ldx, p.bnc / 64))
         return -1;
     maps.b1 = maps.b0;
     if (p.splits > 1) {
@@ -888,7 +916,7 @@ extern "C" int rl2_gated_forward(void* opaque, const rl2_gated_forward_args* g, 
         !matrix_ok("output", g->out, g->ld_out, plan->hidden, 2))
         return -1;
     return project(plan, g->rows, g->x, g->ldx, g->gate_weight, g->ld_gate, g->up_weight, g->ld_up, nullptr, 0, g->out,
-                   g->ld_out, g->ld_out * g->rows, g->health, as_stream(stream));
+                   g->ld_out, g->health, as_stream(stream));
 }
 
 extern "C" int rl2_gated_backward(void* opaque, const rl2_gated_backward_args* g, void* stream) {
@@ -932,9 +960,8 @@ extern "C" int rl2_gated_backward(void* opaque, const rl2_gated_backward_args* g
         set_error("gated MLP backward: grad_x may not be x (the weight gradients read x after it is written)");
         return -1;
     }
-    const long long ldw = pad(F, 8);
     if (project(plan, g->rows, g->x, g->ldx, g->gate_weight, g->ld_gate, g->up_weight, g->ld_up, g->grad_out,
-                g->ld_grad_out, g->workspace, ldw, ldw * g->rows, g->health, s))
+                g->ld_grad_out, g->workspace, 0, g->health, s))
         return -1;
     if (g->grad_x && input_gradient(plan, g, s)) return -1;
     return weights ? weight_gradients(plan, g, s) : 0;
