@@ -870,7 +870,9 @@ int rl2_peer_mean(long long count, const rl2_syncbn_exchange* ex, void* stream);
  * dg = grad_out u act'(g), du = grad_out act(g), rounded to the operand type once.
  * grad_x may be null, and grad_gate with grad_up; gradients are assigned, not added.
  * grad_weight_fp32: the weight gradients are fp32 (row strides in floats, multiples of
- * 4). workspace: rl2_gated_workspace_bytes(plan) bytes, 256-byte aligned, free to use
+ * 4). grad_weight_scale (a device float, optional) multiplies them before they are
+ * rounded: the inverse of the loss scale that grad_out carries. workspace:
+ * rl2_gated_workspace_bytes(plan) bytes, 256-byte aligned, free to use
  * again after the call's work. rows = 0 is allowed (zero weight gradients).
  * ------------------------------------------------------------------------- */
 typedef struct rl2_gated_desc {
@@ -908,6 +910,7 @@ typedef struct rl2_gated_backward_args {
     void* grad_up;
     long long ld_grad_up;
     int grad_weight_fp32;
+    const float* grad_weight_scale;
     void* workspace;
     int* health;
 } rl2_gated_backward_args;

@@ -75,6 +75,7 @@ struct Params {
     int store_cols;     // columns that the store engine writes; the rest of a row (less than 16 bytes) by plain stores
     void* out[2];       // kForward, kInput: out[0]; kWeight: by gate / up
     long long ld_out[2];
+    const float* scale; // kWeight, not split: multiplies the output
     int* health;
 };
 
@@ -322,6 +323,7 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
     uint64_t* in_bar = in_full + (warp - 2);
     const uint32_t n = 2u * p.bnc;
     const int row_bytes = OUT32 ? 128 : p.box_cols * 2;
+    const float scale = MODE == kWeight && p.scale ? *p.scale : 1.0f;
     int i = 0;
     for (int t = blockIdx.x >> 1; t < p.tiles_total; t += gridDim.x >> 1, ++i) {
         const Tile w = decode(p, t);
@@ -406,6 +408,10 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
                 for (int e = 0; e < p.box_cols; e += 32) {
                     float r[32];
                     ptx::tmem_ld32(base + slot * mine + c + e, r);
+                    if (MODE == kWeight) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) r[k] *= scale;
+                    }
                     if (OUT32) {
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
@@ -508,11 +514,12 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 template <typename OUT>
-__global__ void reduce_kernel(const float* __restrict__ part, int splits, int rows, int cols, int ld_part,
+__global__ void reduce_kernel(const float* __restrict__ part, const float* __restrict__ scale, int splits, int rows, int cols, int ld_part,
                               OUT* __restrict__ gate, long long ld_gate, OUT* __restrict__ up, long long ld_up) {
     const int quads = (cols + 3) / 4;
     const long long per = static_cast<long long>(rows) * quads;
     const long long plane = static_cast<long long>(rows) * ld_part;
+    const float factor = scale ? *scale : 1.0f;
     for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < 2 * per;
          i += static_cast<long long>(gridDim.x) * blockDim.x) {
         const int z = i >= per;
@@ -530,10 +537,10 @@ __global__ void reduce_kernel(const float* __restrict__ part, int splits, int ro
             sum.w += v.w;
         }
         OUT* dst = (z ? up + row * ld_up : gate + row * ld_gate) + col;
-        dst[0] = narrow<OUT>(sum.x);
-        if (col + 1 < cols) dst[1] = narrow<OUT>(sum.y);
-        if (col + 2 < cols) dst[2] = narrow<OUT>(sum.z);
-        if (col + 3 < cols) dst[3] = narrow<OUT>(sum.w);
+        dst[0] = narrow<OUT>(sum.x * factor);
+        if (col + 1 < cols) dst[1] = narrow<OUT>(sum.y * factor);
+        if (col + 2 < cols) dst[2] = narrow<OUT>(sum.z * factor);
+        if (col + 3 < cols) dst[3] = narrow<OUT>(sum.w * factor);
     }
 }
 
@@ -775,7 +782,7 @@ template <typename OUT>
 void reduce(const float* part, int splits, int rows, int cols, int ld, const rl2_gated_backward_args* g, cudaStream_t stream) {
     const long long quads = 2LL * rows * ((cols + 3) / 4);
     const int blocks = static_cast<int>(std::min<long long>((quads + 255) / 256, 148 * 8));
-    reduce_kernel<OUT><<<blocks, 256, 0, stream>>>(part, splits, rows, cols, ld, static_cast<OUT*>(g->grad_gate),
+    reduce_kernel<OUT><<<blocks, 256, 0, stream>>>(part, g->grad_weight_scale, splits, rows, cols, ld, static_cast<OUT*>(g->grad_gate),
                                                    g->ld_grad_gate, static_cast<OUT*>(g->grad_up), g->ld_grad_up);
 }
 
@@ -807,6 +814,7 @@ int weight_gradients(const Plan* plan, const rl2_gated_backward_args* g, cudaStr
     p.out[1] = g->grad_up;
     p.ld_out[0] = g->ld_grad_gate;
     p.ld_out[1] = g->ld_grad_up;
+    p.scale = p.splits > 1 ? nullptr : g->grad_weight_scale;
     Maps maps;
     if (!make_block_map(&maps.a, type, g->workspace, hidden_blocks(plan, rows), p.row_blocks, 64, kBK, kBM / 64) ||
         !make_chunk_map(&maps.b0, &p.b_merged, "x", type, g->x, K, rows, g->ldx, p.bnc / 64))

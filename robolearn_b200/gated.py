@@ -81,10 +81,11 @@ class GatedMLP:
                                up_weight.data_ptr(), _ld(up_weight), out.data_ptr(), _ld(out), N.ptr(health))
         N.check(self._lib.rl2_gated_forward(self.handle, ctypes.byref(a), N.raw_stream(stream, self.device.index)), "gated MLP forward")
 
-    def backward(self, *, x, gate_weight, up_weight, grad_out, grad_x=None, grad_gate=None, grad_up=None, health=None,
-                 stream=None) -> None:
+    def backward(self, *, x, gate_weight, up_weight, grad_out, grad_x=None, grad_gate=None, grad_up=None,
+                 grad_weight_scale=None, health=None, stream=None) -> None:
         """Gradients of ``sum(out * grad_out)``: ``grad_x`` (optional) in the operand type, ``grad_gate`` and
-        ``grad_up`` (both or neither) in the operand type or both fp32. They are assigned."""
+        ``grad_up`` (both or neither) in the operand type or both fp32, times ``grad_weight_scale`` (one device
+        float, optional: the inverse loss scale). They are assigned."""
         rows, K, F, dt, dev = x.shape[0], self.features, self.hidden, self.dtype, self.device
         _matrix("x", x, rows, K, dt, dev)
         _matrix("gate_weight", gate_weight, F, K, dt, dev)
@@ -108,6 +109,10 @@ class GatedMLP:
             a.grad_gate, a.ld_grad_gate = grad_gate.data_ptr(), _ld(grad_gate)
             a.grad_up, a.ld_grad_up = grad_up.data_ptr(), _ld(grad_up)
             a.grad_weight_fp32 = int(wt == torch.float32)
+            if grad_weight_scale is not None:
+                if grad_weight_scale.numel() != 1 or grad_weight_scale.dtype != torch.float32 or grad_weight_scale.device != dev:
+                    raise ValueError(f"grad_weight_scale must be one float32 on {dev}")
+                a.grad_weight_scale = grad_weight_scale.data_ptr()
         N.check(self._lib.rl2_gated_backward(self.handle, ctypes.byref(a), N.raw_stream(stream, self.device.index)), "gated MLP backward")
 
     def close(self) -> None:

@@ -131,6 +131,20 @@ def test_fp32_weight_gradients(rows, features, hidden, dtype):
     run(rows, features, hidden, dtype, "silu", weight_dtype=torch.float32)
 
 
+@pytest.mark.parametrize("rows,features,hidden,dtype", [(40, 64, 96, torch.float16), (17000, 64, 128, torch.float16)])
+def test_scaled_weight_gradients(rows, features, hidden, dtype):
+    """A power of two before the rounding: the same bits, scaled (also where the rows are split)."""
+    x, wg, wu, dh = inputs(rows, features, hidden, dtype)
+    op = GatedMLP(rows, features, hidden, dtype=dtype)
+    make = lambda: (matrix(hidden, features, torch.float32), matrix(hidden, features, torch.float32))  # noqa: E731
+    a, b = make()
+    op.backward(x=x, gate_weight=wg, up_weight=wu, grad_out=dh, grad_gate=a, grad_up=b)
+    c, d = make()
+    op.backward(x=x, gate_weight=wg, up_weight=wu, grad_out=dh, grad_gate=c, grad_up=d,
+                grad_weight_scale=torch.full((1,), 2.0 ** -10, device="cuda"))
+    assert torch.equal(c * 1024, a) and torch.equal(d * 1024, b)
+
+
 def test_outputs_stay_inside():
     """The padding between rows (poisoned with NaN on input) is neither read nor written."""
     x, wg, wu, _ = inputs(70, 77, 83, torch.float16, extra=16)
@@ -262,5 +276,7 @@ def test_refusals():
         op.backward(**back)
     with pytest.raises(ValueError, match="come together"):
         op.backward(**back, grad_gate=matrix(24, 16, torch.float16))
+    with pytest.raises(ValueError, match="grad_weight_scale must be"):
+        op.backward(**back, grad_gate=matrix(24, 16, torch.float16), grad_up=matrix(24, 16, torch.float16), grad_weight_scale=dh)
     with pytest.raises(RuntimeError, match="may not be x"):
         op.backward(**back, grad_x=x)
