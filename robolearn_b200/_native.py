@@ -278,6 +278,28 @@ def raw_stream(stream, device_index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
+def matrix(name: str, t, rows: int, cols: int, types, device) -> tuple[int, int]:
+    """Address and row stride (elements) of a [rows, cols] matrix with contiguous rows on ``device``, of one of
+    ``types``; anything else is refused. A single row's stride is its own length."""
+    stride = t.stride()
+    if t.shape != (rows, cols):
+        raise ValueError(f"{name} must be of shape ({rows}, {cols}), got {tuple(t.shape)}")
+    if t.dtype not in types:
+        raise ValueError(f"{name} must be {' or '.join(map(str, types))}, got {t.dtype}")
+    if t.get_device() != device.index:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if cols > 1 and stride[1] != 1:
+        raise ValueError(f"{name} must have contiguous rows (column stride 1, got {stride[1]})")
+    return t.data_ptr(), stride[0] if rows > 1 else cols
+
+
+def vector(name: str, t, n: int, dtype, device) -> int:
+    """Address of ``n`` contiguous values of ``dtype`` on ``device``; anything else is refused."""
+    if t.shape != (n,) or t.dtype != dtype or t.get_device() != device.index or not t.is_contiguous():
+        raise ValueError(f"{name} must be {n} contiguous {dtype} values on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
 class ReplayIngestArgs(ctypes.Structure):
     """``rl2_replay_ingest_args`` (include/rl2.h)."""
 

@@ -24,19 +24,13 @@ class TopKDistillation:
         self.counter = torch.zeros(1, dtype=torch.int32, device=device)
         self.row_loss = torch.zeros(self.rows, device=device)
         self.device = self.counter.device
+        self._counter = self.counter.data_ptr()
 
     def _matrix(self, name, t, rows, cols, types):
-        if t.shape != (rows, cols) or t.dtype not in types or t.device != self.device:
-            raise ValueError(f"{name} must be ({rows}, {cols}) of {sorted(map(str, types))} on {self.device}, got "
-                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
-        if cols > 1 and t.stride(1) != 1:
-            raise ValueError(f"{name} must have contiguous rows")
-        return t.data_ptr(), t.stride(0) if rows > 1 else cols, types[t.dtype]
+        return *N.matrix(name, t, rows, cols, types, self.device), types[t.dtype]
 
     def _vector(self, name, t, n):
-        if t.shape != (n,) or t.dtype != torch.float32 or t.device != self.device or not t.is_contiguous():
-            raise ValueError(f"{name} must be {n} contiguous float32 values on {self.device}")
-        return t.data_ptr()
+        return N.vector(name, t, n, torch.float32, self.device)
 
     def run(self, *, logits, teacher_values, teacher_indices, temperature=1.0, row_weight=None, loss_weight=1.0,
             row_loss=None, loss_out=None, dlogits=None, grad_scale=None, health=None, stream=None) -> None:
@@ -46,12 +40,10 @@ class TopKDistillation:
         n = logits.shape[0]
         if n > self.rows:
             raise ValueError(f"at most {self.rows} rows, got {n}")
-        a = N.DistillArgs(rows=n, vocab=self.vocab, top=self.top, temperature=temperature, loss_weight=loss_weight,
-                          counter=self.counter.data_ptr(), health=N.ptr(health))
-        a.logits, a.ld_logits, a.logits_dtype = self._matrix("logits", logits, n, self.vocab, DTYPES)
-        a.teacher_values, a.ld_values, a.values_dtype = self._matrix("teacher_values", teacher_values, n, self.top, DTYPES)
-        a.teacher_indices, a.ld_indices, a.index_bits = self._matrix("teacher_indices", teacher_indices, n, self.top,
-                                                                     INDEX_BITS)
+        a = N.DistillArgs(n, self.vocab, self.top, *self._matrix("logits", logits, n, self.vocab, DTYPES),
+                          *self._matrix("teacher_values", teacher_values, n, self.top, DTYPES),
+                          *self._matrix("teacher_indices", teacher_indices, n, self.top, INDEX_BITS), temperature, None,
+                          loss_weight, counter=self._counter, health=N.ptr(health))
         if row_weight is not None:
             a.row_weight = self._vector("row_weight", row_weight, n)
         a.row_loss = self.row_loss.data_ptr() if row_loss is None else self._vector("row_loss", row_loss, n)

@@ -13,27 +13,6 @@ DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
 
 
-def _matrix(name: str, t: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """Refuse what the kernels cannot read: shape, type, device, row layout."""
-    if t.shape != (rows, cols):
-        raise ValueError(f"{name} must have shape ({rows}, {cols}), got {tuple(t.shape)}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if cols > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name} must have contiguous rows (column stride 1, got {t.stride(1)})")
-    return t
-
-
-def _ld(t: torch.Tensor) -> int:
-    """Row stride in elements; a single row's is free, so it is its padded length (16-byte multiples)."""
-    if t.shape[0] > 1:
-        return t.stride(0)
-    quantum = 16 // t.element_size()
-    return -(-t.shape[1] // quantum) * quantum
-
-
 class GatedMLP:
     """Plan of one gated block for up to ``rows`` rows: ``x`` [rows, features], ``gate_weight`` and
     ``up_weight`` [hidden, features], output [rows, hidden], all ``dtype`` (fp16 or bf16).
@@ -51,6 +30,7 @@ class GatedMLP:
         self.handle = None
         self.rows, self.features, self.hidden = int(rows), int(features), int(hidden)
         self.dtype, self.activation = dtype, activation
+        self._types = (dtype,)
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
@@ -60,6 +40,12 @@ class GatedMLP:
         with torch.cuda.device(self.device):
             self.handle = N.created(self._lib.rl2_gated_create(ctypes.byref(desc)), "create gated MLP plan")
         self._workspace = None
+
+    def _matrix(self, name, t, rows, cols, types=None) -> tuple[int, int]:
+        address, ld = N.matrix(name, t, rows, cols, types or self._types, self.device)
+        # a single row's stride is free: its length, padded to 16 bytes
+        quantum = 8 if t.dtype != torch.float32 else 4
+        return address, ld if rows > 1 else -(-cols // quantum) * quantum
 
     def workspace_bytes(self) -> int:
         return self._lib.rl2_gated_workspace_bytes(self.handle)
@@ -72,47 +58,37 @@ class GatedMLP:
 
     def forward(self, *, x, gate_weight, up_weight, out, health=None, stream=None) -> None:
         """``out = act(x gate_weight^T) * (x up_weight^T)`` for ``x.shape[0]`` <= ``rows`` rows."""
-        rows, K, F, dt, dev = x.shape[0], self.features, self.hidden, self.dtype, self.device
-        _matrix("x", x, rows, K, dt, dev)
-        _matrix("gate_weight", gate_weight, F, K, dt, dev)
-        _matrix("up_weight", up_weight, F, K, dt, dev)
-        _matrix("out", out, rows, F, dt, dev)
-        a = N.GatedForwardArgs(rows, x.data_ptr(), _ld(x), gate_weight.data_ptr(), _ld(gate_weight),
-                               up_weight.data_ptr(), _ld(up_weight), out.data_ptr(), _ld(out), N.ptr(health))
-        N.check(self._lib.rl2_gated_forward(self.handle, ctypes.byref(a), N.raw_stream(stream, self.device.index)), "gated MLP forward")
+        rows, K, F = x.shape[0], self.features, self.hidden
+        m = self._matrix
+        a = N.GatedForwardArgs(rows, *m("x", x, rows, K), *m("gate_weight", gate_weight, F, K),
+                               *m("up_weight", up_weight, F, K), *m("out", out, rows, F),
+                               None if health is None else health.data_ptr())
+        N.check(self._lib.rl2_gated_forward(self.handle, ctypes.byref(a), N.raw_stream(stream, self.device.index)),
+                "gated MLP forward")
 
     def backward(self, *, x, gate_weight, up_weight, grad_out, grad_x=None, grad_gate=None, grad_up=None,
                  grad_weight_scale=None, health=None, stream=None) -> None:
         """Gradients of ``sum(out * grad_out)``: ``grad_x`` (optional) in the operand type, ``grad_gate`` and
         ``grad_up`` (both or neither) in the operand type or both fp32, times ``grad_weight_scale`` (one device
         float, optional: the inverse loss scale). They are assigned."""
-        rows, K, F, dt, dev = x.shape[0], self.features, self.hidden, self.dtype, self.device
-        _matrix("x", x, rows, K, dt, dev)
-        _matrix("gate_weight", gate_weight, F, K, dt, dev)
-        _matrix("up_weight", up_weight, F, K, dt, dev)
-        _matrix("grad_out", grad_out, rows, F, dt, dev)
+        rows, K, F = x.shape[0], self.features, self.hidden
+        m = self._matrix
         if (grad_gate is None) != (grad_up is None):
             raise ValueError("grad_gate and grad_up come together")
-        a = N.GatedBackwardArgs(rows=rows, x=x.data_ptr(), ldx=_ld(x), gate_weight=gate_weight.data_ptr(),
-                                ld_gate=_ld(gate_weight), up_weight=up_weight.data_ptr(), ld_up=_ld(up_weight),
-                                grad_out=grad_out.data_ptr(), ld_grad_out=_ld(grad_out), health=N.ptr(health),
+        a = N.GatedBackwardArgs(rows, *m("x", x, rows, K), *m("gate_weight", gate_weight, F, K),
+                                *m("up_weight", up_weight, F, K), *m("grad_out", grad_out, rows, F), health=N.ptr(health),
                                 workspace=self.workspace().data_ptr())
         if grad_x is not None:
-            _matrix("grad_x", grad_x, rows, K, dt, dev)
-            a.grad_x, a.ld_grad_x = grad_x.data_ptr(), _ld(grad_x)
+            a.grad_x, a.ld_grad_x = m("grad_x", grad_x, rows, K)
         if grad_gate is not None:
-            wt = grad_gate.dtype
-            if wt not in (dt, torch.float32):
-                raise ValueError(f"weight gradients must be {dt} or float32, got {wt}")
-            _matrix("grad_gate", grad_gate, F, K, wt, dev)
-            _matrix("grad_up", grad_up, F, K, wt, dev)
-            a.grad_gate, a.ld_grad_gate = grad_gate.data_ptr(), _ld(grad_gate)
-            a.grad_up, a.ld_grad_up = grad_up.data_ptr(), _ld(grad_up)
-            a.grad_weight_fp32 = int(wt == torch.float32)
+            types = (grad_gate.dtype,)
+            if types[0] not in (self.dtype, torch.float32):
+                raise ValueError(f"weight gradients must be {self.dtype} or float32, got {types[0]}")
+            a.grad_gate, a.ld_grad_gate = m("grad_gate", grad_gate, F, K, types)
+            a.grad_up, a.ld_grad_up = m("grad_up", grad_up, F, K, types)
+            a.grad_weight_fp32 = int(types[0] == torch.float32)
             if grad_weight_scale is not None:
-                if grad_weight_scale.numel() != 1 or grad_weight_scale.dtype != torch.float32 or grad_weight_scale.device != dev:
-                    raise ValueError(f"grad_weight_scale must be one float32 on {dev}")
-                a.grad_weight_scale = grad_weight_scale.data_ptr()
+                a.grad_weight_scale = N.vector("grad_weight_scale", grad_weight_scale, 1, torch.float32, self.device)
         N.check(self._lib.rl2_gated_backward(self.handle, ctypes.byref(a), N.raw_stream(stream, self.device.index)), "gated MLP backward")
 
     def close(self) -> None:
