@@ -1070,6 +1070,16 @@ struct Work {
             group.sync();
         }
     }
+    // the counts alone
+    __device__ __forceinline__ void merge_counts() {
+        group.sync();
+        if (group.size > 1) {
+            if (group.rank != 0)
+                for (int i = threadIdx.x; i < kBins; i += kT)
+                    if (const uint32_t c = sh->count[i]) add32(peer(&sh->count[i], 0), c);
+            group.sync();
+        }
+    }
     // The bin of the merged histogram at which the limit is reached; on every CTA.
     __device__ __forceinline__ Found search(bool by_mass, u64 limit) {
         if (group.rank == 0) {
@@ -1529,8 +1539,8 @@ __global__ void __launch_bounds__(kT, 2) row_kernel(const rl2_sample_args a, con
                     if (bin < kBins - 1) atomicAdd(&sh->count[bin], 1u);
                 }
                 static_assert(kEach == 4, "four bins a thread");
-                if (size == 1 || r.top_k <= kList / 2 / size) {
-                    // each CTA's own bound is one of the whole row (and the list still short)
+                work.merge_counts();
+                if (rank == 0) {
                     if (tid == 0) sh->found.bin = kBins;
                     __syncthreads();
                     const uint4 mine = *reinterpret_cast<const uint4*>(&sh->count[tid * kEach]);
@@ -1543,12 +1553,10 @@ __global__ void __launch_bounds__(kT, 2) row_kernel(const rl2_sample_args a, con
                         at += in_order[e];
                     }
                     __syncthreads();
-                    bound = min(bound, sh->found.bin);
-                    if (size > 1) bound = static_cast<int>(~work.group.max_key(~static_cast<uint32_t>(bound)));
-                } else {
-                    work.merge(kBins);
-                    bound = min(bound, work.search(false, static_cast<u64>(r.top_k)).bin);
+                    if (tid > 0 && tid < size) store32(peer(&sh->found.bin, tid), static_cast<uint32_t>(sh->found.bin));
                 }
+                if (size > 1) work.group.sync();
+                bound = min(bound, sh->found.bin);
             }
             if (r.top_p >= 1.0f && r.min_p > 0.0f)  // one bin of slack for the rounding of the logarithm
                 bound = min(bound, static_cast<int>(min(-logf(r.min_p) * (kBins / kReach) + 1.0f, kBins - 1.0f)));
