@@ -401,7 +401,7 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
                 ptx::bulk_commit();
             }
         } else {
-            const int z = MODE == kWeight ? (p.splits > 1 ? w.split * 2 + w.z : 0) : 0;
+            const int z = p.splits > 1 ? (MODE == kWeight ? w.split * 2 + w.z : w.split) : 0;
             const CUtensorMap* dst = MODE == kWeight && p.splits == 1 && w.z ? &maps.d1 : &maps.d0;
             for (int c = 0; c < mine; c += p.box_cols) {
                 if (lane == 0) ptx::bulk_wait_read0();
@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(kStripThreads, 1) strip_kernel(const __grid_co
     }
 }
 
-// out_z[f][k] = sum over splits, in split order, of part[split][z][f][k]; z = gate, up
+// out_z[f][k] = sum over splits, in split order, of part[split][z][f][k]; z = gate, up (or one matrix alone)
 template <typename OUT>
 __device__ __forceinline__ OUT narrow(float v);
 template <>
@@ -771,13 +771,13 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 template <typename OUT>
-__global__ void reduce_kernel(const float* __restrict__ part, const float* __restrict__ scale, int splits, int rows, int cols, int ld_part,
+__global__ void reduce_kernel(const float* __restrict__ part, const float* __restrict__ scale, int splits, int matrices, int rows, int cols, int ld_part,
                               OUT* __restrict__ gate, long long ld_gate, OUT* __restrict__ up, long long ld_up) {
     const int quads = (cols + 3) / 4;
     const long long per = static_cast<long long>(rows) * quads;
     const long long plane = static_cast<long long>(rows) * ld_part;
     const float factor = scale ? *scale : 1.0f;
-    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < 2 * per;
+    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < matrices * per;
          i += static_cast<long long>(gridDim.x) * blockDim.x) {
         const int z = i >= per;
         const long long j = i - z * per;
@@ -787,7 +787,7 @@ __global__ void reduce_kernel(const float* __restrict__ part, const float* __res
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (int s = 0; s < splits; ++s) {
-            const float4 v = *reinterpret_cast<const float4*>(src + 2 * s * plane);
+            const float4 v = *reinterpret_cast<const float4*>(src + static_cast<long long>(matrices) * s * plane);
             sum.x += v.x;
             sum.y += v.y;
             sum.z += v.z;
@@ -904,6 +904,7 @@ KernelFn gated_kernel(int mode, int act) {
 KernelFn kernel_of(const Plan* plan, int mode, bool out32) {
     if (mode == kForward || mode == kGate)
         return plan->bf16 ? gated_kernel<true>(mode, plan->act) : gated_kernel<false>(mode, plan->act);
+    if (mode == kInput && out32) return plan->bf16 ? product_kernel<kInput, true, 0, true> : product_kernel<kInput, false, 0, true>;
     if (mode == kInput) return plan->bf16 ? product_kernel<kInput, true, 0, false> : product_kernel<kInput, false, 0, false>;
     if (out32) return plan->bf16 ? product_kernel<kWeight, true, 0, true> : product_kernel<kWeight, false, 0, true>;
     return plan->bf16 ? product_kernel<kWeight, true, 0, false> : product_kernel<kWeight, false, 0, false>;
@@ -960,9 +961,11 @@ int hidden_blocks(const Plan* plan, int rows) {
 long long gate_bytes(const Plan* plan) {
     return 2LL * row_blocks(plan->rows) * ((plan->hidden + 127) / 128 * 2) * kBM * 128;
 }
-long long part_bytes(const Plan* plan) {  // splits grow with the rows
+long long part_bytes(const Plan* plan) {  // the weight gradients' splits grow with the rows
     const long long s = splits_for(plan, plan->rows);
-    return s > 1 ? s * 2 * plan->hidden * pad(plan->features, 4) * 4 : 0;
+    const long long weights = s > 1 ? s * 2 * plan->hidden * pad(plan->features, 4) * 4 : 0;
+    // the input gradient's partial sums: at most a 256 x 128 tile (its last columns padded to 4) per pair
+    return std::max(weights, plan->pairs * 256LL * 132 * 4);
 }
 
 bool ready(const Plan* plan, int rows) {
@@ -1015,6 +1018,22 @@ int project(const Plan* plan, int rows, const void* x, long long ldx, const void
     if (grad_out && !make_map(&maps.in, "output gradient", type, grad_out, F, rows, 1, ld_grad, ld_grad * rows, p.box_cols, 32))
         return -1;
     return launch(plan, mode, false, p, maps, stream);
+}
+
+template <typename OUT>
+void reduce_as(const float* part, const float* scale, int splits, int matrices, int rows, int cols, int ld, void* first, long long ld_first,
+               void* second, long long ld_second, cudaStream_t stream) {
+    const long long quads = static_cast<long long>(matrices) * rows * ((cols + 3) / 4);
+    const int blocks = static_cast<int>(std::min<long long>((quads + 255) / 256, 148 * 8));
+    reduce_kernel<OUT><<<blocks, 256, 0, stream>>>(part, scale, splits, matrices, rows, cols, ld, static_cast<OUT*>(first), ld_first,
+                                                   static_cast<OUT*>(second), ld_second);
+}
+
+int reduce(const Plan* plan, bool fp32, const float* part, const float* scale, int splits, int matrices, int rows, int cols, int ld, void* first,
+           long long ld_first, void* second, long long ld_second, cudaStream_t stream) {
+    const auto run = fp32 ? reduce_as<float> : plan->bf16 ? reduce_as<__nv_bfloat16> : reduce_as<__half>;
+    run(part, scale, splits, matrices, rows, cols, ld, first, ld_first, second, ld_second, stream);
+    return launch_status("gated MLP reduction of splits");
 }
 
 // 17 to 128 rows, forward. Device time for that of the 256-row tiles: 15.0 us for 20.3 (32 rows) and 17.5 for 22.2
@@ -1072,13 +1091,20 @@ int input_gradient(const Plan* plan, const rl2_gated_backward_args* g, cudaStrea
     p.bnc = width_for(plan, p.tiles_m, K, 2);
     p.tile_cols = 2 * p.bnc;
     p.tiles_n = (K + p.tile_cols - 1) / p.tile_cols;
-    p.tiles_z = p.splits = 1;
+    p.tiles_z = 1;
     p.kb_segment = (F + kBK - 1) / kBK;
-    p.kblocks = p.kb_per_split = 2 * p.kb_segment;
-    p.box_cols = 64;
+    p.kblocks = 2 * p.kb_segment;
+    // few tiles: the contraction in pieces of at least 16 k-blocks, while each adds pairs at work
+    p.splits = static_cast<int>(std::max<long long>(1, std::min<long long>(plan->pairs / (static_cast<long long>(p.tiles_m) * p.tiles_n), p.kblocks / 16)));
+    p.kb_per_split = (p.kblocks + p.splits - 1) / p.splits;
+    p.splits = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;  // every split non-empty
+    const bool split = p.splits > 1;
+    const long long ldp = pad(K, 4);
+    float* part = reinterpret_cast<float*>(static_cast<char*>(g->workspace) + gate_bytes(plan));
+    p.box_cols = split ? 32 : 64;
     p.out_rows = rows;
     p.out_cols = K;
-    p.store_cols = K / 8 * 8;
+    p.store_cols = split ? K : K / 8 * 8;
     p.out[0] = g->grad_x;
     p.ld_out[0] = g->ld_grad_x;
     p.health = g->health;
@@ -1086,19 +1112,14 @@ int input_gradient(const Plan* plan, const rl2_gated_backward_args* g, cudaStrea
     if (!make_block_map(&maps.a, type, g->workspace, hidden_blocks(plan, rows), p.row_blocks, 64, kBM, 1) ||
         !make_chunk_map(&maps.b0, &p.b_merged, "gate weight", type, g->gate_weight, K, F, g->ld_gate, p.bnc / 64) ||
         !make_chunk_map(&maps.b1, &p.b_merged, "up weight", type, g->up_weight, K, F, g->ld_up, p.bnc / 64) ||
-        !make_map(&maps.d0, "input gradient", type, g->grad_x, stored(K, 8), rows, 1, g->ld_grad_x, g->ld_grad_x * rows, 64, 32))
+        !(split ? make_map(&maps.d0, "partial input gradients", CU_TENSOR_MAP_DATA_TYPE_FLOAT32, part, K, rows, p.splits, ldp, ldp * rows, 32, 32)
+                : make_map(&maps.d0, "input gradient", type, g->grad_x, stored(K, 8), rows, 1, g->ld_grad_x, g->ld_grad_x * rows, 64, 32)))
         return -1;
     maps.d1 = maps.in = maps.d0;
-    return launch(plan, kInput, false, p, maps, stream);
+    if (launch(plan, kInput, split, p, maps, stream)) return -1;
+    return split ? reduce(plan, false, part, nullptr, p.splits, 1, rows, K, static_cast<int>(ldp), g->grad_x, g->ld_grad_x, nullptr, 0, stream) : 0;
 }
 
-template <typename OUT>
-void reduce(const float* part, int splits, int rows, int cols, int ld, const rl2_gated_backward_args* g, cudaStream_t stream) {
-    const long long quads = 2LL * rows * ((cols + 3) / 4);
-    const int blocks = static_cast<int>(std::min<long long>((quads + 255) / 256, 148 * 8));
-    reduce_kernel<OUT><<<blocks, 256, 0, stream>>>(part, g->grad_weight_scale, splits, rows, cols, ld, static_cast<OUT*>(g->grad_gate),
-                                                   g->ld_grad_gate, static_cast<OUT*>(g->grad_up), g->ld_grad_up);
-}
 
 int weight_gradients(const Plan* plan, const rl2_gated_backward_args* g, cudaStream_t stream) {
     const int K = plan->features, F = plan->hidden, rows = g->rows;
@@ -1146,13 +1167,8 @@ int weight_gradients(const Plan* plan, const rl2_gated_backward_args* g, cudaStr
     maps.in = maps.d0;
     if (launch(plan, kWeight, out32, p, maps, stream)) return -1;
     if (p.splits == 1) return 0;
-    if (g->grad_weight_fp32)
-        reduce<float>(part, p.splits, F, K, static_cast<int>(ldp), g, stream);
-    else if (plan->bf16)
-        reduce<__nv_bfloat16>(part, p.splits, F, K, static_cast<int>(ldp), g, stream);
-    else
-        reduce<__half>(part, p.splits, F, K, static_cast<int>(ldp), g, stream);
-    return launch_status("gated MLP weight-gradient reduction");
+    return reduce(plan, g->grad_weight_fp32, part, g->grad_weight_scale, p.splits, 2, F, K, static_cast<int>(ldp), g->grad_gate,
+                  g->ld_grad_gate, g->grad_up, g->ld_grad_up, stream);
 }
 
 }  // namespace gated
@@ -1181,23 +1197,23 @@ extern "C" void* rl2_gated_create(const rl2_gated_desc* d) {
         return nullptr;
     }
     // pairs resident at once, asked (and the kernels' shared memory limits raised) once a device and kernel
-    static std::atomic<int> resident[64][2][3][5];
+    static std::atomic<int> resident[64][2][3][6];
     int sms = 0;
     bool ok = cudaGetDevice(&plan->device) == cudaSuccess &&
               cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, plan->device) == cudaSuccess;
     plan->pairs = sms / 2;
-    for (int i = 0; ok && i < 5; ++i) {
+    for (int i = 0; ok && i < 6; ++i) {  // the four modes, then kInput and kWeight with fp32 outputs
         std::atomic<int>* known = plan->device < 64 ? &resident[plan->device][d->dtype][d->activation][i] : nullptr;
         int clusters = known ? known->load() : 0;
         if (clusters == 0) {
-            const void* fn = reinterpret_cast<const void*>(kernel_of(plan, std::min(i, 3), i == 4));
+            const void* fn = reinterpret_cast<const void*>(kernel_of(plan, i < 4 ? i : i - 2, i >= 4));
             cudaLaunchConfig_t cfg = {};
             cudaLaunchAttribute attr[1];
             attr[0].id = cudaLaunchAttributeClusterDimension;
             attr[0].val.clusterDim.x = 2;
             attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
             cfg.gridDim = dim3(static_cast<unsigned>(2 * std::max(1, sms / 2)));
-            cfg.blockDim = dim3(threads_of(std::min(i, 3)));
+            cfg.blockDim = dim3(threads_of(i < 4 ? i : i - 2));
             cfg.dynamicSmemBytes = kMaxSmem - kStaticSmem;
             cfg.attrs = attr;
             cfg.numAttrs = 1;

@@ -3,6 +3,7 @@ and its backward pass on the tcgen05 tensor cores, without storing either projec
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -37,7 +38,7 @@ class GatedMLP:
         self._lib = N.load()
         desc = N.GatedDesc(rows=self.rows, features=self.features, hidden=self.hidden, dtype=DTYPES[dtype],
                            activation=ACTIVATIONS[activation])
-        with torch.cuda.device(self.device):
+        with contextlib.nullcontext() if self.device.index == torch.cuda.current_device() else torch.cuda.device(self.device):
             self.handle = N.created(self._lib.rl2_gated_create(ctypes.byref(desc)), "create gated MLP plan")
         self._workspace = None
 
