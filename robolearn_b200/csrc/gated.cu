@@ -539,14 +539,14 @@ struct FewArgs {
     int rows, features, hidden, act;
 };
 
-// 8 elements of a row from column k on that reaches past `cols`: 0 there (the rows' padding is not data)
+// 8 elements of a row from column k on where it may end before: 0 past `cols` (the rows' padding is neither data nor
+// read: the last row's need not exist)
 __device__ __forceinline__ uint4 load_end(const uint16_t* row, int k, int cols) {
-    if (k >= cols) return make_uint4(0, 0, 0, 0);
-    uint4 v = __ldg(reinterpret_cast<const uint4*>(row + k));
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if (k + 8 <= cols) return __ldg(reinterpret_cast<const uint4*>(row + k));
+    uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (k + e >= cols) w[e / 2] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+    for (int e = 0; e < 7; ++e)
+        if (k + e < cols) w[e / 2] |= static_cast<uint32_t>(__ldg(row + k + e)) << (16 * (e & 1));
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -927,9 +927,14 @@ int launch(const Plan* plan, int mode, bool out32, Params& p, const Maps& maps, 
     return launch_status("gated MLP product");
 }
 
-// Tile width: 128 B rows per CTA, or 64 when the wider tiles would leave pairs without one.
+// Tile width: 128 B rows per CTA, or 64 where that ends sooner, by waves of tiles times a tile's cost (its width,
+// and its share of the A rows as much as 16 columns).
 int width_for(const Plan* plan, long long row_tiles, long long cols, int per_row) {
-    return row_tiles * ((cols + 128 * per_row - 1) / (128 * per_row)) < plan->pairs ? 64 : 128;
+    auto cost = [&](int width) {
+        const long long tiles = row_tiles * ((cols + width * per_row - 1) / (width * per_row));
+        return (tiles + plan->pairs - 1) / plan->pairs * (width + 16);
+    };
+    return cost(64) < cost(128) ? 64 : 128;
 }
 
 // Splits of the weight gradients' contraction over `rows`: one tile per pair where the splits stay at least 16

@@ -90,6 +90,8 @@ class GatedMLP:
             a.grad_weight_fp32 = int(types[0] == torch.float32)
             if grad_weight_scale is not None:
                 a.grad_weight_scale = N.vector("grad_weight_scale", grad_weight_scale, 1, torch.float32, self.device)
+        if stream is not None:  # the workspace is the current stream's; this call's work on it is another's
+            self._workspace.record_stream(stream)
         N.check(self._lib.rl2_gated_backward(self.handle, ctypes.byref(a), N.raw_stream(stream, self.device.index)), "gated MLP backward")
 
     def close(self) -> None:
