@@ -279,9 +279,10 @@ __device__ __forceinline__ void finish(const rl2_distill_args& a) {
     if (!last) return;
     __threadfence();
     float sum = 0.0f;
+#pragma unroll 8
     for (int n = tid; n < a.rows; n += threads) {
-        const float w = a.row_weight ? a.row_weight[n] : 1.0f;
-        if (w != 0.0f) sum += w * __ldcg(a.row_loss + n);
+        const float w = a.row_weight ? a.row_weight[n] : 1.0f, loss = __ldcg(a.row_loss + n);
+        sum += w != 0.0f ? w * loss : 0.0f;
     }
     sum = warp_sum(sum);
     if ((tid & 31) == 0) part[tid >> 5] = sum;
@@ -711,9 +712,10 @@ __global__ void __launch_bounds__(1024) total_kernel(const rl2_distill_args a) {
     __shared__ float part[32];
     const int tid = threadIdx.x;
     float sum = 0.0f;
+#pragma unroll 4
     for (int n = tid; n < a.rows; n += 1024) {
-        const float w = a.row_weight ? a.row_weight[n] : 1.0f;
-        if (w != 0.0f) sum += w * a.row_loss[n];
+        const float w = a.row_weight ? a.row_weight[n] : 1.0f, loss = a.row_loss[n];
+        sum += w != 0.0f ? w * loss : 0.0f;
     }
     sum = warp_sum(sum);
     if ((tid & 31) == 0) part[tid >> 5] = sum;
@@ -761,16 +763,19 @@ int launch_long(const rl2_distill_args& a, cudaStream_t stream) {
 
 template <typename L, typename G>
 int launch(const rl2_distill_args& a, cudaStream_t stream) {
+    if (a.vocab > 2048) return launch_long<L, G>(a, stream);
+    // short rows: the total by the last CTA, or with many rows (whose losses one small CTA takes long to add: 22 us
+    // for 6 + 3 at 4096 x 101) by a launch of its own
+    rl2_distill_args each = a;
+    if (a.rows > 1024) each.loss_out = nullptr;
     if (a.vocab <= 1024 && a.top <= kFewTop) {
         const long long blocks = std::min<long long>((static_cast<long long>(a.rows) + kRowWarps - 1) / kRowWarps, 148 * 8);
-        warp_kernel<L, G><<<static_cast<int>(blocks), 32 * kRowWarps, 0, stream>>>(a);
-        return launch_status("distillation");
+        warp_kernel<L, G><<<static_cast<int>(blocks), 32 * kRowWarps, 0, stream>>>(each);
+    } else {
+        row_kernel<L, G, 128><<<std::min(a.rows, 148 * 16), 128, 0, stream>>>(each);
     }
-    if (a.vocab <= 2048) {
-        row_kernel<L, G, 128><<<std::min(a.rows, 148 * 16), 128, 0, stream>>>(a);
-        return launch_status("distillation");
-    }
-    return launch_long<L, G>(a, stream);
+    if (a.loss_out && !each.loss_out) total_kernel<<<1, 1024, 0, stream>>>(a);
+    return launch_status("distillation");
 }
 
 template <typename L>

@@ -210,15 +210,15 @@ __device__ __forceinline__ Kept both_cuts(const Row& r, int vocab, float best, S
 
 // ---- up to 1024 tokens: a warp per row, N tokens a lane (token lane * N + i) -----------------
 //
-// A cut comes from a histogram of the row over 128 bins of (max - l) / T in shared memory (count, and weight
-// as a low and a high word), then from counting among the tokens of its bin.
+// A cut comes from a histogram of the row over 128 bins of (max - l) / T in shared memory (two words a bin: the
+// count above the weights' low 11 bits, and the weights' high 20), then from counting among the tokens of its bin.
 
 constexpr int kRowWarps = 4;
 constexpr int kRowBins = 128;
 constexpr float kReach = 21.6f;  // exp(-21.6) 2^30 rounds to 0: what is further from the best has no weight
 
 struct RowShared {
-    alignas(16) uint32_t count[kRowBins], low[kRowBins], high[kRowBins];
+    alignas(16) uint32_t low[kRowBins], high[kRowBins];
     float few_value[32];
     uint32_t few_w[32];
 };
@@ -303,7 +303,6 @@ __global__ void __launch_bounds__(32 * kRowWarps) warp_kernel(const rl2_sample_a
             if (!counted) {
                 counted = true;
                 __syncwarp();
-                reinterpret_cast<uint4*>(sh.count)[lane] = make_uint4(0, 0, 0, 0);
                 reinterpret_cast<uint4*>(sh.low)[lane] = make_uint4(0, 0, 0, 0);
                 reinterpret_cast<uint4*>(sh.high)[lane] = make_uint4(0, 0, 0, 0);
                 __syncwarp();
@@ -311,25 +310,25 @@ __global__ void __launch_bounds__(32 * kRowWarps) warp_kernel(const rl2_sample_a
                 for (int i = 0; i < N; ++i)
                     if (w[i]) {
                         const int bin = bin_of(v[i]);
-                        atomicAdd(&sh.count[bin], 1u);
-                        atomicAdd(&sh.low[bin], w[i] & 0xFFFFu);  // 1024 tokens at most: neither word overflows
-                        atomicAdd(&sh.high[bin], w[i] >> 16);
+                        // at most 1024 tokens of at most 2^30: the low words sum to less than 2^21, the high to 2^29
+                        atomicAdd(&sh.low[bin], (1u << 21) | (w[i] & 0x7FFu));
+                        atomicAdd(&sh.high[bin], w[i] >> 11);
                     }
                 __syncwarp();
             }
             Sum mine[4], sum{0, 0};
-            const uint4 c = reinterpret_cast<const uint4*>(sh.count)[lane], lo = reinterpret_cast<const uint4*>(sh.low)[lane],
-                        hi = reinterpret_cast<const uint4*>(sh.high)[lane];
-            mine[0] = Sum{c.x, (static_cast<u64>(hi.x) << 16) + lo.x};
-            mine[1] = Sum{c.y, (static_cast<u64>(hi.y) << 16) + lo.y};
-            mine[2] = Sum{c.z, (static_cast<u64>(hi.z) << 16) + lo.z};
-            mine[3] = Sum{c.w, (static_cast<u64>(hi.w) << 16) + lo.w};
+            const uint4 lo = reinterpret_cast<const uint4*>(sh.low)[lane], hi = reinterpret_cast<const uint4*>(sh.high)[lane];
+            auto bin_sum = [](uint32_t low, uint32_t high) { return Sum{low >> 21, (static_cast<u64>(high) << 11) + (low & 0x1FFFFFu)}; };
+            mine[0] = bin_sum(lo.x, hi.x);
+            mine[1] = bin_sum(lo.y, hi.y);
+            mine[2] = bin_sum(lo.z, hi.z);
+            mine[3] = bin_sum(lo.w, hi.w);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 sum.count += mine[e].count;
                 sum.mass += mine[e].mass;
             }
-            Sum at{warp_scan(sum.count), warp_scan64(sum.mass)};
+            Sum at{kMass ? 0u : warp_scan(sum.count), warp_scan64(sum.mass)};  // a cut by weight needs no counts
             // the bin at which the limit is reached: in one lane
             int bin = -1;
             uint32_t inside = 0;
