@@ -355,6 +355,15 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t cluster_bar) {
                  : "memory");
 }
 
+// ---- programmatic launches ----------------------------------------------------
+
+// The grids before this one in the stream have completed and their memory is visible. Every thread that touches
+// global memory, before it does; every thread of a kernel launched by launch_early.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// The next grid of the stream may take the SMs that this one leaves (it waits in grid_wait for this one's end).
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ uint32_t elect_one() {
     uint32_t pred = 0;
     asm volatile(
@@ -366,6 +375,23 @@ __device__ __forceinline__ uint32_t elect_one() {
 }
 
 }  // namespace ptx
+
+// Launches a kernel whose prologue may run while the stream's previous grid ends (the kernel calls
+// ptx::grid_wait before it touches global memory).
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
 
 // Warp-level reductions shared by the streaming kernels.
 __device__ __forceinline__ float warp_sum(float v) {

@@ -478,6 +478,8 @@ __global__ void __launch_bounds__(threads_of(MODE), 1) __cluster_dims__(2, 1, 1)
     ptx::cluster_sync();  // both CTAs' barriers exist before any remote use
     ptx::tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    ptx::grid_release();
+    ptx::grid_wait();
 
     if (warp == 0) {
         if (ptx::elect_one()) produce<MODE>(maps, p, smem, stage_bytes, full, empty, &abort_flag);
@@ -558,6 +560,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(const FewArgs 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int f0 = blockIdx.x * kFewUnits;
+    ptx::grid_release();
+    ptx::grid_wait();
     // Rows past the end repeat the last one: what they give is not stored.
     const uint16_t* w[4];  // gate rows g and g + 8, up rows g and g + 8
 #pragma unroll
@@ -682,6 +686,8 @@ __global__ void __launch_bounds__(kStripThreads, 1) strip_kernel(const __grid_co
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    ptx::grid_release();
+    ptx::grid_wait();
     if (warp == 0) {
         if (ptx::elect_one()) {
             int issued = 0;
@@ -773,6 +779,8 @@ __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return
 template <typename OUT>
 __global__ void reduce_kernel(const float* __restrict__ part, const float* __restrict__ scale, int splits, int matrices, int rows, int cols, int ld_part,
                               OUT* __restrict__ gate, long long ld_gate, OUT* __restrict__ up, long long ld_up) {
+    ptx::grid_release();
+    ptx::grid_wait();
     const int quads = (cols + 3) / 4;
     const long long per = static_cast<long long>(rows) * quads;
     const long long plane = static_cast<long long>(rows) * ld_part;
@@ -879,15 +887,19 @@ bool matrix_ok(const char* what, const void* base, long long ld, long long cols,
 
 typedef void (*KernelFn)(const Maps, const Params);
 
+int launched(cudaError_t e) {
+    if (e == cudaSuccess) return launch_status("gated MLP");
+    set_error("gated MLP launch: %s", cudaGetErrorString(e));
+    return -1;
+}
+
 template <bool BF16>
 int launch_few(const FewArgs& a, cudaStream_t stream) {
     const int blocks = (a.hidden + kFewUnits - 1) / kFewUnits;
     constexpr int kSums = kFewWarps * 2 * 8 * kFewUnits * 4;  // bytes per 8 rows
-    if (a.rows <= 8)
-        few_rows_kernel<BF16, 1><<<blocks, 32 * kFewWarps, kSums, stream>>>(a);
-    else
-        few_rows_kernel<BF16, 2><<<blocks, 32 * kFewWarps, 2 * kSums, stream>>>(a);
-    return launch_status("gated MLP few-row product");
+    const bool eight = a.rows <= 8;
+    return launched(launch_early(eight ? few_rows_kernel<BF16, 1> : few_rows_kernel<BF16, 2>, blocks, 32 * kFewWarps,
+                                 eight ? kSums : 2 * kSums, stream, a));
 }
 
 template <bool BF16>
@@ -923,8 +935,7 @@ int launch(const Plan* plan, int mode, bool out32, Params& p, const Maps& maps, 
     }
     p.tiles_total = static_cast<int>(total);
     const int pairs = static_cast<int>(std::min<long long>(total, plan->pairs));
-    kernel_of(plan, mode, out32)<<<2 * pairs, threads_of(mode), p.stages * stage + fixed, stream>>>(maps, p);
-    return launch_status("gated MLP product");
+    return launched(launch_early(kernel_of(plan, mode, out32), 2 * pairs, threads_of(mode), p.stages * stage + fixed, stream, maps, p));
 }
 
 // Tile width: 128 B rows per CTA, or 64 where that ends sooner, by waves of tiles times a tile's cost (its width,
@@ -1026,19 +1037,18 @@ int project(const Plan* plan, int rows, const void* x, long long ldx, const void
 }
 
 template <typename OUT>
-void reduce_as(const float* part, const float* scale, int splits, int matrices, int rows, int cols, int ld, void* first, long long ld_first,
+cudaError_t reduce_as(const float* part, const float* scale, int splits, int matrices, int rows, int cols, int ld, void* first, long long ld_first,
                void* second, long long ld_second, cudaStream_t stream) {
     const long long quads = static_cast<long long>(matrices) * rows * ((cols + 3) / 4);
     const int blocks = static_cast<int>(std::min<long long>((quads + 255) / 256, 148 * 8));
-    reduce_kernel<OUT><<<blocks, 256, 0, stream>>>(part, scale, splits, matrices, rows, cols, ld, static_cast<OUT*>(first), ld_first,
-                                                   static_cast<OUT*>(second), ld_second);
+    return launch_early(reduce_kernel<OUT>, blocks, 256, 0, stream, part, scale, splits, matrices, rows, cols, ld, static_cast<OUT*>(first),
+                        ld_first, static_cast<OUT*>(second), ld_second);
 }
 
 int reduce(const Plan* plan, bool fp32, const float* part, const float* scale, int splits, int matrices, int rows, int cols, int ld, void* first,
            long long ld_first, void* second, long long ld_second, cudaStream_t stream) {
     const auto run = fp32 ? reduce_as<float> : plan->bf16 ? reduce_as<__nv_bfloat16> : reduce_as<__half>;
-    run(part, scale, splits, matrices, rows, cols, ld, first, ld_first, second, ld_second, stream);
-    return launch_status("gated MLP reduction of splits");
+    return launched(run(part, scale, splits, matrices, rows, cols, ld, first, ld_first, second, ld_second, stream));
 }
 
 // 17 to 128 rows, forward. Device time for that of the 256-row tiles: 15.0 us for 20.3 (32 rows) and 17.5 for 22.2
@@ -1083,8 +1093,7 @@ int launch_strip(const Plan* plan, const rl2_gated_forward_args* g, cudaStream_t
         }
         if (plan->device <= 63) seen.fetch_or(1ull << plan->device);
     }
-    kernel<<<(F + p.units - 1) / p.units, kStripThreads, smem, stream>>>(maps, p);
-    return launch_status("gated MLP strip product");
+    return launched(launch_early(kernel, (F + p.units - 1) / p.units, kStripThreads, smem, stream, maps, p));
 }
 
 int input_gradient(const Plan* plan, const rl2_gated_backward_args* g, cudaStream_t stream) {
