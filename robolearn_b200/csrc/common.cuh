@@ -379,18 +379,27 @@ __device__ __forceinline__ uint32_t elect_one() {
 // Launches a kernel whose prologue may run while the stream's previous grid ends (the kernel calls
 // ptx::grid_wait before it touches global memory).
 template <typename... P, typename... A>
-cudaError_t launch_early(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, const A&... args) {
+cudaError_t launch_early_clusters(void (*kernel)(P...), unsigned cluster, unsigned grid, unsigned block, size_t smem,
+                                  cudaStream_t stream, const A&... args) {
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, const A&... args) {
+    return launch_early_clusters(kernel, 0, grid, block, smem, stream, args...);
 }
 
 // Warp-level reductions shared by the streaming kernels.

@@ -305,6 +305,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) warp_kernel(const rl2_distill_
     __shared__ float q_s[kRowWarps][kFewTop];
     __shared__ int i_s[kRowWarps][kFewTop];
     const int warp = threadIdx.x >> 5;
+    ptx::grid_release();
+    ptx::grid_wait();
     for (long long row = static_cast<long long>(blockIdx.x) * kRowWarps + warp; row < a.rows;
          row += static_cast<long long>(gridDim.x) * kRowWarps)
         row_by_group<L, G, 32>(a, row, threadIdx.x & 31, nullptr, nullptr, q_s[warp], i_s[warp]);
@@ -317,6 +319,8 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const rl2_distill_args a) 
     __shared__ float red[32], red2[32];
     __shared__ float q_s[kMaxTop];
     __shared__ int i_s[kMaxTop];
+    ptx::grid_release();
+    ptx::grid_wait();
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x)
         row_by_group<L, G, THREADS>(a, row, threadIdx.x, red, red2, q_s, i_s);
     finish(a);
@@ -464,6 +468,8 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
     int* token = reinterpret_cast<int*>(kept + kKept);         // -1: absent
     float* given = reinterpret_cast<float*>(token + padded);   // the teacher's value
     const float scale = kLog2e / a.temperature;
+    ptx::grid_release();
+    ptx::grid_wait();
     const float weight = a.row_weight ? a.row_weight[row] : 1.0f;
     G* ds = a.dlogits ? static_cast<G*>(a.dlogits) + row * a.ld_dlogits : nullptr;
     if (tid == 0) {
@@ -712,6 +718,8 @@ __global__ void __launch_bounds__(1024) total_kernel(const rl2_distill_args a) {
     __shared__ float part[32];
     const int tid = threadIdx.x;
     float sum = 0.0f;
+    ptx::grid_release();
+    ptx::grid_wait();
 #pragma unroll 4
     for (int n = tid; n < a.rows; n += 1024) {
         const float w = a.row_weight ? a.row_weight[n] : 1.0f, loss = a.row_loss[n];
@@ -726,6 +734,12 @@ __global__ void __launch_bounds__(1024) total_kernel(const rl2_distill_args a) {
     }
 }
 
+int launched(cudaError_t e) {
+    if (e == cudaSuccess) return launch_status("distillation");
+    set_error("distillation: %s", cudaGetErrorString(e));
+    return -1;
+}
+
 template <typename L, typename G>
 int launch_long(const rl2_distill_args& a, cudaStream_t stream) {
     // few rows: more CTAs a row, while each has four vectors a thread
@@ -734,17 +748,7 @@ int launch_long(const rl2_distill_args& a, cudaStream_t stream) {
            a.vocab / Slice<L>::kN / (size * 2) >= kHeld * kLong)
         size *= 2;
     constexpr int kMost = kKept * 16 + kMaxTop * 8;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = size;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(static_cast<long long>(a.rows) * size));
-    cfg.blockDim = dim3(kLong);
-    cfg.dynamicSmemBytes = kMost - (kMaxTop - (a.top + 3) / 4 * 4) * 8;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    const size_t smem = kMost - (kMaxTop - (a.top + 3) / 4 * 4) * 8;
     static std::atomic<unsigned long long> allowed{0};  // devices (up to 64) whose limit is raised
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
@@ -752,13 +756,10 @@ int launch_long(const rl2_distill_args& a, cudaStream_t stream) {
         e = cudaFuncSetAttribute(reinterpret_cast<const void*>(long_kernel<L, G>), cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
         if (e == cudaSuccess && device <= 63) allowed.fetch_or(1ull << device);
     }
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, long_kernel<L, G>, a, size);
-    if (e != cudaSuccess) {
-        set_error("distillation: %s", cudaGetErrorString(e));
-        return -1;
-    }
-    if (a.loss_out) total_kernel<<<1, 1024, 0, stream>>>(a);
-    return launch_status("distillation");
+    if (e == cudaSuccess)
+        e = launch_early_clusters(long_kernel<L, G>, size, static_cast<unsigned>(static_cast<long long>(a.rows) * size), kLong, smem, stream, a, size);
+    if (e == cudaSuccess && a.loss_out) e = launch_early(total_kernel, 1, 1024, 0, stream, a);
+    return launched(e);
 }
 
 template <typename L, typename G>
@@ -767,15 +768,16 @@ int launch(const rl2_distill_args& a, cudaStream_t stream) {
     // short rows: the total by the last CTA, or with many rows (whose losses one small CTA takes long to add: 22 us
     // for 6 + 3 at 4096 x 101) by a launch of its own
     rl2_distill_args each = a;
+    cudaError_t e;
     if (a.rows > 1024) each.loss_out = nullptr;
     if (a.vocab <= 1024 && a.top <= kFewTop) {
         const long long blocks = std::min<long long>((static_cast<long long>(a.rows) + kRowWarps - 1) / kRowWarps, 148 * 8);
-        warp_kernel<L, G><<<static_cast<int>(blocks), 32 * kRowWarps, 0, stream>>>(each);
+        e = launch_early(warp_kernel<L, G>, static_cast<unsigned>(blocks), 32 * kRowWarps, 0, stream, each);
     } else {
-        row_kernel<L, G, 128><<<std::min(a.rows, 148 * 16), 128, 0, stream>>>(each);
+        e = launch_early(row_kernel<L, G, 128>, std::min(a.rows, 148 * 16), 128, 0, stream, each);
     }
-    if (a.loss_out && !each.loss_out) total_kernel<<<1, 1024, 0, stream>>>(a);
-    return launch_status("distillation");
+    if (e == cudaSuccess && a.loss_out && !each.loss_out) e = launch_early(total_kernel, 1, 1024, 0, stream, a);
+    return launched(e);
 }
 
 template <typename L>

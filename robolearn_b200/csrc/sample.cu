@@ -251,6 +251,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) warp_kernel(const rl2_sample_a
     const int lane = threadIdx.x & 31;
     const int V = a.vocab;
     WarpGroup group;
+    ptx::grid_release();
+    ptx::grid_wait();
     for (long long row = static_cast<long long>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); row < a.rows;
          row += static_cast<long long>(gridDim.x) * kRowWarps) {
         const L* s = static_cast<const L*>(a.logits) + row * a.ld_logits + lane * N;
@@ -1500,6 +1502,8 @@ __global__ void __launch_bounds__(kT, 2) row_kernel(const rl2_sample_args a, con
     const int tid = threadIdx.x, warp = tid >> 5;
     const int V = a.vocab;
     const uint32_t rank = size > 1 ? ptx::cluster_rank() : 0u;
+    ptx::grid_release();
+    ptx::grid_wait();
     for (long long row = blockIdx.x / size; row < a.rows; row += gridDim.x / size) {
         const Reader<L> in(static_cast<const L*>(a.logits) + row * a.ld_logits, V);
         const int log_per = shift - 5 - (kN == 8 ? 3 : 2);
@@ -1585,29 +1589,26 @@ __global__ void __launch_bounds__(kT, 2) row_kernel(const rl2_sample_args a, con
     if (size > 1) ptx::cluster_sync();  // no CTA leaves while another may read its shared memory
 }
 
+int launched(cudaError_t e) {
+    if (e == cudaSuccess) return launch_status("token sampling");
+    set_error("token sampling: %s", cudaGetErrorString(e));
+    return -1;
+}
+
 template <typename L, int N>
-void launch_warps(const rl2_sample_args& a, cudaStream_t stream) {
+int launch_warps(const rl2_sample_args& a, cudaStream_t stream) {
     const int blocks = static_cast<int>(std::min<long long>((static_cast<long long>(a.rows) + kRowWarps - 1) / kRowWarps, 148 * 16));
-    warp_kernel<L, N><<<blocks, 32 * kRowWarps, 0, stream>>>(a);
+    return launched(launch_early(warp_kernel<L, N>, blocks, 32 * kRowWarps, 0, stream, a));
 }
 
 template <typename L>
 int launch(const rl2_sample_args& a, cudaStream_t stream) {
-    if (a.vocab <= 1024) {
-        if (a.vocab <= 32)
-            launch_warps<L, 1>(a, stream);
-        else if (a.vocab <= 64)
-            launch_warps<L, 2>(a, stream);
-        else if (a.vocab <= 128)
-            launch_warps<L, 4>(a, stream);
-        else if (a.vocab <= 256)
-            launch_warps<L, 8>(a, stream);
-        else if (a.vocab <= 512)
-            launch_warps<L, 16>(a, stream);
-        else
-            launch_warps<L, 32>(a, stream);
-        return launch_status("token sampling");
-    }
+    if (a.vocab <= 32) return launch_warps<L, 1>(a, stream);
+    if (a.vocab <= 64) return launch_warps<L, 2>(a, stream);
+    if (a.vocab <= 128) return launch_warps<L, 4>(a, stream);
+    if (a.vocab <= 256) return launch_warps<L, 8>(a, stream);
+    if (a.vocab <= 512) return launch_warps<L, 16>(a, stream);
+    if (a.vocab <= 1024) return launch_warps<L, 32>(a, stream);
     // stretches of 32 vectors, or more where that gives over kStretches of them
     constexpr int kN = Reader<L>::kN;
     int shift = 5 + (kN == 8 ? 3 : 2);
@@ -1616,17 +1617,6 @@ int launch(const rl2_sample_args& a, cudaStream_t stream) {
     int size = 1;
     while (size < 8 && static_cast<long long>(a.rows) * size * 2 <= 148 && a.vocab / (2 * size) >= 4096) size *= 2;
     const long long clusters = std::min<long long>(a.rows, std::max(1, 148 * 2 / size));
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = size;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(clusters * size));
-    cfg.blockDim = dim3(kT);
-    cfg.dynamicSmemBytes = sizeof(Shared);
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
     static std::atomic<unsigned long long> allowed{0};  // devices (up to 64) whose limit is raised
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
@@ -1635,12 +1625,9 @@ int launch(const rl2_sample_args& a, cudaStream_t stream) {
                                  sizeof(Shared));
         if (e == cudaSuccess && device <= 63) allowed.fetch_or(1ull << device);
     }
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, row_kernel<L>, a, size, shift);
-    if (e != cudaSuccess) {
-        set_error("token sampling: %s", cudaGetErrorString(e));
-        return -1;
-    }
-    return launch_status("token sampling");
+    if (e == cudaSuccess)
+        e = launch_early_clusters(row_kernel<L>, size, static_cast<unsigned>(clusters * size), kT, sizeof(Shared), stream, a, size, shift);
+    return launched(e);
 }
 
 }  // namespace sample
