@@ -364,6 +364,15 @@ __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;
 // The next grid of the stream may take the SMs that this one leaves (it waits in grid_wait for this one's end).
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// 16 bytes, by a load that stays behind grid_wait. A read-only load (__ldg, or a __restrict__ const pointer) need not: it
+// may be moved ahead of the wait, and what it reads has to hold for the whole grid, which begins while the grid before
+// may still be writing it.
+__device__ __forceinline__ uint4 load_vector(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 __device__ __forceinline__ uint32_t elect_one() {
     uint32_t pred = 0;
     asm volatile(

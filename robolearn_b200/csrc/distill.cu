@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
     auto load = [&](uint4 (&to)[kHeld], int first) {
 #pragma unroll
         for (int k = 0; k < kHeld; ++k)
-            to[k] = first + k * kLong + tid < in.count ? __ldg(data + first + k * kLong) : nothing(L(0.0f));
+            to[k] = first + k * kLong + tid < in.count ? ptx::load_vector(data + first + k * kLong) : nothing(L(0.0f));
     };
     // the second pass's: from shared memory where the first kept them
     auto load_again = [&](uint4 (&to)[kHeld], int first) {

@@ -544,11 +544,11 @@ struct FewArgs {
 // 8 elements of a row from column k on where it may end before: 0 past `cols` (the rows' padding is neither data nor
 // read: the last row's need not exist)
 __device__ __forceinline__ uint4 load_end(const uint16_t* row, int k, int cols) {
-    if (k + 8 <= cols) return __ldg(reinterpret_cast<const uint4*>(row + k));
+    if (k + 8 <= cols) return ptx::load_vector(row + k);
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < 7; ++e)
-        if (k + e < cols) w[e / 2] |= static_cast<uint32_t>(__ldg(row + k + e)) << (16 * (e & 1));
+        if (k + e < cols) w[e / 2] |= static_cast<uint32_t>(row[k + e]) << (16 * (e & 1));
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -596,9 +596,9 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(const FewArgs 
         for (int s = 0; s < kAhead; ++s) {
             const int k = (step0 + min(s, n_here - 1)) * 32;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m[s][i] = __ldg(reinterpret_cast<const uint4*>(w[i] + k));
+            for (int i = 0; i < 4; ++i) m[s][i] = ptx::load_vector(w[i] + k);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) b[s][n] = __ldg(reinterpret_cast<const uint4*>(xr[n] + k));
+            for (int n = 0; n < NT; ++n) b[s][n] = ptx::load_vector(xr[n] + k);
         }
 #pragma unroll
         for (int s = 0; s < kAhead; ++s)
@@ -777,8 +777,8 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 template <typename OUT>
-__global__ void reduce_kernel(const float* __restrict__ part, const float* __restrict__ scale, int splits, int matrices, int rows, int cols, int ld_part,
-                              OUT* __restrict__ gate, long long ld_gate, OUT* __restrict__ up, long long ld_up) {
+__global__ void reduce_kernel(const float* part, const float* scale, int splits, int matrices, int rows, int cols, int ld_part,
+                              OUT* gate, long long ld_gate, OUT* up, long long ld_up) {
     ptx::grid_release();
     ptx::grid_wait();
     const int quads = (cols + 3) / 4;

@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) warp_kernel(const rl2_sample_a
 #pragma unroll
             for (int i = 0; i < N; i += kVec) {
                 L x[kVec];
-                *reinterpret_cast<uint4*>(x) = __ldg(reinterpret_cast<const uint4*>(s + i));
+                *reinterpret_cast<uint4*>(x) = ptx::load_vector(s + i);
 #pragma unroll
                 for (int k = 0; k < kVec; ++k) v[i + k] = clean(to_float(x[k]));
             }
@@ -939,7 +939,7 @@ struct Reader {
     __device__ __forceinline__ int first(int b) const { return b * kN - mis; }
     __device__ __forceinline__ bool whole(int j) const { return j >= 0 && j + kN <= vocab; }
     __device__ __forceinline__ bool inside(int b) const { return b * kN >= mis && (b + 32) * kN - mis <= vocab; }
-    __device__ __forceinline__ uint4 raw(int b) const { return __ldg(reinterpret_cast<const uint4*>(s + first(b))); }
+    __device__ __forceinline__ uint4 raw(int b) const { return ptx::load_vector(s + first(b)); }
     __device__ __forceinline__ float at(int j) const { return clean(to_float(s[j])); }
     // elements outside the row are -inf
     __device__ __forceinline__ void load(int b, float (&v)[kN]) const {
