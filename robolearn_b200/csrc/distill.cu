@@ -331,7 +331,8 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const rl2_distill_args a) 
 // 512 threads read the row (of a cluster: each CTA its part) 32 KB at a time, the next 32 KB on their way, and
 // keep the first 64 KB in shared memory; the second pass takes those from there and the rest from L2, the last
 // read first. Two CTAs an SM: one row's reading goes along with the other's writing. What bounds it is DRAM:
-// 1.05 GB in 217 us at 2047 x 128257 bf16 (4.8 TB/s of algorithmic bytes; 84% of the DRAM time was busy when the
+// 1.05 GB in 218 us at 2047 x 128257 bf16 (4.8 TB/s of algorithmic bytes; 227 in a row of calls on other inputs
+// each; 84% of the DRAM time was busy when the
 // second pass read forward and kept nothing, because two thirds of the rows had left L2 by then: 246 us).
 // Slower there: rows held in registers by clusters of four CTAs (389 us), rows streamed through a ring in
 // shared memory by bulk copies (308 us), both waiting for one another at each row.

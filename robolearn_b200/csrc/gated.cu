@@ -26,9 +26,16 @@
 // last two products read them so: as rows of the matrix, a block is 128 pieces of 128 bytes in as many DRAM pages,
 // and dx at 8192 x 512 x 2048 took 0.53 us a k-block for the 0.38 that the tensor cores take. Rows and hidden units
 // past the matrix are zeros there (the projections of zero-filled operands).
-// Warp roles as in the dense products: TMA producer, MMA issuer, eight epilogue warps on a
+// Warp roles as in the dense products: TMA producer, MMA issuer, eight or sixteen epilogue warps on a
 // double-buffered accumulator. Outputs leave through shared-memory boxes and TMA stores, which
 // clip at the output's extents. Every wait is bounded by wall-clock time.
+//
+// Two forms without these tiles, forward only: few_rows_kernel (up to 16 rows) and strip_kernel (up to 128).
+//
+// Measured: forward 65536 x 1024 x 4096 bf16 810 us (1360 TFLOP/s, the rate that the card sustains under its power
+// limit); backward 32768 x 1024 x 4096 bf16 1428 us (1155 TFLOP/s; each product alone 1180 to 1260); backward
+// 8192 x 512 x 2048 fp16 100 us: the projections and their epilogue 41 (839 TFLOP/s; the epilogue's arithmetic and the
+// 32 k-blocks or fewer of every tile bound it), dx 27, dW 33 (split over rows, then summed).
 
 #include "common.cuh"
 #include "../../include/rl2.h"
@@ -939,7 +946,8 @@ int launch(const Plan* plan, int mode, bool out32, Params& p, const Maps& maps, 
 }
 
 // Tile width: 128 B rows per CTA, or 64 where that ends sooner, by waves of tiles times a tile's cost (its width,
-// and its share of the A rows as much as 16 columns).
+// and its share of the A rows as much as 16 columns). The backward at 8192 x 512 x 2048 took 118 us with 128
+// throughout and takes 104 so.
 int width_for(const Plan* plan, long long row_tiles, long long cols, int per_row) {
     auto cost = [&](int width) {
         const long long tiles = row_tiles * ((cols + width * per_row - 1) / (width * per_row));
