@@ -301,6 +301,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
+// The same without publishing this thread's memory accesses, for a barrier that hands back a TMEM buffer whose loads
+// have completed (tcgen05.wait::ld). A release at cluster scope waits for every access of the thread that is under
+// way, bulk stores' reads of shared memory among them: 3000 cycles a tile in a product's epilogue.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
 // Tiled TMA load into this CTA's shared memory whose transaction bytes complete on an
 // mbarrier of either CTA of the pair (shared::cluster address).
 __device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y,

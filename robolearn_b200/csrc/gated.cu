@@ -63,10 +63,10 @@ enum Act { kSilu = 0, kGelu = 1, kRelu = 2 };
 // steps an element need the warps to hide them), two where it only rounds and stores.
 __host__ __device__ constexpr int epi_warps(int mode) { return mode == kForward || mode == kGate ? 16 : 8; }
 __host__ __device__ constexpr int threads_of(int mode) { return 64 + 32 * epi_warps(mode); }
-// Store boxes: 32 rows of 32 (or 16) hidden units, one a warp (kForward) or two (kGate: dh and dg, du); or of 128
-// bytes, one a warp.
+// Boxes: 32 rows of 32 (or 16) hidden units, one a warp (kForward) or three (kGate: dg, du, and dh, which is on its way
+// while the tile before is stored); or of 128 bytes, one a warp.
 __host__ __device__ constexpr int box_bytes(int mode) { return mode == kForward || mode == kGate ? 2048 : 4096; }
-__host__ __device__ constexpr int boxes_of(int mode) { return mode == kGate ? 2 : 1; }
+__host__ __device__ constexpr int boxes_of(int mode) { return mode == kGate ? 3 : 1; }
 
 struct Params {
     int b_merged;       // N-contiguous operand: one copy brings all its 64-wide chunks
@@ -328,27 +328,26 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
     const int rank = static_cast<int>(blockIdx.x & 1u);
     uint8_t* box = boxes + (warp - 2) * boxes_of(MODE) * box_bytes(MODE);
     uint8_t* box1 = box + box_bytes(MODE);
+    uint8_t* in_box = box1 + box_bytes(MODE);
     uint64_t* in_bar = in_full + (warp - 2);
     const uint32_t n = 2u * p.bnc;
     const int row_bytes = OUT32 ? 128 : p.box_cols * 2;
     const float scale = MODE == kWeight && p.scale ? *p.scale : 1.0f;
+    const int mine = kGated ? p.bnc / kSlots : 2 * p.bnc / kSlots;  // this warp's output columns
+    auto load_in = [&](int t) {  // a tile's dh, by one lane
+        const Tile w = decode(p, t);
+        ptx::mbar_arrive_expect_tx(in_bar, 32u * p.box_cols * 2u);
+        ptx::tma_load_3d(in_box, &maps.in, in_bar, w.n * p.tile_cols + slot * mine, w.m * 2 * kBM + rank * kBM + q * 32, 0);
+    };
+    if (MODE == kGate && lane == 0 && (blockIdx.x >> 1) < p.tiles_total) load_in(blockIdx.x >> 1);
     int i = 0;
     for (int t = blockIdx.x >> 1; t < p.tiles_total; t += gridDim.x >> 1, ++i) {
         const Tile w = decode(p, t);
         const int buf = i & 1;
         const int row0 = w.m * 2 * kBM + rank * kBM + q * 32;
-        const int mine = kGated ? p.bnc / kSlots : 2 * p.bnc / kSlots;  // this warp's output columns
         const int col0 = w.n * p.tile_cols + slot * mine;
-        if (MODE == kGate) {  // this tile's dh, while the products run
-            if (lane == 0) {
-                ptx::bulk_wait_read0();
-                ptx::mbar_arrive_expect_tx(in_bar, 32u * p.box_cols * 2u);
-                ptx::tma_load_3d(box, &maps.in, in_bar, col0, row0, 0);
-            }
-            __syncwarp();
-        }
         const bool ready = wait_bar(&acc_full[buf], (i >> 1) & 1, p.health, abort_flag);
-        if (MODE == kGate) {  // the copy has landed before the box (or the CTA) goes on
+        if (MODE == kGate) {  // the copy has landed before the CTA goes on (the next is not under way yet)
             const bool in = wait_bar(in_bar, i & 1, p.health, nullptr);
             if (!in || !ready) break;
         } else if (!ready) {
@@ -357,22 +356,38 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
         ptx::tc_fence_after();
         const uint32_t base = tmem + static_cast<uint32_t>(buf) * n + (static_cast<uint32_t>(q * 32) << 16);
         if (kGated) {
-            if (MODE == kForward) {
-                if (lane == 0) ptx::bulk_wait_read0();
-                __syncwarp();
+            // the accumulators, then their buffer is the next tile's
+            uint32_t gs[2][16], us[2][16];
+            ptx::tmem_ld16_issue(base + slot * mine, gs[0]);
+            ptx::tmem_ld16_issue(base + p.bnc + slot * mine, us[0]);
+            if (mine == 32) {
+                ptx::tmem_ld16_issue(base + slot * mine + 16, gs[1]);
+                ptx::tmem_ld16_issue(base + p.bnc + slot * mine + 16, us[1]);
             }
-            for (int c = 0; c < mine; c += 16) {
-                uint32_t gr[16], ur[16];
-                ptx::tmem_ld16_issue(base + slot * mine + c, gr);
-                ptx::tmem_ld16_issue(base + p.bnc + slot * mine + c, ur);
-                ptx::tmem_ld_wait(gr);
-                ptx::tmem_ld_wait(ur);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                ptx::tmem_ld_wait(gs[h]);
+                ptx::tmem_ld_wait(us[h]);
+            }
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                ptx::mbar_arrive_cluster_relaxed(ptx::cluster_addr(&acc_empty[buf], 0));
+                ptx::bulk_wait_read0();
+            }
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h == 1 && mine != 32) break;
+                const int c = 16 * h;
+                const uint32_t(&gr)[16] = gs[h];
+                const uint32_t(&ur)[16] = us[h];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t at = box_at(lane, c / 8 + e, row_bytes);
                     uint32_t o0[4], o1[4];
                     uint4 in4 = make_uint4(0, 0, 0, 0);
-                    if (MODE == kGate) in4 = *reinterpret_cast<const uint4*>(box + at);
+                    if (MODE == kGate) in4 = *reinterpret_cast<const uint4*>(in_box + at);
                     const uint32_t in[4] = {in4.x, in4.y, in4.z, in4.w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -393,12 +408,10 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
                     if (MODE == kGate) *reinterpret_cast<uint4*>(box1 + at) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
                 }
             }
-            ptx::tc_fence_before();
             if (MODE == kForward) store_tail<2>(p, box, row_bytes, p.out[0], p.ld_out[0], col0, row0, lane);
             ptx::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-                ptx::mbar_arrive_cluster(ptx::cluster_addr(&acc_empty[buf], 0));
                 if (MODE == kGate) {
                     ptx::tma_store_4d(&maps.d0, box, col0 % 64, row0 % kBM, col0 / 64, row0 / kBM);
                     ptx::tma_store_4d(&maps.d0, box1, col0 % 64, row0 % kBM, col0 / 64, row0 / kBM + p.row_blocks);
@@ -406,6 +419,7 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
                     ptx::tma_store_3d(&maps.d0, box, col0, row0, 0);
                 }
                 ptx::bulk_commit();
+                if (MODE == kGate && t + (gridDim.x >> 1) < p.tiles_total) load_in(t + (gridDim.x >> 1));
             }
         } else {
             const int z = p.splits > 1 ? (MODE == kWeight ? w.split * 2 + w.z : w.split) : 0;
@@ -416,6 +430,11 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
                 for (int e = 0; e < p.box_cols; e += 32) {
                     float r[32];
                     ptx::tmem_ld32(base + slot * mine + c + e, r);
+                    if (c + e + 32 >= mine) {  // the accumulators are read: their buffer is the next tile's
+                        ptx::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive_cluster_relaxed(ptx::cluster_addr(&acc_empty[buf], 0));
+                    }
                     if (MODE == kWeight) {
 #pragma unroll
                         for (int k = 0; k < 32; ++k) r[k] *= scale;
@@ -433,12 +452,10 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
                                            pack2<BF16>(r[8 * k + 4], r[8 * k + 5]), pack2<BF16>(r[8 * k + 6], r[8 * k + 7]));
                     }
                 }
-                if (c + p.box_cols >= mine) ptx::tc_fence_before();
                 store_tail<OUT32 ? 4 : 2>(p, box, row_bytes, w.z ? p.out[1] : p.out[0], w.z ? p.ld_out[1] : p.ld_out[0], col0 + c, row0, lane);
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    if (c + p.box_cols >= mine) ptx::mbar_arrive_cluster(ptx::cluster_addr(&acc_empty[buf], 0));
                     if (col0 + c < p.store_cols && row0 < p.out_rows) ptx::tma_store_3d(dst, box, col0 + c, row0, z);
                     ptx::bulk_commit();
                 }
