@@ -47,6 +47,29 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// two fp32 operations in one instruction, each rounded as by itself
+__device__ __forceinline__ unsigned long long pair_of(float lo, float hi) {
+    return static_cast<unsigned long long>(__float_as_uint(hi)) << 32 | __float_as_uint(lo);
+}
+__device__ __forceinline__ float2 halves_of(unsigned long long x) {
+    return make_float2(__uint_as_float(static_cast<uint32_t>(x)), __uint_as_float(static_cast<uint32_t>(x >> 32)));
+}
+__device__ __forceinline__ float2 fma_pair(float2 a, float b, float c) {
+    unsigned long long y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(pair_of(a.x, a.y)), "l"(pair_of(b, b)), "l"(pair_of(c, c)));
+    return halves_of(y);
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+    unsigned long long y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(pair_of(a.x, a.y)), "l"(pair_of(b.x, b.y)));
+    return halves_of(y);
+}
+__device__ __forceinline__ float2 mul_pair(float2 a, float b) {
+    unsigned long long y;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(pair_of(a.x, a.y)), "l"(pair_of(b, b)));
+    return halves_of(y);
+}
+
 // two values as one word of 16-bit elements, rounded to nearest
 template <typename T>
 __device__ __forceinline__ uint32_t narrow2(float lo, float hi);
@@ -571,17 +594,18 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
         const float up = fmaxf(o, m * scale);
         sum *= exp2_fast(o - up);
         o = up;
+        float2 part = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int k = 0; k < kHeld; ++k) {
-            float v[kN], part = 0.0f;
+            float v[kN];
             unpack<L>(x[k], v);
 #pragma unroll
             for (int e = 0; e < kN; e += 2) {
-                sum += exp2_fast(fmaf(v[e], scale, -o));
-                part += exp2_fast(fmaf(v[e + 1], scale, -o));
+                const float2 z = fma_pair(make_float2(v[e], v[e + 1]), scale, -o);
+                part = add_pair(part, make_float2(exp2_fast(z.x), exp2_fast(z.y)));
             }
-            sum += part;
         }
+        sum += part.x + part.y;
         if (first < kKept) {
 #pragma unroll
             for (int k = 0; k < kHeld; ++k) kept[first + k * kLong + tid] = x[k];
@@ -649,8 +673,16 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
                     float v[kN];
                     unpack<L>(x[k], v);
 #pragma unroll
-                    for (int e = 0; e < kN; ++e)
-                        v[e] = decltype(is_plain)::value ? exp2_fast(fmaf(v[e], scale, -o)) * f : (some ? grad(v[e]) : 0.0f);
+                    for (int e = 0; e < kN; e += 2) {
+                        if (decltype(is_plain)::value) {
+                            const float2 z = fma_pair(make_float2(v[e], v[e + 1]), scale, -o);
+                            const float2 y = mul_pair(make_float2(exp2_fast(z.x), exp2_fast(z.y)), f);
+                            v[e] = y.x, v[e + 1] = y.y;
+                        } else {
+                            v[e] = some ? grad(v[e]) : 0.0f;
+                            v[e + 1] = some ? grad(v[e + 1]) : 0.0f;
+                        }
+                    }
                     if (first + k * kLong + tid >= in.count) break;
                     G* to = out + (first + k * kLong) * static_cast<long long>(kN);
                     if (vec) {
