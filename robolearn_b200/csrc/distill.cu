@@ -351,12 +351,13 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const rl2_distill_args a) 
 
 // ---- long rows: a CTA each, or with few rows a cluster of CTAs ---------------------------
 //
-// 512 threads read the row (of a cluster: each CTA its part) 32 KB at a time, the next 32 KB on their way, and
-// keep the first 64 KB in shared memory; the second pass takes those from there and the rest from L2, the last
-// read first. Two CTAs an SM: one row's reading goes along with the other's writing. What bounds it is DRAM:
-// 1.05 GB in 218 us at 2047 x 128257 bf16 (4.8 TB/s of algorithmic bytes; 227 in a row of calls on other inputs
-// each; 84% of the DRAM time was busy when the
-// second pass read forward and kept nothing, because two thirds of the rows had left L2 by then: 246 us).
+// T threads read the row (of a cluster: each CTA its part) four vectors each at a time, the next four on their way,
+// and keep the first eight in shared memory; the second pass takes those from there and the rest from L2, the last read
+// first. 1024 threads an SM, so that one row's reading goes along with another's writing: 512 a CTA for the longest rows
+// and for few of them, fewer for shorter ones, whose barriers and first loads weigh more (4096 x 4096 bf16: 77 us with
+// 512, 40 with 256, 26 with 128; 2048 x 50257 bf16: 104, 87, 98; 2047 x 128257 bf16: 214, 241). What bounds it is DRAM:
+// 1.05 GB in 214 us at 2047 x 128257 bf16 (4.9 TB/s; 227 in a row of calls on other inputs each); the second pass misses
+// L2 for 0.15 of the row. 246 us when it read forward and kept nothing.
 // Slower there: rows held in registers by clusters of four CTAs (389 us), rows streamed through a ring in
 // shared memory by bulk copies (308 us), both waiting for one another at each row.
 //
@@ -369,19 +370,19 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const rl2_distill_args a) 
 // element, and the rounding of o cancels. Rows where that does not hold (no logit above -1e30, or one above
 // 1e30 after scaling, or NaN) are done again from (s - max) c.
 
-constexpr int kLong = 512;  // threads of a CTA
-constexpr int kLongWarps = kLong / 32;
+constexpr int kLongThreads = 1024;  // of an SM, in CTAs of T
 constexpr int kMaxCluster = 8;
 constexpr int kHeld = 4;                      // vectors a thread has in registers
-constexpr int kKept = 2 * kHeld * kLong;      // vectors kept in shared memory
+constexpr int kSteps = 2;                     // times that, a thread, are kept in shared memory
 constexpr float kTame = 1e30f;
 
+template <int WARPS>
 struct Meeting {
     uint64_t met[2];
     float2 meet[2][kMaxCluster];
-    float top[2][kLongWarps], sum[2][kLongWarps];
-    Running teacher[kLongWarps];
-    float loss[kLongWarps];
+    float top[2][WARPS], sum[2][WARPS];
+    Running teacher[WARPS];
+    float loss[WARPS];
 };
 
 // mbarrier that other CTAs of the cluster arrive on; bounded to 4 s (then the timeout bit of *health)
@@ -478,10 +479,11 @@ __device__ __forceinline__ void store_vector(G* to, const float (&y)[N]) {
     }
 }
 
-template <typename L, typename G>
-__global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a, const int size) {
+template <typename L, typename G, int T>
+__global__ void __launch_bounds__(T, kLongThreads / T) long_kernel(const rl2_distill_args a, const int size) {
     extern __shared__ __align__(16) uint8_t raw[];  // the row's first vectors; the teacher's entries
-    __shared__ Meeting sh;
+    constexpr int kWarps = T / 32, kKept = kSteps * kHeld * T;
+    __shared__ Meeting<kWarps> sh;
     constexpr int kN = Slice<L>::kN;
     uint4* kept = reinterpret_cast<uint4*>(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -506,14 +508,14 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
     auto load = [&](uint4 (&to)[kHeld], int first) {
 #pragma unroll
         for (int k = 0; k < kHeld; ++k)
-            to[k] = first + k * kLong + tid < in.count ? ptx::load_vector(data + first + k * kLong) : nothing(L(0.0f));
+            to[k] = first + k * T + tid < in.count ? ptx::load_vector(data + first + k * T) : nothing(L(0.0f));
     };
     // the second pass's: from shared memory where the first kept them
     auto load_again = [&](uint4 (&to)[kHeld], int first) {
         if (first < 0) return;
         if (first < kKept) {
 #pragma unroll
-            for (int k = 0; k < kHeld; ++k) to[k] = kept[first + k * kLong + tid];
+            for (int k = 0; k < kHeld; ++k) to[k] = kept[first + k * T + tid];
         } else {
             load(to, first);
         }
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
     const float edge = has_edge ? to_float(in.s[edge_at]) : -INFINITY;
     // the teacher: its softmax as a running one
     Running teacher{-INFINITY, 0.0f};
-    for (int k = tid; k < padded; k += kLong) {
+    for (int k = tid; k < padded; k += T) {
         const long long i = k < K ? teacher_index(a, row, k) : -1;
         if (i >= a.vocab && weight != 0.0f && a.health) atomicOr(a.health, kHealthIndex);
         const bool here = i >= 0 && i < a.vocab;
@@ -542,7 +544,7 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
     if (weight == 0.0f) {
         const int lo = rank == 0 ? 0 : in.head + in.from * kN, hi = static_cast<int>(rank) == size - 1 ? a.vocab : in.head + (in.from + in.count) * kN;
         if (ds)
-            for (int j = lo + tid; j < hi; j += kLong) ds[j] = narrow<G>(0.0f);
+            for (int j = lo + tid; j < hi; j += T) ds[j] = narrow<G>(0.0f);
         if (tid == 0 && rank == 0) a.row_loss[row] = 0.0f;
         return;
     }
@@ -560,9 +562,9 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
             sh.sum[buf][warp] = sum;
         }
         __syncthreads();
-        top = sh.top[buf][lane % kLongWarps];
+        top = sh.top[buf][lane % kWarps];
         all = warp_max(top);
-        sum = warp_sum(lane < kLongWarps ? sh.sum[buf][lane % kLongWarps] * relative(top, all) : 0.0f);
+        sum = warp_sum(lane < kWarps ? sh.sum[buf][lane % kWarps] * relative(top, all) : 0.0f);
         if (size > 1) {
             if (warp == 0 && lane < size) {
                 const uint32_t to = ptx::cluster_addr(&sh.meet[buf][rank], lane);
@@ -581,7 +583,7 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
     float o = fmaxf(edge * scale, -kTame);
     float sum = exp2_fast(fmaf(edge, scale, -o));  // 0 without one (-inf)
     for (int first = 0;;) {
-        const int after = first + kHeld * kLong;
+        const int after = first + kHeld * T;
         uint4 next[kHeld];
         load(next, after);  // on its way while this is worked on
         float m = -INFINITY;
@@ -608,7 +610,7 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
         sum += part.x + part.y;
         if (first < kKept) {
 #pragma unroll
-            for (int k = 0; k < kHeld; ++k) kept[first + k * kLong + tid] = x[k];
+            for (int k = 0; k < kHeld; ++k) kept[first + k * T + tid] = x[k];
         }
         first = after;
         if (first >= in.count) break;
@@ -621,20 +623,20 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
     const float2 whole = meet(o, sum, false);
     o = whole.x;
     sum = whole.y;
-    teacher = sh.teacher[lane % kLongWarps];
+    teacher = sh.teacher[lane % kWarps];
 #pragma unroll
-    for (int w = kLongWarps / 2; w; w >>= 1)
+    for (int w = kWarps / 2; w; w >>= 1)
         teacher = merge(teacher, Running{__shfl_xor_sync(0xffffffffu, teacher.max, w), __shfl_xor_sync(0xffffffffu, teacher.sum, w)}, scale);
     float base = 0.0f;
     const bool tame = o < kTame && sum > 0.0f;
     if (!tame) {  // from (s - max) c
         auto each = [&](auto&& f) {
             if (has_edge) f(edge);
-            for (int first = 0; first < in.count; first += kHeld * kLong) {
+            for (int first = 0; first < in.count; first += kHeld * T) {
                 load_again(x, first);
 #pragma unroll
                 for (int k = 0; k < kHeld; ++k) {
-                    if (first + k * kLong + tid >= in.count) continue;
+                    if (first + k * T + tid >= in.count) continue;
                     float v[kN];
                     unpack<L>(x[k], v);
 #pragma unroll
@@ -663,11 +665,11 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
         const bool vec = reinterpret_cast<uintptr_t>(out) % (sizeof(G) * kN <= 16 ? sizeof(G) * kN : 16) == 0;
         auto write = [&](auto is_plain) {
             // the last read first: they are the likeliest still in L2
-            const int last = in.count > 0 ? (in.count - 1) / (kHeld * kLong) * (kHeld * kLong) : -1;
+            const int last = in.count > 0 ? (in.count - 1) / (kHeld * T) * (kHeld * T) : -1;
             load_again(x, last);
-            for (int first = last; first >= 0; first -= kHeld * kLong) {
+            for (int first = last; first >= 0; first -= kHeld * T) {
                 uint4 next[kHeld];
-                load_again(next, first - kHeld * kLong);
+                load_again(next, first - kHeld * T);
 #pragma unroll
                 for (int k = 0; k < kHeld; ++k) {
                     float v[kN];
@@ -683,8 +685,8 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
                             v[e + 1] = some ? grad(v[e + 1]) : 0.0f;
                         }
                     }
-                    if (first + k * kLong + tid >= in.count) break;
-                    G* to = out + (first + k * kLong) * static_cast<long long>(kN);
+                    if (first + k * T + tid >= in.count) break;
+                    G* to = out + (first + k * T) * static_cast<long long>(kN);
                     if (vec) {
                         store_vector<G, kN>(to, v);
                     } else {
@@ -708,7 +710,7 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
     const int lo = rank == 0 ? 0 : in.head + in.from * kN, hi = in.head + (in.from + in.count) * kN;
     float loss = 0.0f;
     if (some) {
-        for (int k = tid; k < K; k += kLong) {
+        for (int k = tid; k < K; k += T) {
             const int i = token[k];
             const float s = k == tid || i < 0 ? own : to_float(in.s[i]);
             float q = share(k);
@@ -739,7 +741,7 @@ __global__ void __launch_bounds__(kLong, 2) long_kernel(const rl2_distill_args a
         if (lane == 0) sh.loss[warp] = loss;
         __syncthreads();
         if (warp == 0) {
-            loss = warp_sum(lane < kLongWarps ? sh.loss[lane] : 0.0f);
+            loss = warp_sum(lane < kWarps ? sh.loss[lane] : 0.0f);
             if (lane == 0) a.row_loss[row] = some ? a.temperature * a.temperature * loss : 0.0f;
         }
     }
@@ -773,31 +775,39 @@ int launched(cudaError_t e) {
     return -1;
 }
 
-template <typename L, typename G>
+template <typename L, typename G, int T>
 int launch_long(const rl2_distill_args& a, cudaStream_t stream) {
     // few rows: more CTAs a row, while each has four vectors a thread
+    constexpr int kResident = 148 * (kLongThreads / T);
     int size = 1;
-    while (size < kMaxCluster && static_cast<long long>(a.rows) * size * 2 <= 148 * 2 &&
-           a.vocab / Slice<L>::kN / (size * 2) >= kHeld * kLong)
+    while (size < kMaxCluster && static_cast<long long>(a.rows) * size * 2 <= kResident && a.vocab / Slice<L>::kN / (size * 2) >= kHeld * T)
         size *= 2;
-    constexpr int kMost = kKept * 16 + kMaxTop * 8;
+    constexpr int kMost = kSteps * kHeld * T * 16 + kMaxTop * 8;
     const size_t smem = kMost - (kMaxTop - (a.top + 3) / 4 * 4) * 8;
     static std::atomic<unsigned long long> allowed{0};  // devices (up to 64) whose limit is raised
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess && (device > 63 || !(allowed.load() >> device & 1))) {
-        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(long_kernel<L, G>), cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(long_kernel<L, G, T>), cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
         if (e == cudaSuccess && device <= 63) allowed.fetch_or(1ull << device);
     }
     if (e == cudaSuccess)
-        e = launch_early_clusters(long_kernel<L, G>, size, static_cast<unsigned>(static_cast<long long>(a.rows) * size), kLong, smem, stream, a, size);
+        e = launch_early_clusters(long_kernel<L, G, T>, size, static_cast<unsigned>(static_cast<long long>(a.rows) * size), T, smem, stream, a, size);
     if (e == cudaSuccess && a.loss_out) e = launch_early(total_kernel, 1, 1024, 0, stream, a);
     return launched(e);
 }
 
 template <typename L, typename G>
 int launch(const rl2_distill_args& a, cudaStream_t stream) {
-    if (a.vocab > 2048) return launch_long<L, G>(a, stream);
+    if (a.vocab > 2048) {
+        // more and smaller CTAs while the rows under way stay in L2 (148 x 4 of 140 KB, read and written), a row gives
+        // every thread work in each step, and the teacher has at most an entry a thread
+        const long long bytes = a.vocab * static_cast<long long>(sizeof(L));
+        const bool many = a.rows > 148 * 2;
+        if (many && bytes <= 48 << 10 && a.top <= 128) return launch_long<L, G, 128>(a, stream);
+        if (many && bytes <= 140000 && a.top <= 256) return launch_long<L, G, 256>(a, stream);
+        return launch_long<L, G, 512>(a, stream);
+    }
     // short rows: the total by the last CTA, or with many rows (whose losses one small CTA takes long to add: 22 us
     // for 6 + 3 at 4096 x 101) by a launch of its own
     rl2_distill_args each = a;
