@@ -7,8 +7,8 @@
 //   ds_j     = c w_n T (p_j - sum_{k: i_k = j} q_k) (* *grad_scale)
 //
 // A row is read from memory once and stays on the chip between its two passes (running maximum and
-// sum of the softmax; gradient): in L1 behind a warp (up to 1024 tokens) or a CTA (up to
-// 2048), and above that in shared memory and L2 (long_kernel). All sums
+// sum of the softmax; gradient): in a warp's registers (up to 256 tokens, 1024 of fp32), in L1 behind a
+// warp (up to 1024) or a CTA (up to 2048), and above that in shared memory and L2 (long_kernel). All sums
 // are fp32; exponentials are the hardware's exp2 of s log2(e) / T less the same of the maximum, so every
 // value is within a few units in the last place of fp32 times 1 + its argument.
 
