@@ -103,6 +103,23 @@ def test_types_of_the_gradient(dtype, grad, vocab):
     run(*inputs(13, vocab, 20, dtype, index=torch.int32, values_dtype=torch.float32), temperature=2.5, grad=grad, scale=64.0)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,top", [(297, 2049, 128), (310, 6144, 100), (300, 12301, 129), (301, 24001, 256), (299, 34990, 7),
+                                            (300, 36000, 300), (1030, 3001, 12), (1100, 700, 20), (1201, 255, 40)])
+def test_many_rows(rows, vocab, top, dtype):
+    """Rows enough for every split of long rows over CTAs; absent and repeated entries, rows without weight, half of the
+    tokens that are not the teacher's masked."""
+    student, values, indices, weight = inputs(rows, vocab, top, dtype, seed=vocab)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    masked = torch.rand(rows, vocab, generator=gen, device="cuda") < 0.5
+    masked.scatter_(1, indices, False)
+    student = student.masked_fill(masked, -INF)
+    indices = torch.where(torch.rand(rows, top, generator=gen, device="cuda") < 0.1, -1, indices)
+    indices[:, top // 2] = indices[:, 0]
+    weight = torch.where(torch.rand(rows, generator=gen, device="cuda") < 0.1, 0.0, weight)
+    run(student, values, indices, weight, temperature=1.7, grad=torch.float32 if dtype == torch.bfloat16 else None)
+
+
 @pytest.mark.parametrize("vocab", [60, 3000, 70000])
 def test_absent_repeated_and_weightless(vocab):
     s, v, i, w = inputs(16, vocab, 12, torch.float32, seed=3)
