@@ -871,7 +871,9 @@ int rl2_peer_mean(long long count, const rl2_syncbn_exchange* ex, void* stream);
  * grad_x may be null, and grad_gate with grad_up; gradients are assigned, not added.
  * grad_weight_fp32: the weight gradients are fp32 (row strides in floats, multiples of
  * 4). grad_weight_scale (a device float, optional) multiplies them before they are
- * rounded: the inverse of the loss scale that grad_out carries. workspace:
+ * rounded: the inverse of the loss scale that grad_out carries. *found_inf (optional) becomes
+ * 1 where a value of dg, du or a gradient is not finite in the type that it is rounded to
+ * (else it is left as it is); without it that sets the overflow bit of *health. workspace:
  * rl2_gated_workspace_bytes(plan) bytes, 256-byte aligned, free to use
  * again after the call's work. rows = 0 is allowed (zero weight gradients).
  * ------------------------------------------------------------------------- */
@@ -913,6 +915,7 @@ typedef struct rl2_gated_backward_args {
     const float* grad_weight_scale;
     void* workspace;
     int* health;
+    int* found_inf;
 } rl2_gated_backward_args;
 
 void* rl2_gated_create(const rl2_gated_desc* desc);

@@ -452,7 +452,7 @@ class GatedBackwardArgs(ctypes.Structure):
         ("rows", I), ("x", P), ("ldx", LL), ("gate_weight", P), ("ld_gate", LL), ("up_weight", P), ("ld_up", LL),
         ("grad_out", P), ("ld_grad_out", LL), ("grad_x", P), ("ld_grad_x", LL), ("grad_gate", P),
         ("ld_grad_gate", LL), ("grad_up", P), ("ld_grad_up", LL), ("grad_weight_fp32", I), ("grad_weight_scale", P), ("workspace", P),
-        ("health", P),
+        ("health", P), ("found_inf", P),
     ]
 
 

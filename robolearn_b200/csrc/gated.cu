@@ -46,6 +46,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <initializer_list>
 #include <new>
 
@@ -87,6 +88,7 @@ struct Params {
     long long ld_out[2];
     const float* scale; // kWeight, not split: multiplies the output
     int* health;
+    int* found_inf;     // the backward's: a rounded value is not finite (see Rounded)
 };
 
 struct Maps {
@@ -134,6 +136,34 @@ template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
     if (BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Whether all 16-bit words that a thread has rounded are finite: their largest magnitude, in which a NaN stays (two
+// instructions a word).
+template <bool BF16>
+struct Rounded {
+    uint32_t most = 0;
+    __device__ __forceinline__ void add(uint32_t w) {
+        if (BF16) {
+            const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&most), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w)));
+            most = *reinterpret_cast<const uint32_t*>(&m);
+        } else {
+            const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2*>(&most), __habs2(*reinterpret_cast<const __half2*>(&w)));
+            most = *reinterpret_cast<const uint32_t*>(&m);
+        }
+    }
+    __device__ __forceinline__ bool finite() const {
+        constexpr uint32_t kInf = BF16 ? 0x7F80u : 0x7C00u;
+        return (most & 0xFFFFu) < kInf && (most >> 16) < kInf;
+    }
+};
+
+// A step whose gradients are not finite: *found_inf, or without one the overflow bit of *health.
+__device__ __forceinline__ void report_overflow(int* found_inf, int* health) {
+    if (found_inf)
+        atomicOr(found_inf, 1);
+    else if (health)
+        atomicOr(health, kHealthOverflow);
 }
 
 // act(g) and act'(g). The exponential and the division are the fast fp32 forms (a few units in
@@ -342,6 +372,9 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
         ptx::tma_load_3d(in_box, &maps.in, in_bar, w.n * p.tile_cols + slot * mine, w.m * 2 * kBM + rank * kBM + q * 32, 0);
     };
     if (MODE == kGate && lane == 0 && (blockIdx.x >> 1) < p.tiles_total) load_in(blockIdx.x >> 1);
+    // Rounded values past the matrices are zeros (so are the operands there), or NaN where an operand within is not finite.
+    Rounded<BF16> rounded;
+    bool over = false;
     int i = 0;
     for (int t = blockIdx.x >> 1; t < p.tiles_total; t += gridDim.x >> 1, ++i) {
         const Tile w = decode(p, t);
@@ -404,6 +437,8 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
                             act_both<ACT>(g1, a1, s1);
                             o0[k] = pack2<BF16>(dh.x * u0 * s0, dh.y * u1 * s1);
                             o1[k] = pack2<BF16>(dh.x * a0, dh.y * a1);
+                            rounded.add(o0[k]);
+                            rounded.add(o1[k]);
                         }
                     }
                     *reinterpret_cast<uint4*>(box + at) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
@@ -442,16 +477,22 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
                         for (int k = 0; k < 32; ++k) r[k] *= scale;
                     }
                     if (OUT32) {
+                        if (p.splits == 1) {  // else partial sums: the reduction reports
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) over |= !(fabsf(r[k]) <= FLT_MAX);
+                        }
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
                             *reinterpret_cast<float4*>(box + box_at(lane, e / 4 + k, 128)) =
                                 make_float4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
                     } else {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            *reinterpret_cast<uint4*>(box + box_at(lane, e / 8 + k, row_bytes)) =
-                                make_uint4(pack2<BF16>(r[8 * k], r[8 * k + 1]), pack2<BF16>(r[8 * k + 2], r[8 * k + 3]),
-                                           pack2<BF16>(r[8 * k + 4], r[8 * k + 5]), pack2<BF16>(r[8 * k + 6], r[8 * k + 7]));
+                        for (int k = 0; k < 4; ++k) {
+                            const uint4 o = make_uint4(pack2<BF16>(r[8 * k], r[8 * k + 1]), pack2<BF16>(r[8 * k + 2], r[8 * k + 3]),
+                                                       pack2<BF16>(r[8 * k + 4], r[8 * k + 5]), pack2<BF16>(r[8 * k + 6], r[8 * k + 7]));
+                            for (uint32_t w : {o.x, o.y, o.z, o.w}) rounded.add(w);
+                            *reinterpret_cast<uint4*>(box + box_at(lane, e / 8 + k, row_bytes)) = o;
+                        }
                     }
                 }
                 store_tail<OUT32 ? 4 : 2>(p, box, row_bytes, w.z ? p.out[1] : p.out[0], w.z ? p.ld_out[1] : p.ld_out[0], col0 + c, row0, lane);
@@ -464,6 +505,7 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
             }
         }
     }
+    if (MODE != kForward && (over || !rounded.finite())) report_overflow(p.found_inf, p.health);
     if (lane == 0) ptx::bulk_wait0();
 }
 
@@ -804,13 +846,19 @@ __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return
 
 template <typename OUT>
 __global__ void reduce_kernel(const float* part, const float* scale, int splits, int matrices, int rows, int cols, int ld_part,
-                              OUT* gate, long long ld_gate, OUT* up, long long ld_up) {
+                              OUT* gate, long long ld_gate, OUT* up, long long ld_up, int* found_inf, int* health) {
     ptx::grid_release();
     ptx::grid_wait();
     const int quads = (cols + 3) / 4;
     const long long per = static_cast<long long>(rows) * quads;
     const long long plane = static_cast<long long>(rows) * ld_part;
     const float factor = scale ? *scale : 1.0f;
+    bool over = false;
+    auto rounded = [&](float v) {
+        const OUT y = narrow<OUT>(v);
+        over |= !(fabsf(static_cast<float>(y)) <= FLT_MAX);
+        return y;
+    };
     for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < matrices * per;
          i += static_cast<long long>(gridDim.x) * blockDim.x) {
         const int z = i >= per;
@@ -828,11 +876,12 @@ __global__ void reduce_kernel(const float* part, const float* scale, int splits,
             sum.w += v.w;
         }
         OUT* dst = (z ? up + row * ld_up : gate + row * ld_gate) + col;
-        dst[0] = narrow<OUT>(sum.x * factor);
-        if (col + 1 < cols) dst[1] = narrow<OUT>(sum.y * factor);
-        if (col + 2 < cols) dst[2] = narrow<OUT>(sum.z * factor);
-        if (col + 3 < cols) dst[3] = narrow<OUT>(sum.w * factor);
+        dst[0] = rounded(sum.x * factor);
+        if (col + 1 < cols) dst[1] = rounded(sum.y * factor);
+        if (col + 2 < cols) dst[2] = rounded(sum.z * factor);
+        if (col + 3 < cols) dst[3] = rounded(sum.w * factor);
     }
+    if (over) report_overflow(found_inf, health);
 }
 
 // ---- host ---------------------------------------------------------------------
@@ -1030,7 +1079,7 @@ bool ready(const Plan* plan, int rows) {
 
 // The two projections: forward (out = h) or backward (grad_out in, dg and du out).
 int project(const Plan* plan, int rows, const void* x, long long ldx, const void* wg, long long ldg, const void* wu,
-            long long ldu, const void* grad_out, long long ld_grad, void* out, long long ld_out, int* health,
+            long long ldu, const void* grad_out, long long ld_grad, void* out, long long ld_out, int* found_inf, int* health,
             cudaStream_t stream) {
     const int K = plan->features, F = plan->hidden;
     const CUtensorMapDataType type = plan->bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -1049,6 +1098,7 @@ int project(const Plan* plan, int rows, const void* x, long long ldx, const void
     p.row_blocks = row_blocks(rows);
     p.out[0] = out;
     p.ld_out[0] = ld_out;
+    p.found_inf = found_inf;
     p.health = health;
     Maps maps;
     if (!make_map(&maps.a, "x", type, x, K, rows, 1, ldx, ldx * rows, kBK, kBM) ||
@@ -1065,17 +1115,17 @@ int project(const Plan* plan, int rows, const void* x, long long ldx, const void
 
 template <typename OUT>
 cudaError_t reduce_as(const float* part, const float* scale, int splits, int matrices, int rows, int cols, int ld, void* first, long long ld_first,
-               void* second, long long ld_second, cudaStream_t stream) {
+               void* second, long long ld_second, int* found_inf, int* health, cudaStream_t stream) {
     const long long quads = static_cast<long long>(matrices) * rows * ((cols + 3) / 4);
     const int blocks = static_cast<int>(std::min<long long>((quads + 255) / 256, 148 * 8));
     return launch_early(reduce_kernel<OUT>, blocks, 256, 0, stream, part, scale, splits, matrices, rows, cols, ld, static_cast<OUT*>(first),
-                        ld_first, static_cast<OUT*>(second), ld_second);
+                        ld_first, static_cast<OUT*>(second), ld_second, found_inf, health);
 }
 
 int reduce(const Plan* plan, bool fp32, const float* part, const float* scale, int splits, int matrices, int rows, int cols, int ld, void* first,
-           long long ld_first, void* second, long long ld_second, cudaStream_t stream) {
+           long long ld_first, void* second, long long ld_second, int* found_inf, int* health, cudaStream_t stream) {
     const auto run = fp32 ? reduce_as<float> : plan->bf16 ? reduce_as<__nv_bfloat16> : reduce_as<__half>;
-    return launched(run(part, scale, splits, matrices, rows, cols, ld, first, ld_first, second, ld_second, stream));
+    return launched(run(part, scale, splits, matrices, rows, cols, ld, first, ld_first, second, ld_second, found_inf, health, stream));
 }
 
 // 17 to 128 rows, forward. Device time for that of the 256-row tiles: 15.0 us for 20.3 (32 rows) and 17.5 for 22.2
@@ -1148,6 +1198,7 @@ int input_gradient(const Plan* plan, const rl2_gated_backward_args* g, cudaStrea
     p.store_cols = split ? K : K / 8 * 8;
     p.out[0] = g->grad_x;
     p.ld_out[0] = g->ld_grad_x;
+    p.found_inf = g->found_inf;
     p.health = g->health;
     Maps maps;
     if (!make_block_map(&maps.a, type, g->workspace, hidden_blocks(plan, rows), p.row_blocks, 64, kBM, 1) ||
@@ -1158,7 +1209,7 @@ int input_gradient(const Plan* plan, const rl2_gated_backward_args* g, cudaStrea
         return -1;
     maps.d1 = maps.in = maps.d0;
     if (launch(plan, kInput, split, p, maps, stream)) return -1;
-    return split ? reduce(plan, false, part, nullptr, p.splits, 1, rows, K, static_cast<int>(ldp), g->grad_x, g->ld_grad_x, nullptr, 0, stream) : 0;
+    return split ? reduce(plan, false, part, nullptr, p.splits, 1, rows, K, static_cast<int>(ldp), g->grad_x, g->ld_grad_x, nullptr, 0, g->found_inf, g->health, stream) : 0;
 }
 
 
@@ -1179,6 +1230,7 @@ int weight_gradients(const Plan* plan, const rl2_gated_backward_args* g, cudaStr
     p.tiles_n = (K + p.tile_cols - 1) / p.tile_cols;
     p.out_rows = F;
     p.out_cols = K;
+    p.found_inf = g->found_inf;
     p.health = g->health;
     float* part = reinterpret_cast<float*>(static_cast<char*>(g->workspace) + gate_bytes(plan));
     const bool out32 = p.splits > 1 || g->grad_weight_fp32;
@@ -1209,7 +1261,7 @@ int weight_gradients(const Plan* plan, const rl2_gated_backward_args* g, cudaStr
     if (launch(plan, kWeight, out32, p, maps, stream)) return -1;
     if (p.splits == 1) return 0;
     return reduce(plan, g->grad_weight_fp32, part, g->grad_weight_scale, p.splits, 2, F, K, static_cast<int>(ldp), g->grad_gate,
-                  g->ld_grad_gate, g->grad_up, g->ld_grad_up, stream);
+                  g->ld_grad_gate, g->grad_up, g->ld_grad_up, g->found_inf, g->health, stream);
 }
 
 }  // namespace gated
@@ -1308,7 +1360,7 @@ extern "C" int rl2_gated_forward(void* opaque, const rl2_gated_forward_args* g, 
     }
     if (g->rows <= kStripRows) return launch_strip(plan, g, as_stream(stream));
     return project(plan, g->rows, g->x, g->ldx, g->gate_weight, g->ld_gate, g->up_weight, g->ld_up, nullptr, 0, g->out,
-                   g->ld_out, g->health, as_stream(stream));
+                   g->ld_out, nullptr, g->health, as_stream(stream));
 }
 
 extern "C" int rl2_gated_backward(void* opaque, const rl2_gated_backward_args* g, void* stream) {
@@ -1353,7 +1405,7 @@ extern "C" int rl2_gated_backward(void* opaque, const rl2_gated_backward_args* g
         return -1;
     }
     if (project(plan, g->rows, g->x, g->ldx, g->gate_weight, g->ld_gate, g->up_weight, g->ld_up, g->grad_out,
-                g->ld_grad_out, g->workspace, 0, g->health, s))
+                g->ld_grad_out, g->workspace, 0, g->found_inf, g->health, s))
         return -1;
     if (g->grad_x && input_gradient(plan, g, s)) return -1;
     return weights ? weight_gradients(plan, g, s) : 0;

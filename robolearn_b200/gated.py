@@ -68,10 +68,11 @@ class GatedMLP:
                 "gated MLP forward")
 
     def backward(self, *, x, gate_weight, up_weight, grad_out, grad_x=None, grad_gate=None, grad_up=None,
-                 grad_weight_scale=None, health=None, stream=None) -> None:
+                 grad_weight_scale=None, found_inf=None, health=None, stream=None) -> None:
         """Gradients of ``sum(out * grad_out)``: ``grad_x`` (optional) in the operand type, ``grad_gate`` and
         ``grad_up`` (both or neither) in the operand type or both fp32, times ``grad_weight_scale`` (one device
-        float, optional: the inverse loss scale). They are assigned."""
+        float, optional: the inverse loss scale). They are assigned. ``found_inf`` (one device int32, optional) becomes
+        1 where one of them, or a hidden gradient on the way, overflows its type or is not a number."""
         rows, K, F = x.shape[0], self.features, self.hidden
         m = self._matrix
         if (grad_gate is None) != (grad_up is None):
@@ -90,6 +91,8 @@ class GatedMLP:
             a.grad_weight_fp32 = int(types[0] == torch.float32)
             if grad_weight_scale is not None:
                 a.grad_weight_scale = N.vector("grad_weight_scale", grad_weight_scale, 1, torch.float32, self.device)
+        if found_inf is not None:
+            a.found_inf = N.vector("found_inf", found_inf, 1, torch.int32, self.device)
         if stream is not None:  # the workspace is the current stream's; this call's work on it is another's
             self._workspace.record_stream(stream)
         N.check(self._lib.rl2_gated_backward(self.handle, ctypes.byref(a), N.raw_stream(stream, self.device.index)), "gated MLP backward")

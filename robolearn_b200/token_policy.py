@@ -139,7 +139,8 @@ class TokenPolicy:
     def _run_gated_backward(self):
         self.gated.backward(x=self._h0[:, :self.hidden], grad_out=self._dgated, grad_x=self._dx[:, :self.hidden],
                             grad_gate=self.weights["gate"].arena(self.grads), grad_up=self.weights["up"].arena(self.grads),
-                            grad_weight_scale=self.inverse_scale, health=self.health, **self._gated_weights())
+                            grad_weight_scale=self.inverse_scale, found_inf=self.found_inf, health=self.health,
+                            **self._gated_weights())
 
     def _adam(self, learning_rate: float):
         prepare = N.AdamPrepareArgs(state=self.opt_state.data_ptr(), found_inf=self.found_inf.data_ptr(), formula=0, beta1=0.9,
