@@ -289,6 +289,11 @@ __device__ __forceinline__ void row_by_group(const rl2_distill_args& a, long lon
     sync();
 }
 
+// A row's part of the total. The loss weight goes in first: a mean of large losses does not overflow on the way.
+__device__ __forceinline__ float weighted(const rl2_distill_args& a, float w, float loss) {
+    return w != 0.0f ? a.loss_weight * w * loss : 0.0f;
+}
+
 // The last CTA to finish adds the rows' losses in a fixed order (all threads of the CTA).
 __device__ __forceinline__ void finish(const rl2_distill_args& a) {
     __shared__ bool last;
@@ -305,7 +310,7 @@ __device__ __forceinline__ void finish(const rl2_distill_args& a) {
 #pragma unroll 8
     for (int n = tid; n < a.rows; n += threads) {
         const float w = a.row_weight ? a.row_weight[n] : 1.0f, loss = __ldcg(a.row_loss + n);
-        sum += w != 0.0f ? w * loss : 0.0f;
+        sum += weighted(a, w, loss);
     }
     sum = warp_sum(sum);
     if ((tid & 31) == 0) part[tid >> 5] = sum;
@@ -313,7 +318,7 @@ __device__ __forceinline__ void finish(const rl2_distill_args& a) {
     if (tid < 32) {
         sum = warp_sum(tid < threads / 32 ? part[tid] : 0.0f);
         if (tid == 0) {
-            *a.loss_out = a.loss_weight * sum;
+            *a.loss_out = sum;
             *a.counter = 0;
         }
     }
@@ -892,14 +897,14 @@ __global__ void __launch_bounds__(1024) total_kernel(const rl2_distill_args a) {
 #pragma unroll 4
     for (int n = tid; n < a.rows; n += 1024) {
         const float w = a.row_weight ? a.row_weight[n] : 1.0f, loss = a.row_loss[n];
-        sum += w != 0.0f ? w * loss : 0.0f;
+        sum += weighted(a, w, loss);
     }
     sum = warp_sum(sum);
     if ((tid & 31) == 0) part[tid >> 5] = sum;
     __syncthreads();
     if (tid < 32) {
         sum = warp_sum(part[tid]);
-        if (tid == 0) *a.loss_out = a.loss_weight * sum;
+        if (tid == 0) *a.loss_out = sum;
     }
 }
 
