@@ -506,14 +506,16 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const rl2_distill_args a) 
 // one thread's each.
 //
 // The passes use the offset o = max log2(e) / T: p = 2^(s c - o) / sum needs one multiply-add and one exp2 an
-// element, and the rounding of o cancels. Rows where that does not hold (no logit above -1e30, or one above
-// 1e30 after scaling, or NaN) are done again from (s - max) c.
+// element. o is rounded, the product in the multiply-add is not, so every exponent carries the same error of up to
+// half a unit in o's last place, which the division by the sum takes out as long as 2 to that error is an ordinary
+// number: while |o| < 2^24 it is at most a factor of sqrt 2. Rows whose maximum lies outside (a mask's large finite fill; no
+// logit that is not -inf), or with NaN, are done again from (s - max) c.
 
 constexpr int kLongThreads = 1024;  // of an SM, in CTAs of T
 constexpr int kMaxCluster = 8;
 constexpr int kHeld = 4;                      // vectors a thread has in registers
 constexpr int kSteps = 2;                     // times that, a thread, are kept in shared memory
-constexpr float kTame = 1e30f;
+constexpr float kTame = 16777216.0f;  // 2^24
 
 template <int WARPS>
 struct Meeting {
@@ -767,7 +769,7 @@ __global__ void __launch_bounds__(T, kLongThreads / T) long_kernel(const rl2_dis
     for (int w = kWarps / 2; w; w >>= 1)
         teacher = merge(teacher, Running{__shfl_xor_sync(0xffffffffu, teacher.max, w), __shfl_xor_sync(0xffffffffu, teacher.sum, w)}, scale);
     float base = 0.0f;
-    const bool tame = o < kTame && sum > 0.0f;
+    const bool tame = fabsf(o) < kTame && sum > 0.0f;  // at -kTame nothing is above it
     if (!tame) {  // from (s - max) c
         auto each = [&](auto&& f) {
             if (has_edge) f(edge);
