@@ -941,7 +941,8 @@ int rl2_gated_backward(void* plan, const rl2_gated_backward_args* args, void* st
  * and alignment (16-byte aligned rows, or logits and gradient rows equally misaligned, are
  * fastest). dlogits, grad_scale (a device float: the loss scale of fp16 gradients),
  * row_weight, loss_out and health may be null. counter: one zero-initialised unsigned int
- * that the kernel leaves at zero; calls that overlap need one each.
+ * that the kernel leaves at zero; calls that overlap need one each. Buffers and stream are
+ * the current device's.
  * ------------------------------------------------------------------------- */
 typedef struct rl2_distill_args {
     int rows, vocab, top;
@@ -986,7 +987,8 @@ int rl2_distill_topk(const rl2_distill_args* args, void* stream);
  * counts as 0, one at or above 1 as just below it.
  * Scalars apply to all rows; temperatures, top_ks, top_ps and min_ps (device arrays
  * [rows], each optional) replace them. Logits: 0 = fp32, 1 = fp16, 2 = bf16, contiguous
- * rows of 1..2^20 tokens, any row stride and alignment.
+ * rows of 1..2^20 tokens, any row stride and alignment. Buffers and stream are the current
+ * device's.
  * ------------------------------------------------------------------------- */
 typedef struct rl2_sample_args {
     int rows, vocab;

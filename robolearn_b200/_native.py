@@ -270,12 +270,19 @@ def stream_ptr(stream=None) -> int:
 
 def raw_stream(stream, device_index: int) -> int:
     """Address of ``stream``, or of the current stream of a device (without building a Stream object: about
-    3 us less a call than ``stream_ptr``)."""
-    if stream is not None:
-        return stream.cuda_stream
+    3 us less a call than ``stream_ptr``). A launch goes to the current device: if that is another than the
+    operator's, or the stream another device's, the call is refused."""
     import torch
 
-    return torch._C._cuda_getCurrentRawStream(device_index)
+    c = torch._C
+    if c._cuda_getDevice() != device_index:
+        raise ValueError(f"the operator and its tensors are on cuda:{device_index}, the current device is "
+                         f"cuda:{c._cuda_getDevice()}: call it under torch.cuda.device()")
+    if stream is None:
+        return c._cuda_getCurrentRawStream(device_index)
+    if stream.device_index != device_index:
+        raise ValueError(f"the stream must be of cuda:{device_index}, got one of cuda:{stream.device_index}")
+    return stream.cuda_stream
 
 
 def matrix(name: str, t, rows: int, cols: int, types, device) -> tuple[int, int]:

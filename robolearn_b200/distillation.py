@@ -53,7 +53,8 @@ class TopKDistillation:
             a.dlogits, a.ld_dlogits, a.dlogits_dtype = self._matrix("dlogits", dlogits, n, self.vocab, DTYPES)
         if grad_scale is not None:
             a.grad_scale = self._vector("grad_scale", grad_scale, 1)
+        to = N.raw_stream(stream, self.device.index)
         if stream is not None:  # these are the current stream's; this call's work on them is another's
             self.counter.record_stream(stream)
             self.row_loss.record_stream(stream)
-        N.check(self._lib.rl2_distill_topk(ctypes.byref(a), N.raw_stream(stream, self.device.index)), "distillation objective")
+        N.check(self._lib.rl2_distill_topk(ctypes.byref(a), to), "distillation objective")

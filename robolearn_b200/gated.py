@@ -93,9 +93,10 @@ class GatedMLP:
                 a.grad_weight_scale = N.vector("grad_weight_scale", grad_weight_scale, 1, torch.float32, self.device)
         if found_inf is not None:
             a.found_inf = N.vector("found_inf", found_inf, 1, torch.int32, self.device)
+        to = N.raw_stream(stream, self.device.index)
         if stream is not None:  # the workspace is the current stream's; this call's work on it is another's
             self._workspace.record_stream(stream)
-        N.check(self._lib.rl2_gated_backward(self.handle, ctypes.byref(a), N.raw_stream(stream, self.device.index)), "gated MLP backward")
+        N.check(self._lib.rl2_gated_backward(self.handle, ctypes.byref(a), to), "gated MLP backward")
 
     def close(self) -> None:
         if self.handle:
