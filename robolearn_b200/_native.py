@@ -285,6 +285,33 @@ def raw_stream(stream, device_index: int) -> int:
     return stream.cuda_stream
 
 
+class Buffers:
+    """Device buffers that an operator keeps, made by the current stream and used by calls on any. Two things follow from
+    the caching allocator, which orders memory by the stream that it was made on: a call elsewhere must not start before
+    that stream is done with what it has under way there (the fill of a new buffer; an earlier owner's work on the
+    memory), so the host waits for it once, here; and the memory must not go to a new owner while another stream still
+    works on it, so every stream is recorded at its first use. In a CUDA graph's capture there is nothing to wait for (the
+    memory is the graph's); the operator is kept for as long as the graph is."""
+
+    def __init__(self, device, *tensors):
+        import torch
+
+        self.device, self.tensors = device, tensors
+        stream = torch.cuda.current_stream(device)
+        if not torch.cuda.is_current_stream_capturing():
+            stream.synchronize()
+        self.streams = {stream.cuda_stream}
+
+    def use(self, address: int, stream) -> None:
+        """A call on ``stream`` (None: the current one), whose address is given."""
+        if address not in self.streams:
+            import torch
+
+            for t in self.tensors:
+                t.record_stream(torch.cuda.current_stream(self.device) if stream is None else stream)
+            self.streams.add(address)
+
+
 def matrix(name: str, t, rows: int, cols: int, types, device) -> tuple[int, int]:
     """Address and row stride (elements) of a [rows, cols] matrix with contiguous rows on ``device``, of one of
     ``types``; anything else is refused. A single row's stride is its own length."""

@@ -25,6 +25,7 @@ class TopKDistillation:
         self.row_loss = torch.zeros(self.rows, device=device)
         self.device = self.counter.device
         self._counter = self.counter.data_ptr()
+        self._buffers = N.Buffers(self.device, self.counter, self.row_loss)
 
     def _matrix(self, name, t, rows, cols, types):
         return *N.matrix(name, t, rows, cols, types, self.device), types[t.dtype]
@@ -54,7 +55,5 @@ class TopKDistillation:
         if grad_scale is not None:
             a.grad_scale = self._vector("grad_scale", grad_scale, 1)
         to = N.raw_stream(stream, self.device.index)
-        if stream is not None:  # these are the current stream's; this call's work on them is another's
-            self.counter.record_stream(stream)
-            self.row_loss.record_stream(stream)
+        self._buffers.use(to, stream)
         N.check(self._lib.rl2_distill_topk(ctypes.byref(a), to), "distillation objective")

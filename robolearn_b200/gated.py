@@ -55,6 +55,7 @@ class GatedMLP:
         """The backward's workspace (allocate it here before capturing a CUDA graph)."""
         if self._workspace is None:
             self._workspace = torch.empty(self.workspace_bytes(), dtype=torch.uint8, device=self.device)
+            self._buffers = N.Buffers(self.device, self._workspace)
         return self._workspace
 
     def forward(self, *, x, gate_weight, up_weight, out, health=None, stream=None) -> None:
@@ -94,8 +95,7 @@ class GatedMLP:
         if found_inf is not None:
             a.found_inf = N.vector("found_inf", found_inf, 1, torch.int32, self.device)
         to = N.raw_stream(stream, self.device.index)
-        if stream is not None:  # the workspace is the current stream's; this call's work on it is another's
-            self._workspace.record_stream(stream)
+        self._buffers.use(to, stream)
         N.check(self._lib.rl2_gated_backward(self.handle, ctypes.byref(a), to), "gated MLP backward")
 
     def close(self) -> None:
