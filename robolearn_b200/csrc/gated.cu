@@ -166,12 +166,37 @@ __device__ __forceinline__ void report_overflow(int* found_inf, int* health) {
         atomicOr(health, kHealthOverflow);
 }
 
+// The normal distribution function Phi(g), and exp(-g^2 / 2), which its density shares. Phi(-|g|) is taken itself, not as
+// what 1 leaves: exp(-g^2 / 2) t P(t) with t = 1 / (1 + 0.3 |g|), the form of Hastings (Abramowitz and Stegun 7.1.26), P
+// fitted here to erfcx(|g| / sqrt 2) / 2 over 0 .. 13.4 in the relative error: 1.3e-7, 4e-7 with the roundings. The
+// exponent's rounding adds g^2 2^-24. So the lower tail keeps its digits down to g = -13 (1e-38), where a form with 1 + erf has
+// lost 4% at -5 and all at -6. 8192 x 512 x 2048 forward: 33 us with that form, 50 with the library's erfcf, which has too many steps for
+// an epilogue.
+__device__ __forceinline__ float normal_cdf(float g, float& bell) {
+    const float z = fabsf(g), t = __fdividef(1.0f, fmaf(0.3f, z, 1.0f));
+    float s = 0.0359838195f;
+    s = fmaf(s, t, -0.158493891f);
+    s = fmaf(s, t, 0.208583847f);
+    s = fmaf(s, t, -0.0557430983f);
+    s = fmaf(s, t, 0.129655257f);
+    s = fmaf(s, t, 0.0995806456f);
+    s = fmaf(s, t, 0.120807566f);
+    s = fmaf(s, t, 0.119625784f);
+    bell = __expf(-0.5f * g * g);
+    const float tail = bell * (s * t);
+    return g < 0.0f ? tail : 1.0f - tail;
+}
+
 // act(g) and act'(g). The exponential and the division are the fast fp32 forms (a few units in
-// the last place of fp32): the result is rounded to 16 bits, 2^13 to 2^16 times coarser.
+// the last place of fp32): the result is rounded to 16 bits, 2^13 to 2^16 times coarser. SiLU and its slope are 0 below -87
+// (1e-36), where the exponential leaves fp32.
 template <int ACT>
 __device__ __forceinline__ float act_value(float g) {
     if (ACT == kSilu) return __fdividef(g, 1.0f + __expf(-g));
-    if (ACT == kGelu) return 0.5f * g * (1.0f + erff(g * 0.70710678f));
+    if (ACT == kGelu) {
+        float bell;
+        return g * normal_cdf(g, bell);
+    }
     return g > 0.0f ? g : (g == g ? 0.0f : g);
 }
 
@@ -182,9 +207,10 @@ __device__ __forceinline__ void act_both(float g, float& value, float& slope) {
         value = g * s;
         slope = s * (1.0f + g * (1.0f - s));
     } else if (ACT == kGelu) {
-        const float cdf = 0.5f * (1.0f + erff(g * 0.70710678f));
+        float bell;
+        const float cdf = normal_cdf(g, bell);
         value = g * cdf;
-        slope = cdf + g * 0.39894228f * __expf(-0.5f * g * g);
+        slope = fmaf(g * 0.39894228f, bell, cdf);
     } else {
         value = g > 0.0f ? g : (g == g ? 0.0f : g);
         slope = g > 0.0f ? 1.0f : 0.0f;
