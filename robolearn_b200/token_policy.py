@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _native as N
-from .dense import FP16, DensePlan, operand_ld
+from .dense import FP16, TF32X3, DensePlan, operand_ld
 from .distillation import TopKDistillation
 from .gated import GatedMLP
 from .token_sampling import TokenSampler
@@ -28,13 +28,15 @@ _STATE_FLOATS = 9  # rl2_adam_prepare's optimizer state
 
 
 class _Weight:
-    """One weight matrix: fp32 parameters and gradient in the arenas, fp16 operand plane with padded rows."""
+    """One weight matrix: fp32 parameters and gradient in the arenas (rows padded to 16 bytes where ``aligned``, as the gated
+    block writes them), fp16 operand plane with padded rows."""
 
-    def __init__(self, out: int, inp: int, offset: int, plane_offset: int):
+    def __init__(self, out: int, inp: int, offset: int, plane_offset: int, aligned: bool):
         self.out, self.inp, self.offset, self.plane_offset, self.ld = out, inp, offset, plane_offset, operand_ld(inp, FP16)
+        self.arena_ld = operand_ld(inp, TF32X3) if aligned else inp
 
     def arena(self, flat: torch.Tensor) -> torch.Tensor:
-        return flat[self.offset:self.offset + self.out * self.inp].view(self.out, self.inp)
+        return flat[self.offset:self.offset + self.out * self.arena_ld].view(self.out, self.arena_ld)[:, :self.inp]
 
     def plane(self, flat: torch.Tensor) -> torch.Tensor:
         return flat[self.plane_offset:self.plane_offset + self.out * self.ld].view(self.out, self.ld)[:, :self.inp]
@@ -54,8 +56,8 @@ class TokenPolicy:
         self.weights: dict[str, _Weight] = {}
         for name, out, inp in (("in", hidden, observation_dim), ("gate", wide, hidden), ("up", wide, hidden),
                                ("down", hidden, wide), ("head", tokens, hidden)):
-            self.weights[name] = w = _Weight(out, inp, offset, plane)
-            offset += -(-out * inp // 4) * 4
+            self.weights[name] = w = _Weight(out, inp, offset, plane, name in ("gate", "up"))
+            offset += -(-out * w.arena_ld // 4) * 4
             plane += out * w.ld
         gen = torch.Generator().manual_seed(seed)
         host = torch.zeros(offset)
@@ -70,13 +72,14 @@ class TokenPolicy:
         self.health = torch.zeros(1, dtype=torch.int32, device=dev)
         self.opt_state = torch.zeros(_STATE_FLOATS, **f32)
         self.opt_state[6] = 65536.0
-        segments = [(w.offset + r * w.inp, -1, w.plane_offset + r * w.ld, w.inp, 0)
+        segments = [(w.offset + r * w.arena_ld, -1, w.plane_offset + r * w.ld, w.inp, 0)
                     for w in self.weights.values() for r in range(w.out)]
         self._segments, self._count, self._warp_segments = N.segment_table(segments, dev)
         # ---- buffers
         def half(cols):
             return torch.zeros(rows, operand_ld(cols, FP16), dtype=torch.float16, device=dev)
 
+        self.observation_dim, self.wide = observation_dim, wide
         self.obs, self._h0, self._h1, self._gated = half(observation_dim), half(hidden), half(hidden), half(wide)
         self._dh1, self._dgated, self._dx = half(hidden), half(wide), half(hidden)
         self._residual = torch.zeros(rows, hidden, **f32)
@@ -127,17 +130,17 @@ class TokenPolicy:
         """``dW (+)= dy^T x / loss scale``."""
         w = self.weights[name]
         return DensePlan(kind=FP16, m=w.out, n=w.inp, k=self.rows, a=dy, lda=dy.stride(0), a_major=1, b=x, ldb=x.stride(0),
-                         b_major=1, d=w.arena(self.grads), ldd=w.inp, accumulate=accumulate, scale=self.inverse_scale,
+                         b_major=1, d=w.arena(self.grads), ldd=w.arena_ld, accumulate=accumulate, scale=self.inverse_scale,
                          health=self.health)
 
     def _gated_weights(self):
         return dict(gate_weight=self.weights["gate"].plane(self.planes), up_weight=self.weights["up"].plane(self.planes))
 
     def _run_gated(self):
-        self.gated.forward(x=self._h0[:, :self.hidden], out=self._gated, health=self.health, **self._gated_weights())
+        self.gated.forward(x=self._h0[:, :self.hidden], out=self._gated[:, :self.wide], health=self.health, **self._gated_weights())
 
     def _run_gated_backward(self):
-        self.gated.backward(x=self._h0[:, :self.hidden], grad_out=self._dgated, grad_x=self._dx[:, :self.hidden],
+        self.gated.backward(x=self._h0[:, :self.hidden], grad_out=self._dgated[:, :self.wide], grad_x=self._dx[:, :self.hidden],
                             grad_gate=self.weights["gate"].arena(self.grads), grad_up=self.weights["up"].arena(self.grads),
                             grad_weight_scale=self.inverse_scale, found_inf=self.found_inf, health=self.health,
                             **self._gated_weights())
