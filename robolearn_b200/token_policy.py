@@ -172,7 +172,10 @@ class TokenPolicy:
 
     # ------------------------------------------------------------------ the policy
     def load_observations(self, obs: torch.Tensor) -> None:
-        self.obs[:, :obs.shape[1]].copy_(obs)
+        """The batch's observations [rows, observation_dim] (or one for all rows)."""
+        if obs.shape not in ((self.rows, self.observation_dim), (1, self.observation_dim)):
+            raise ValueError(f"observations must be of shape ({self.rows}, {self.observation_dim}), got {tuple(obs.shape)}")
+        self.obs[:, :self.observation_dim].copy_(obs)
 
     def forward(self) -> torch.Tensor:
         """Logits [rows, tokens] (fp32) of the loaded observations."""
