@@ -32,6 +32,36 @@ inline bool aligned(const void* p, std::size_t bytes) noexcept {
     return reinterpret_cast<std::uintptr_t>(p) % bytes == 0;
 }
 
+// Rows of `width` bytes, `stride` bytes apart (at least `width`).
+struct Extent {
+    const void* base;
+    long long rows, width, stride;
+};
+
+// Whether two matrices share a byte. Views side by side in one buffer (of one stride) do not.
+inline bool overlap(const Extent& a, const Extent& b) noexcept {
+    if (!a.base || !b.base || a.rows < 1 || b.rows < 1 || a.width < 1 || b.width < 1) return false;
+    const long long start = static_cast<long long>(reinterpret_cast<std::uintptr_t>(b.base) - reinterpret_cast<std::uintptr_t>(a.base));
+    if (start >= (a.rows - 1) * a.stride + a.width || start + (b.rows - 1) * b.stride + b.width <= 0) return false;
+    if (a.stride == b.stride) {
+        // rows i of a and j of b meet where (i - j) stride lies between start - a.width and start + b.width
+        const long long near = start / a.stride;
+        for (long long k = near - 1; k <= near + 1; ++k)
+            if (k > -b.rows && k < a.rows && k * a.stride > start - a.width && k * a.stride < start + b.width) return true;
+        return false;
+    }
+    for (long long i = 0, j = 0; i < a.rows && j < b.rows;) {
+        const long long at = i * a.stride, to = start + j * b.stride;
+        if (at + a.width <= to)
+            ++i;
+        else if (to + b.width <= at)
+            ++j;
+        else
+            return true;
+    }
+    return false;
+}
+
 inline cudaStream_t as_stream(void* s) noexcept { return reinterpret_cast<cudaStream_t>(s); }
 
 // Bounded spin limit for every device-side wait: a wait that runs out sets the

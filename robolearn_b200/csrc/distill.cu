@@ -1020,17 +1020,24 @@ extern "C" int rl2_distill_topk(const rl2_distill_args* a, void* stream) {
         set_error("distillation: logits, teacher values and indices and row_loss must be non-null");
         return -1;
     }
-    if (a->ld_logits < a->vocab || a->ld_values < a->top || a->ld_indices < a->top || (a->dlogits && a->ld_dlogits < a->vocab)) {
+    if (a->ld_logits < a->vocab || (a->dlogits && a->ld_dlogits < a->vocab)) {
+        set_error("distillation: a row stride is shorter than its row");
+        return -1;
+    }
+    auto extent = [&](const void* base, long long ld, int size) {
+        return Extent{base, a->rows, static_cast<long long>(a->vocab) * size, ld * size};
+    };
+    if (overlap(extent(a->logits, a->ld_logits, esize[a->logits_dtype]), extent(a->dlogits, a->ld_dlogits, esize[a->dlogits_dtype]))) {
+        set_error("distillation: the gradient may not overwrite the logits");
+        return -1;
+    }
+    if (a->ld_values < a->top || a->ld_indices < a->top) {
         set_error("distillation: a row stride is shorter than its row");
         return -1;
     }
     if (!aligned(a->logits, esize[a->logits_dtype]) || !aligned(a->teacher_values, esize[a->values_dtype]) ||
         !aligned(a->teacher_indices, a->index_bits / 8) || !aligned(a->dlogits, esize[a->dlogits_dtype])) {
         set_error("distillation: a matrix is not aligned to its element");
-        return -1;
-    }
-    if (a->dlogits == a->logits) {
-        set_error("distillation: the gradient may not overwrite the logits");
         return -1;
     }
     if (a->logits_dtype == 0) return launch_for<float>(*a, as_stream(stream));
