@@ -859,7 +859,9 @@ int rl2_peer_mean(long long count, const rl2_syncbn_exchange* ex, void* stream);
  * and its backward pass. x [rows][features], Wg and Wu [hidden][features], h
  * [rows][hidden], all of one 16-bit type with fp32 accumulation and one rounding of each
  * output. Rows contiguous; bases 16-byte aligned and row strides (in elements) multiples
- * of 16 bytes, as operand planes are; any extents.
+ * of 16 bytes, as operand planes are; any extents. An output shares no memory with what is
+ * still read when it is written, nor with another output (refused): of the backward's inputs
+ * it may be grad_out, or for a weight's gradient the weight.
  *
  * A plan is for up to `rows` rows and belongs to the device that was current at its
  * creation. dtype 0 = fp16, 1 = bf16; activation 0 = SiLU, 1 = GELU (the error-function

@@ -986,6 +986,16 @@ bool matrix_ok(const char* what, const void* base, long long ld, long long cols,
     return false;
 }
 
+// What of a call may not share memory: an output and what is still read, or written, when it is written.
+bool apart(const char* what, const Extent& out, std::initializer_list<Extent> others) {
+    for (const Extent& other : others)
+        if (overlap(out, other)) {
+            set_error("gated MLP: %s may not overlap the operands or another output", what);
+            return false;
+        }
+    return true;
+}
+
 typedef void (*KernelFn)(const Maps, const Params);
 
 int launched(cudaError_t e) {
@@ -1378,6 +1388,10 @@ extern "C" int rl2_gated_forward(void* opaque, const rl2_gated_forward_args* g, 
         !matrix_ok("up weight", g->up_weight, g->ld_up, plan->features, 2) ||
         !matrix_ok("output", g->out, g->ld_out, plan->hidden, 2))
         return -1;
+    const long long K = plan->features, F = plan->hidden;
+    if (!apart("output", {g->out, g->rows, F * 2, g->ld_out * 2},
+               {{g->x, g->rows, K * 2, g->ldx * 2}, {g->gate_weight, F, K * 2, g->ld_gate * 2}, {g->up_weight, F, K * 2, g->ld_up * 2}}))
+        return -1;
     if (g->rows <= kFewRows) {
         const FewArgs few{static_cast<const uint16_t*>(g->x), static_cast<const uint16_t*>(g->gate_weight),
                           static_cast<const uint16_t*>(g->up_weight), static_cast<uint16_t*>(g->out), g->ldx, g->ld_gate, g->ld_up,
@@ -1430,6 +1444,12 @@ extern "C" int rl2_gated_backward(void* opaque, const rl2_gated_backward_args* g
         set_error("gated MLP backward: grad_x may not be x (the weight gradients read x after it is written)");
         return -1;
     }
+    // grad_out is done with before any gradient is written, the weights before theirs
+    const Extent x{weights ? g->x : nullptr, g->rows, K * 2LL, g->ldx * 2}, dx{g->grad_x, g->rows, K * 2LL, g->ld_grad_x * 2};
+    const Extent gate{g->gate_weight, F, K * 2LL, g->ld_gate * 2}, up{g->up_weight, F, K * 2LL, g->ld_up * 2};
+    const Extent dgate{g->grad_gate, F, static_cast<long long>(K) * elem, g->ld_grad_gate * elem};
+    const Extent dup{g->grad_up, F, static_cast<long long>(K) * elem, g->ld_grad_up * elem};
+    if (!apart("grad_x", dx, {x, gate, up, dgate, dup}) || !apart("grad_gate", dgate, {x, dup}) || !apart("grad_up", dup, {x})) return -1;
     if (project(plan, g->rows, g->x, g->ldx, g->gate_weight, g->ld_gate, g->up_weight, g->ld_up, g->grad_out,
                 g->ld_grad_out, g->workspace, 0, g->found_inf, g->health, s))
         return -1;
