@@ -933,7 +933,7 @@ int rl2_gated_backward(void* plan, const rl2_gated_backward_args* args, void* st
  *   logits; row_loss = T^2 sum_k q_k (log q_k - log p[i_k]);
  *   *loss_out = loss_weight * sum_n w_n row_loss_n, rows added in a fixed order;
  *   dlogits_j = loss_weight w_n T (p_j - sum_{k: i_k = j} q_k) * *grad_scale, assigned.
- * teacher_values / teacher_indices [rows][top], 1 <= top <= 1024, any order; an index < 0
+ * teacher_values / teacher_indices [rows][top], 1 <= top <= 1024, vocab <= 2^30, any order; an index < 0
  * marks an absent entry, one >= vocab is left out and sets bit 8 of *health; a token may
  * appear more than once (its q add up). row_weight null: 1. A row of weight 0
  * (whatever its logits), without a teacher entry above -inf or without a logit above -inf has loss 0

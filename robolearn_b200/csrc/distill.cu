@@ -25,6 +25,7 @@ namespace rl2 {
 namespace distill {
 
 constexpr int kMaxTop = 1024;
+constexpr int kMaxVocab = 1 << 30;  // a column plus a grid's stride stays below 2^31
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
 
@@ -987,8 +988,8 @@ extern "C" int rl2_distill_topk(const rl2_distill_args* a, void* stream) {
         set_error("distillation: null arguments");
         return -1;
     }
-    if (a->rows < 0 || a->vocab < 1 || a->top < 1 || a->top > kMaxTop) {
-        set_error("distillation: rows >= 0, vocab >= 1 and 1..%d teacher entries are needed", kMaxTop);
+    if (a->rows < 0 || a->vocab < 1 || a->vocab > kMaxVocab || a->top < 1 || a->top > kMaxTop) {
+        set_error("distillation: rows >= 0, vocab >= 1 (up to 2^30) and 1..%d teacher entries are needed", kMaxTop);
         return -1;
     }
     const int esize[3] = {4, 2, 2};

@@ -9,6 +9,7 @@ import torch
 from . import _native as N
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+MAX_VOCAB = 1 << 30
 INDEX_BITS = {torch.int32: 32, torch.int64: 64}
 
 
@@ -17,8 +18,8 @@ class TopKDistillation:
     teacher entries a row. One call at a time per object (the calls share its counter)."""
 
     def __init__(self, rows: int, vocab: int, top: int, device="cuda"):
-        if rows < 1 or vocab < 1 or not 1 <= top <= 1024:
-            raise ValueError(f"rows and vocab must be positive and top 1..1024, got {rows}, {vocab}, {top}")
+        if rows < 1 or not 1 <= vocab <= MAX_VOCAB or not 1 <= top <= 1024:
+            raise ValueError(f"rows and vocab (up to {MAX_VOCAB}) must be positive and top 1..1024, got {rows}, {vocab}, {top}")
         self.rows, self.vocab, self.top = int(rows), int(vocab), int(top)
         self._lib = N.load()
         self.counter = torch.zeros(1, dtype=torch.int32, device=device)
