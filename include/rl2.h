@@ -942,7 +942,8 @@ int rl2_gated_backward(void* plan, const rl2_gated_backward_args* args, void* st
  * Types: 0 = fp32, 1 = fp16, 2 = bf16, each matrix its own; rows contiguous, any row stride
  * and alignment (16-byte aligned rows, or logits and gradient rows equally misaligned, are
  * fastest). dlogits, grad_scale (a device float: the loss scale of fp16 gradients),
- * row_weight, loss_out and health may be null. counter: one zero-initialised unsigned int
+ * row_weight, loss_out and health may be null. The temperature and its reciprocal are finite;
+ * what fp32 does not hold of (s - max) / T is infinite. counter: one zero-initialised unsigned int
  * that the kernel leaves at zero; calls that overlap need one each. Buffers and stream are
  * the current device's.
  * ------------------------------------------------------------------------- */

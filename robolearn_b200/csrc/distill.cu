@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <type_traits>
 
 namespace rl2 {
@@ -245,7 +246,7 @@ __device__ __forceinline__ void row_by_group(const rl2_distill_args& a, long lon
         q_s[k] = q;
     }
     loss = block_sum<THREADS>(loss, red);
-    if (tid == 0) a.row_loss[row] = some ? a.temperature * a.temperature * loss : 0.0f;
+    if (tid == 0) a.row_loss[row] = some ? a.temperature * (a.temperature * loss) : 0.0f;
     if (ds) {
         // gradient
         const float factor = weight * a.loss_weight * a.temperature * (a.grad_scale ? *a.grad_scale : 1.0f);
@@ -455,7 +456,7 @@ __device__ __forceinline__ void row_by_warp(const rl2_distill_args& a, long long
         if (first) ds[i] = narrow<G>(some ? exp2_fast(z) * p_factor - factor * all : 0.0f);
     }
     loss = warp_sum(loss);
-    if (lane == 0) a.row_loss[row] = some ? a.temperature * a.temperature * loss : 0.0f;
+    if (lane == 0) a.row_loss[row] = some ? a.temperature * (a.temperature * loss) : 0.0f;
     __syncwarp();  // q_s and i_s are the next row's
 }
 
@@ -884,7 +885,7 @@ __global__ void __launch_bounds__(T, kLongThreads / T) long_kernel(const rl2_dis
         __syncthreads();
         if (warp == 0) {
             loss = warp_sum(lane < kWarps ? sh.loss[lane] : 0.0f);
-            if (lane == 0) a.row_loss[row] = some ? a.temperature * a.temperature * loss : 0.0f;
+            if (lane == 0) a.row_loss[row] = some ? a.temperature * (a.temperature * loss) : 0.0f;
         }
     }
 }
@@ -1002,8 +1003,8 @@ extern "C" int rl2_distill_topk(const rl2_distill_args* a, void* stream) {
         set_error("distillation: teacher indices have 32 or 64 bits");
         return -1;
     }
-    if (!(a->temperature > 0.0f) || a->temperature > 1e30f) {
-        set_error("distillation: the temperature must be positive and finite");
+    if (!(a->temperature > 0.0f) || a->temperature > 1e30f || kLog2e / a->temperature > FLT_MAX) {
+        set_error("distillation: the temperature must be positive and finite, and so must its reciprocal");
         return -1;
     }
     if (a->loss_out && !a->counter) {

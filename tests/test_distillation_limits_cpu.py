@@ -1,4 +1,5 @@
-"""Limits of the distillation without a GPU: vocabularies whose column indexes would leave 32 bits. Every call is refused, by
+"""Limits of the distillation without a GPU: vocabularies whose column indexes would leave 32 bits, temperatures whose
+reciprocal leaves fp32. Every call is refused, by
 the limit or by a later check (a row stride of the teacher's values), so none reaches a launch."""
 
 import ctypes
@@ -21,3 +22,10 @@ def test_vocabulary(vocab):
     assert "2^30" in _refusal(vocab=vocab) and "shorter" in _refusal(vocab=1 << 30)
     with pytest.raises(ValueError, match="vocab"):
         TopKDistillation(1, vocab, 3)
+
+
+@pytest.mark.parametrize("temperature", [1e-45, 1e-39, 4e-39])
+def test_temperature(temperature):
+    assert "reciprocal" in _refusal(temperature=temperature)
+    for good in (4.3e-39, 1e-38, 1e-20, 1e30):
+        assert "shorter" in _refusal(temperature=good)
