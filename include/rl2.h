@@ -982,7 +982,10 @@ int rl2_distill_topk(const rl2_distill_args* args, void* stream);
  * in that order less than top_p of the top-k mass (the first token always; top_p >= 1: all;
  * <= 0: the first alone) and have e >= min_p. tokens[row] is the first index whose
  * cumulative w over the kept tokens exceeds floor(u W), W their sum; log_probs[row]
- * (optional) = log(w / W). Sums are exact integers: the result depends on the inputs alone.
+ * (optional) = log(w / W), the token's probability in this draw: of a token with e = 2^-24
+ * that may lie 0.002 from the logits' own, of one at 2^-30 0.4, and below 2^-31 none is drawn.
+ * log_probs_of_logits asks for the logits' own instead, (l - max) / T - log(W / 2^30) (0 at T = 0),
+ * as a learner computes it again. Sums are exact integers: the result depends on the inputs alone.
  * T = 0 (or below the smallest normal float) takes the first best token. NaN logits count as -inf, +inf as the largest float;
  * a row without a logit above -inf gives token -1 and log-probability -inf, and so does a
  * row whose own parameters are not valid (temperature negative or NaN, top_p NaN, min_p
@@ -1009,6 +1012,7 @@ typedef struct rl2_sample_args {
     int* tokens;
     float* log_probs;
     int* health;
+    int log_probs_of_logits;
 } rl2_sample_args;
 
 int rl2_sample_tokens(const rl2_sample_args* args, void* stream);

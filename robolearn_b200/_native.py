@@ -521,6 +521,7 @@ class SampleArgs(ctypes.Structure):
         ("rows", I), ("vocab", I), ("logits", P), ("ld_logits", LL), ("logits_dtype", I), ("uniforms", P),
         ("temperature", F), ("top_k", I), ("top_p", F), ("min_p", F), ("temperatures", P), ("top_ks", P),
         ("top_ps", P), ("min_ps", P), ("tokens", P), ("log_probs", P), ("health", P),
+        ("log_probs_of_logits", I),
     ]
 
 

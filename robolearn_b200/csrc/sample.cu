@@ -96,6 +96,24 @@ __device__ __forceinline__ float log_share(u64 w, u64 total) {
     return share > 0.5f ? log1pf(-static_cast<float>(total - w) / static_cast<float>(total)) : logf(share);
 }
 
+// The drawn token (weight w of `total` kept) and its log-probability: that of the draw, log(w / W), or the logits' own,
+// (l - max) / T - log sum e, where w's rounding to 2^-30 would show (a token at 2^-24 of the best: 0.002; the sum holds
+// the best token's 2^30 and is hardly touched). One thread.
+__device__ __forceinline__ void write_token(const rl2_sample_args& a, long long row, const Row& r, float best, int token, u64 w, u64 total) {
+    a.tokens[row] = token;
+    if (!a.log_probs) return;
+    if (!a.log_probs_of_logits) {
+        a.log_probs[row] = log_share(w, total);
+        return;
+    }
+    const long long at = row * a.ld_logits + token;
+    const float v = clean(a.logits_dtype == 0   ? static_cast<const float*>(a.logits)[at]
+                          : a.logits_dtype == 1 ? __half2float(static_cast<const __half*>(a.logits)[at])
+                                                : __bfloat162float(static_cast<const __nv_bfloat16*>(a.logits)[at]));
+    const u64 unit = 1ull << 30;
+    a.log_probs[row] = r.greedy ? 0.0f : (v - best) * r.inverse - log1pf(static_cast<float>(total - unit) * (1.0f / kUnit));
+}
+
 // ---- sums over a group of threads ------------------------------------------------
 
 struct Sum {
@@ -404,14 +422,17 @@ __global__ void __launch_bounds__(32 * kRowWarps) warp_kernel(const rl2_sample_a
         const u64 target = target_of(r.uniform, total);
         u64 cum = warp_scan64(sum);
         if (cum <= target && target < cum + sum) {
+            int chosen = 0;
+            uint32_t its = 0;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 if (cum <= target && target < cum + w[i]) {
-                    a.tokens[row] = lane * N + i;
-                    if (a.log_probs) a.log_probs[row] = log_share(w[i], total);
+                    chosen = lane * N + i;
+                    its = w[i];
                 }
                 cum += w[i];
             }
+            write_token(a, row, r, best, chosen, its, total);
         }
     }
 }
@@ -705,13 +726,12 @@ struct Few {
         }
         return hi;
     }
-    __device__ __forceinline__ void write(const rl2_sample_args& a, long long row, int chosen, u64 total) const {
+    __device__ __forceinline__ void write(const rl2_sample_args& a, long long row, const Row& r, float best, int chosen, u64 total) const {
+        uint32_t its = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (token[i] == chosen && w[i]) {
-                a.tokens[row] = chosen;
-                if (a.log_probs) a.log_probs[row] = log_share(w[i], total);
-            }
+            if (token[i] == chosen) its = w[i];
+        if (its) write_token(a, row, r, best, chosen, its, total);
     }
 };
 
@@ -747,7 +767,7 @@ __device__ __noinline__ void draw_few(Shared* sh, int n, const Row r, int vocab,
         total += few.w[i];
     }
     total = few.group.mass(total);
-    few.write(a, row, few.first_over(0, target_of(r.uniform, total), -1, vocab - 1), total);
+    few.write(a, row, r, best, few.first_over(0, target_of(r.uniform, total), -1, vocab - 1), total);
 }
 
 // A longer list: histograms of it (by value for the cuts, by index for the draw), one warp on the bin found.
@@ -901,10 +921,7 @@ __device__ __noinline__ void draw_many(Shared* sh, int n, const Row r, int vocab
         u64 cum = before;
         for (int k = 0; k < few; ++k)
             if (sh->few_index[k] < mine_index) cum += sh->few_w[k];
-        if (cum <= target && target < cum + sh->few_w[lane]) {
-            a.tokens[row] = mine_index;
-            if (a.log_probs) a.log_probs[row] = log_share(sh->few_w[lane], kept_all.mass);
-        }
+        if (cum <= target && target < cum + sh->few_w[lane]) write_token(a, row, r, best, mine_index, sh->few_w[lane], kept_all.mass);
         return;
     }
     int from = lo, to = hi;
@@ -918,12 +935,11 @@ __device__ __noinline__ void draw_many(Shared* sh, int n, const Row r, int vocab
         }
         (before + group.mass(m) > target ? to : from) = mid;
     }
+    uint32_t its = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-        if (token_of(i) == to && w[i]) {
-            a.tokens[row] = to;
-            if (a.log_probs) a.log_probs[row] = log_share(w[i], kept_all.mass);
-        }
+        if (token_of(i) == to) its = w[i];
+    if (its) write_token(a, row, r, best, to, its, kept_all.mass);
 }
 
 // ---- reading a row ------------------------------------------------------------------
@@ -1488,18 +1504,16 @@ __device__ __noinline__ void draw_wide(Work<L>& work, u64 given, const Found* kn
                 if (lane >= o) sum += up;
             }
             const uint32_t hit = __ballot_sync(0xffffffffu, cum + sum > target);
-            if (lane == __ffs(hit) - 1) {
-                a.tokens[row] = (chosen << shift) + i - in.mis;
-                if (a.log_probs) a.log_probs[row] = log_share(mine, total);
-            }
+            if (lane == __ffs(hit) - 1) write_token(a, row, r, best, (chosen << shift) + i - in.mis, mine, total);
             return;
         }
         cum += step;
     }
 }
 
+// The arguments are a grid constant: what is called here takes their address, which would put a copy on each thread's stack.
 template <typename L>
-__global__ void __launch_bounds__(kT, 2) row_kernel(const rl2_sample_args a, const int size, const int shift) {
+__global__ void __launch_bounds__(kT, 2) row_kernel(const __grid_constant__ rl2_sample_args a, const int size, const int shift) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared* sh = reinterpret_cast<Shared*>(raw);
     constexpr int kN = Work<L>::kN, kSlots = Work<L>::kSlots;

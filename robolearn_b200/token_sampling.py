@@ -26,10 +26,12 @@ class TokenSampler:
             self.device = torch.device("cuda", torch.cuda.current_device())
 
     def run(self, *, logits, uniforms, tokens, log_probs=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
-            health=None, stream=None) -> None:
+            log_probs_of_logits=False, health=None, stream=None) -> None:
         """``tokens`` (int32) and ``log_probs`` (float32, optional) of ``logits.shape[0]`` rows. Each of
         ``temperature``, ``top_k``, ``top_p`` and ``min_p`` is one number for all rows or a device tensor
-        with one value a row (float32; int32 for ``top_k``). Definition and special rows in include/rl2.h."""
+        with one value a row (float32; int32 for ``top_k``). ``log_probs`` are those of the draw, whose weights are
+        multiples of 2^-30 of the best token's; ``log_probs_of_logits``: the logits' own among the tokens kept, for a learner
+        that computes them again (they differ for tokens far below the best). Definition and special rows in include/rl2.h."""
         n, device = logits.shape[0], self.device
         if n > self.rows:
             raise ValueError(f"logits must be at most {self.rows} rows, got {n}")
@@ -38,6 +40,7 @@ class TokenSampler:
                          top_p=1.0, tokens=N.vector("tokens", tokens, n, torch.int32, device), health=N.ptr(health))
         if log_probs is not None:
             a.log_probs = N.vector("log_probs", log_probs, n, torch.float32, device)
+            a.log_probs_of_logits = int(log_probs_of_logits)
         for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
                                    ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
             if isinstance(value, torch.Tensor):
