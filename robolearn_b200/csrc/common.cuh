@@ -321,8 +321,10 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
 }
 
 // Every thread of both CTAs: release this CTA's prior memory operations to the cluster,
-// wait for the peer's.
+// wait for the peer's. The instructions are aligned: a warp's lanes, which may have come here by branches and returns of
+// their own, meet first.
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
