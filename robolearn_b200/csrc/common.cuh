@@ -333,9 +333,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
-// The same without publishing this thread's memory accesses, for a barrier that hands back a TMEM buffer whose loads
-// have completed (tcgen05.wait::ld). A release at cluster scope waits for every access of the thread that is under
-// way, bulk stores' reads of shared memory among them: 3000 cycles a tile in a product's epilogue.
+// The same without publishing this thread's memory accesses, for a barrier that hands back a TMEM buffer. Nothing has to be
+// published: what the next MMA may not overtake are the warp's reads of the buffer, and those are over, not only ordered.
+// tcgen05.wait::ld (aligned: all lanes in it) ends when the loads have put their values into registers, and the arriving
+// lane comes here through tcgen05.fence::before_thread_sync and a __syncwarp that every lane reaches after its own wait. The
+// MMA is issued by a thread that has seen the barrier's phase end, behind tcgen05.fence::after_thread_sync. A release at cluster
+// scope waits for every access of the thread that is under way, bulk stores' reads of shared memory among them: 3000
+// cycles a tile in a product's epilogue.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
