@@ -122,6 +122,12 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, int* hea
     }
 }
 
+// The same for all lanes of a warp: they go on together, and all or none of them. (After a wait that ran out, one lane may
+// see another role's abort word and the next the barrier's phase; what follows is for whole warps.)
+__device__ __forceinline__ bool wait_bar_warp(uint64_t* bar, uint32_t phase, int* health, volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, wait_bar(bar, phase, health, abort_flag));
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     if (BF16) {
@@ -407,9 +413,9 @@ __device__ __forceinline__ void drain(const Maps& maps, const Params& p, uint8_t
         const int buf = i & 1;
         const int row0 = w.m * 2 * kBM + rank * kBM + q * 32;
         const int col0 = w.n * p.tile_cols + slot * mine;
-        const bool ready = wait_bar(&acc_full[buf], (i >> 1) & 1, p.health, abort_flag);
+        const bool ready = wait_bar_warp(&acc_full[buf], (i >> 1) & 1, p.health, abort_flag);
         if (MODE == kGate) {  // the copy has landed before the CTA goes on (the next is not under way yet)
-            const bool in = wait_bar(in_bar, i & 1, p.health, nullptr);
+            const bool in = wait_bar_warp(in_bar, i & 1, p.health, nullptr);
             if (!in || !ready) break;
         } else if (!ready) {
             break;
@@ -820,7 +826,7 @@ __global__ void __launch_bounds__(kStripThreads, 1) strip_kernel(const __grid_co
         }
     } else {
         const int q = warp & 3;  // TMEM lanes 32 q .. + 31
-        const bool ready = wait_bar(&acc_full, 0, p.health, &abort_flag);
+        const bool ready = wait_bar_warp(&acc_full, 0, p.health, &abort_flag);
         ptx::tc_fence_after();
         float* sums = reinterpret_cast<float*>(smem);  // [row][lane]: the ring is done with
         for (int c = 0; c < p.n; c += 16) {
@@ -854,6 +860,7 @@ __global__ void __launch_bounds__(kStripThreads, 1) strip_kernel(const __grid_co
         }
     }
     __syncthreads();
+    __syncwarp();
     if (warp == 1) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem, 128);
