@@ -329,7 +329,7 @@ __device__ __forceinline__ void finish(const rl2_distill_args& a) {
 
 // Up to kFewTop teacher entries and 1024 tokens: a warp per row, N tokens a lane in registers (pairs 64 tokens apart),
 // read once; the exponentials of the sum are the gradient's. The row's loads and the teacher's are on their way
-// together. 26 us at 32768 x 101 fp32 (48 with the row read twice through L1), 9 us a call at 512 x 101.
+// together. 25 us at 32768 x 101 fp32 (48 with the row read twice through L1), 9 us a call at 512 x 101.
 constexpr int kRowWarps = 4;
 constexpr int kFewTop = 256;
 
@@ -498,8 +498,8 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const rl2_distill_args a) 
 // first. 1024 threads an SM, so that one row's reading goes along with another's writing: 512 a CTA for the longest rows
 // and for few of them, fewer for shorter ones, whose barriers and first loads weigh more (4096 x 4096 bf16: 77 us with
 // 512, 40 with 256, 26 with 128; 2048 x 50257 bf16: 104, 87, 98; 2047 x 128257 bf16: 214, 241). What bounds it is DRAM:
-// 1.05 GB in 214 us at 2047 x 128257 bf16 (4.9 TB/s; 227 in a row of calls on other inputs each); the second pass misses
-// L2 for 0.15 of the row. 246 us when it read forward and kept nothing.
+// 1.05 GB in 214 us at 2047 x 128257 bf16 (4.9 TB/s; 224 in a row of calls on other inputs each); the second pass misses
+// L2 for 0.12 of the row. 246 us when it read forward and kept nothing.
 // Slower there: rows held in registers by clusters of four CTAs (389 us), rows streamed through a ring in
 // shared memory by bulk copies (308 us), both waiting for one another at each row.
 //

@@ -32,11 +32,11 @@
 //
 // Two forms without these tiles, forward only: few_rows_kernel (up to 16 rows) and strip_kernel (up to 128).
 //
-// Measured: forward 65536 x 1024 x 4096 bf16 810 us (1360 TFLOP/s, the rate that the card sustains under its power
-// limit); backward 32768 x 1024 x 4096 bf16 1415 us (1165 TFLOP/s). At 8192 x 512 x 2048 fp16 the forward takes 26.8 us
-// (1280 TFLOP/s; a library product of its shape 28) and the backward 101: the projections again 39, dx 27, dW 34 (split
-// over rows, then summed). What bounds these is the way between L2 and the SMs: 295 MB in the forward (11 TB/s), 358 MB
-// where dh comes in and dg and du go out (27 us without the stores). Stores of dg and du in whole 4 KB pieces instead of
+// Measured: forward 65536 x 1024 x 4096 bf16 794 us (1385 TFLOP/s, the rate that the card sustains under its power
+// limit); backward 32768 x 1024 x 4096 bf16 1382 to 1429 us (1154 to 1193 TFLOP/s). At 8192 x 512 x 2048 fp16 the forward takes 29
+// us (a library product of its shape 35) and the backward 101: the projections again 40, dx 27, dW 34 (split over rows, then
+// summed). What bounds these is the way between L2 and the SMs: 313 MB in the forward, 449 MB where dh comes in and dg and du go
+// out, 10 to 11 TB/s (27 us without the stores). Stores of dg and du in whole 4 KB pieces instead of
 // tensor boxes change that by less than 1%.
 
 #include "common.cuh"

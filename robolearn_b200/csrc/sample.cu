@@ -18,8 +18,8 @@
 // in registers, v from a histogram. More tokens: a CTA, or with few rows a cluster of CTAs that each
 // read a part of the row, on a short list of candidates.
 //
-// Measured, a call among others: 8.7 us at 4096 x 256 fp32, top-p (16.4 with the cuts by halving the interval of
-// values, two warp reductions a step); 70 us at 256 x 131072 bf16, top-k 2000 (67 MB; 118 with the list's cuts by
+// Measured, a call among others: 8.5 us at 4096 x 256 fp32, top-p (16.4 with the cuts by halving the interval of
+// values, two warp reductions a step); 69 us at 256 x 131072 bf16, top-k 2000 (67 MB; 118 with the list's cuts by
 // halving); 22.5 us at 1 x 128257 fp32, top-k 50 and top-p.
 
 #include "common.cuh"
