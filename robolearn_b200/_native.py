@@ -334,6 +334,15 @@ def vector(name: str, t, n: int, dtype, device) -> int:
     return t.data_ptr()
 
 
+def health_word(t, device) -> int | None:
+    """Address of a health word: one int32 (or the first of several) on ``device``; anything else is refused."""
+    if t is None:
+        return None
+    if t.dtype.itemsize != 4 or t.dtype.is_floating_point or t.get_device() != device.index or t.numel() < 1:
+        raise ValueError(f"health must be an int32 on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
 class ReplayIngestArgs(ctypes.Structure):
     """``rl2_replay_ingest_args`` (include/rl2.h)."""
 

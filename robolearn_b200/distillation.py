@@ -45,7 +45,7 @@ class TopKDistillation:
         a = N.DistillArgs(n, self.vocab, self.top, *self._matrix("logits", logits, n, self.vocab, DTYPES),
                           *self._matrix("teacher_values", teacher_values, n, self.top, DTYPES),
                           *self._matrix("teacher_indices", teacher_indices, n, self.top, INDEX_BITS), temperature, None,
-                          loss_weight, counter=self._counter, health=N.ptr(health))
+                          loss_weight, counter=self._counter, health=N.health_word(health, self.device))
         if row_weight is not None:
             a.row_weight = self._vector("row_weight", row_weight, n)
         a.row_loss = self.row_loss.data_ptr() if row_loss is None else self._vector("row_loss", row_loss, n)

@@ -64,7 +64,7 @@ class GatedMLP:
         m = self._matrix
         a = N.GatedForwardArgs(rows, *m("x", x, rows, K), *m("gate_weight", gate_weight, F, K),
                                *m("up_weight", up_weight, F, K), *m("out", out, rows, F),
-                               None if health is None else health.data_ptr())
+                               N.health_word(health, self.device))
         N.check(self._lib.rl2_gated_forward(self.handle, ctypes.byref(a), N.raw_stream(stream, self.device.index)),
                 "gated MLP forward")
 
@@ -79,7 +79,7 @@ class GatedMLP:
         if (grad_gate is None) != (grad_up is None):
             raise ValueError("grad_gate and grad_up come together")
         a = N.GatedBackwardArgs(rows, *m("x", x, rows, K), *m("gate_weight", gate_weight, F, K),
-                                *m("up_weight", up_weight, F, K), *m("grad_out", grad_out, rows, F), health=N.ptr(health),
+                                *m("up_weight", up_weight, F, K), *m("grad_out", grad_out, rows, F), health=N.health_word(health, self.device),
                                 workspace=self.workspace().data_ptr())
         if grad_x is not None:
             a.grad_x, a.ld_grad_x = m("grad_x", grad_x, rows, K)

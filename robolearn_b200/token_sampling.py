@@ -37,7 +37,7 @@ class TokenSampler:
             raise ValueError(f"logits must be at most {self.rows} rows, got {n}")
         address, ld = N.matrix("logits", logits, n, self.vocab, DTYPES, device)
         a = N.SampleArgs(n, self.vocab, address, ld, DTYPES[logits.dtype], N.vector("uniforms", uniforms, n, torch.float32, device),
-                         top_p=1.0, tokens=N.vector("tokens", tokens, n, torch.int32, device), health=N.ptr(health))
+                         top_p=1.0, tokens=N.vector("tokens", tokens, n, torch.int32, device), health=N.health_word(health, device))
         if log_probs is not None:
             a.log_probs = N.vector("log_probs", log_probs, n, torch.float32, device)
             a.log_probs_of_logits = int(log_probs_of_logits)
